@@ -213,6 +213,46 @@ B2_API int b2_repeat_kv(const void* input, void* output, int64_t n_kv_heads,
                         int64_t elem_bytes, void* stream);
 
 /*
+ * Page table and slot map of one step of a paged cache, on the GPU from the
+ * request lengths (no counterpart in the reference, whose host fills both).
+ * Request b holds context_lens[b] tokens and gets new_lens[b] more (int32 [B];
+ * negative counts as 0).  In one launch:
+ *   page_table int32 [B, max_pages] (rows table_stride apart): the pages that
+ *     the new tokens open are taken from free_pages (int32 [n_free]) in request
+ *     order and written behind the pages the request holds; other entries stay.
+ *   slots int64 [max_tokens]: page * page_size + offset of each new token, the
+ *     requests' tokens one after another; -1 behind the last one, for a token
+ *     whose page lies behind max_pages and for one that found no free page
+ *     (its table entry is -1 as well).  max_tokens has to be at least the sum
+ *     of new_lens (< 2^31): tokens behind it are dropped, with the pages that
+ *     they would open.
+ *   offsets int32 [B + 1]: first token of each request; offsets[B] = the sum.
+ *   pages_used int32 [1]: pages wanted from free_pages (> n_free: too few).
+ */
+B2_API int b2_build_page_table(const int32_t* context_lens, const int32_t* new_lens,
+                               const int32_t* free_pages, int32_t* page_table,
+                               int64_t* slots, int32_t* offsets, int32_t* pages_used,
+                               int64_t B, int64_t page_size, int64_t n_free,
+                               int64_t max_pages, int64_t table_stride,
+                               int64_t max_tokens, void* stream);
+
+/*
+ * New K/V rows into a paged cache by slot: k / v [N, Hkv, D] (element strides
+ * row, head) to k_pages / v_pages [n_pages, page_size, Hkv, D] (element strides
+ * page, token, head), row r to slot slots[r] (int64).  Slots outside
+ * [0, n_pages * page_size) are passed over.  A slot may occur once: which of
+ * several rows with one slot stays is not defined.  Rows and cache share one
+ * dtype, or fp32 rows are rounded to nearest into an fp16 / bf16 cache.  A
+ * contiguous cache [B, Hkv, S, D] is pages of size S: strides (b, s, h).
+ */
+B2_API int b2_store_kv(const void* k, const void* v, void* k_pages, void* v_pages,
+                       const int64_t* slots, int64_t N, int64_t Hkv, int64_t D,
+                       int64_t n_pages, int64_t page_size, const int64_t* k_strides,
+                       const int64_t* v_strides, const int64_t* kp_strides,
+                       const int64_t* vp_strides, int src_dtype, int dst_dtype,
+                       void* stream);
+
+/*
  * KDA (chunked gated delta rule) forward.  No reference counterpart: the
  * reference has no KDA code.  Layout [B, T, H, D] contiguous:
  *   q, k, v : dtype (B2_BF16) [B,T,H,Dk|Dv];  g : fp32 [B,T,H,Dk] log-decay

@@ -39,6 +39,9 @@ SIGNATURES = {
     "b2_decode_attn": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
                               _pi64, _pi64, _vp, _i64, _vp, _f32, _i32, _i32, _vp]),
     "b2_repeat_kv": (_i32, [_vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp]),
+    "b2_build_page_table": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _vp]),
+    "b2_store_kv": (_i32, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _pi64, _pi64, _pi64, _pi64,
+                           _i32, _i32, _vp]),
     "b2_kda_workspace_size": (ctypes.c_size_t, [_i64, _i64, _i64, _i64, _i64, _i64]),
     "b2_kda_fwd_noalloc": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
                                   _i64, _i64, _i64, _i64, _i64, _i64, _f32, _i32, _vp]),
@@ -127,6 +130,35 @@ def fast():
             except ImportError:
                 pass
     return _fast
+
+
+def check_device(ref, **tensors):
+    """Every tensor of a call lies on the device of ``ref`` (a CUDA device):
+    the kernels follow raw pointers."""
+    from .errors import B2ShapeError
+    if not ref.is_cuda:
+        raise B2ShapeError("b200kern ops take CUDA tensors (there is no CPU path)")
+    for name, t in tensors.items():
+        if t is not None and t.device != ref.device:
+            raise B2ShapeError(f"{name} is on {t.device}, not on {ref.device}")
+
+
+class on_device:
+    """Makes a tensor's device current around a launch (its current stream is
+    then the one the caller set for that device).  Does nothing where it is
+    current already."""
+
+    def __init__(self, t):
+        self.ctx = torch.cuda.device(t.device) if t.device.index != torch.cuda.current_device() else None
+
+    def __enter__(self):
+        if self.ctx is not None:
+            self.ctx.__enter__()
+
+    def __exit__(self, *exc):
+        if self.ctx is not None:
+            self.ctx.__exit__(*exc)
+        return False
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
