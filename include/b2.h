@@ -213,6 +213,39 @@ B2_API int b2_repeat_kv(const void* input, void* output, int64_t n_kv_heads,
                         int64_t elem_bytes, void* stream);
 
 /*
+ * Attention of a tree of drafted tokens over a KV cache (speculative
+ * decoding; no counterpart in the reference).  Request b has context_lens[b]
+ * tokens in the cache, then its drafted tokens, whose K/V stand behind them at
+ * positions context_lens[b] + j, j < draft_lens[b] (NULL: T for every request).
+ *   q [B, T, Hq, D] and o like it, element strides (b, t, h).
+ *   K/V contiguous [B, Hkv, S, D] (strides b, h, s; page_size 0, max_keys = S)
+ *   or paged [n_pages, page_size, Hkv, D] (strides page, token, head) with
+ *   page_table int32 [B, max_pages] (max_keys = max_pages * page_size), as in
+ *   b2_decode_attn.  A page number outside [0, n_pages) reads as zeros and is
+ *   recorded in the device error word (b2_device_error).
+ *   tree_mask uint8 [T, T] (mask_stride 0) or [B, T, T] (mask_stride T * T):
+ *   drafted token t sees drafted token j iff tree_mask[t, j] != 0; every
+ *   drafted token sees the whole context.
+ *   scores: s = scale q.k; softcap > 0: s = softcap tanh(s / softcap).
+ * Rows t >= draft_lens[b] and rows that see nothing give 0.  Lengths are
+ * clamped to the cache.  workspace: b2_tree_attn_workspace_size(...) bytes
+ * (may be NULL when it is 0), 16-byte aligned; one per call in flight.
+ */
+B2_API size_t b2_tree_attn_workspace_size(int64_t B, int64_t T, int64_t Hq, int64_t Hkv,
+                                          int64_t D, int64_t max_keys, int q_dtype,
+                                          int kv_dtype);
+B2_API int b2_tree_attn(const void* q, const void* k, const void* v, void* o,
+                        const int32_t* page_table, const int32_t* context_lens,
+                        const int32_t* draft_lens, const uint8_t* tree_mask,
+                        int64_t mask_stride, void* workspace, int64_t B, int64_t T,
+                        int64_t Hq, int64_t Hkv, int64_t D, int64_t max_keys,
+                        int64_t page_size, int64_t max_pages, int64_t n_pages,
+                        const int64_t* q_strides, const int64_t* k_strides,
+                        const int64_t* v_strides, const int64_t* o_strides,
+                        float scale, float softcap, int q_dtype, int kv_dtype,
+                        void* stream);
+
+/*
  * Page table and slot map of one step of a paged cache, on the GPU from the
  * request lengths (no counterpart in the reference, whose host fills both).
  * Request b holds context_lens[b] tokens and gets new_lens[b] more (int32 [B];

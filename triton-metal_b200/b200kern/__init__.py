@@ -10,7 +10,7 @@ from .quant import (int4_matmul, int8_matmul, int4_dequant, gemm_bf16, pack_int4
                     unpack_int4_gptq, pack_int4_ref)
 from .attention import (flash_attention, flash_attention_template, gqa_attention, decode_attention,
                         kv_cache_attention, batched_kv_decode, paged_attention, sliding_window_attention,
-                        rope_attention, repeat_kv)
+                        rope_attention, repeat_kv, tree_attention)
 from .paged import build_page_table, store_kv
 from .kda import kda_chunk_fwd
 from . import _lib
@@ -19,7 +19,7 @@ __all__ = [
     "int4_matmul", "int8_matmul", "gemm_bf16", "flash_attention", "flash_attention_template",
     "gqa_attention", "decode_attention", "kv_cache_attention", "batched_kv_decode",
     "paged_attention", "sliding_window_attention", "rope_attention", "repeat_kv",
-    "build_page_table", "store_kv", "kda_chunk_fwd", "int4_dequant", "pack_int4_gptq", "unpack_int4_gptq",
+    "tree_attention", "build_page_table", "store_kv", "kda_chunk_fwd", "int4_dequant", "pack_int4_gptq", "unpack_int4_gptq",
     "pack_int4_ref", "B2Error", "B2ShapeError", "B2DtypeError", "B2AlignmentError",
     "B2UnsupportedError", "B2LaunchError", "B2TimeoutError", "load_library",
 ]

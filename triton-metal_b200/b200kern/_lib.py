@@ -39,6 +39,9 @@ SIGNATURES = {
     "b2_decode_attn": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
                               _pi64, _pi64, _vp, _i64, _vp, _f32, _i32, _i32, _vp]),
     "b2_repeat_kv": (_i32, [_vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp]),
+    "b2_tree_attn_workspace_size": (ctypes.c_size_t, [_i64, _i64, _i64, _i64, _i64, _i64, _i32, _i32]),
+    "b2_tree_attn": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _i64, _i64,
+                            _i64, _i64, _i64, _pi64, _pi64, _pi64, _pi64, _f32, _f32, _i32, _i32, _vp]),
     "b2_build_page_table": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _vp]),
     "b2_store_kv": (_i32, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _pi64, _pi64, _pi64, _pi64,
                            _i32, _i32, _vp]),

@@ -161,6 +161,80 @@ def decode_attention(q, k_cache, v_cache, seq_lens, scale=None, page_table=None,
     return o
 
 
+def tree_attention(q, k_cache, v_cache, context_lens, tree_mask, draft_lens=None, scale=None, page_table=None,
+                   softcap=0.0, out=None):
+    """Attention of a tree of drafted tokens over a KV cache (speculative decoding).
+
+    q [B, T, Hq, D] (any strides, last dim contiguous): T drafted tokens of each
+    request.  Request b has context_lens[b] tokens in the cache; the K/V of its
+    drafted tokens stand behind them, at positions context_lens[b] + j (store_kv
+    writes them there).  tree_mask bool or uint8 [T, T] or [B, T, T]: token t
+    sees drafted token j iff tree_mask[..., t, j]; all of them see the context.
+    draft_lens int32 [B]: requests with fewer than T drafted tokens (the rest
+    is padding).  Caches as in decode_attention: [B, Hkv, S, D], or
+    [n_pages, page_size, Hkv, D] with page_table int32 [B, max_pages]; GQA: kv
+    head = q head // (Hq // Hkv).  softcap > 0 caps the scores:
+    softcap * tanh(scale q.k / softcap).
+
+    Returns o [B, T, Hq, D] of q's dtype; rows behind a request's drafted
+    tokens and rows that see nothing are 0.  Lengths are clamped to the cache;
+    a page number outside the cache reads as zeros and shows in
+    b2_device_error.  Hidden keys do not count, whatever their values.
+    """
+    if q.dim() != 4 or k_cache.dim() != 4 or k_cache.shape != v_cache.shape:
+        raise B2ShapeError("tree_attention takes q [B, T, Hq, D] and two 4-d caches of one shape")
+    if q.dtype not in _DT or k_cache.dtype not in _DT or v_cache.dtype != k_cache.dtype:
+        raise B2DtypeError("q and the cache must be fp32, fp16 or bf16")
+    B, T, Hq, D = q.shape
+    if k_cache.shape[3] != D:
+        raise B2ShapeError(f"cache head dim {k_cache.shape[3]} != {D}")
+    if page_table is None:
+        if k_cache.shape[0] != B:
+            raise B2ShapeError("a contiguous cache must be [B, Hkv, S, D]")
+        Hkv, keys, ps, max_pages = k_cache.shape[1], k_cache.shape[2], 0, 0
+    else:
+        if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] != B:
+            raise B2ShapeError("page_table must be int32 [B, max_pages]")
+        page_table = page_table.contiguous()
+        ps, Hkv, max_pages = k_cache.shape[1], k_cache.shape[2], page_table.shape[1]
+        keys = ps * max_pages
+        if keys == 0:  # nothing cached anywhere
+            page_table, k_cache, v_cache, ps = None, k_cache[:0, :0], v_cache[:0, :0], 0
+    if Hkv == 0 or Hq % Hkv:
+        raise B2ShapeError(f"Hq={Hq} must be a multiple of Hkv={Hkv}")
+    if tree_mask.dtype not in (torch.bool, torch.uint8) or tuple(tree_mask.shape) not in ((T, T), (B, T, T)):
+        raise B2ShapeError(f"tree_mask must be bool or uint8 [{T}, {T}] or [{B}, {T}, {T}]")
+    if softcap < 0 or not math.isfinite(softcap):
+        raise B2ShapeError("softcap must be a finite number >= 0")
+    for name, t in (("context_lens", context_lens), ("draft_lens", draft_lens)):
+        if t is not None and (t.dtype != torch.int32 or tuple(t.shape) != (B,)):
+            raise B2ShapeError(f"{name} must be int32 [{B}]")
+    _lib.check_device(q, k_cache=k_cache, v_cache=v_cache, context_lens=context_lens, tree_mask=tree_mask,
+                      draft_lens=draft_lens, page_table=page_table, out=out)
+    context_lens = context_lens.contiguous()
+    draft_lens = None if draft_lens is None else draft_lens.contiguous()
+    tree_mask = tree_mask.contiguous()
+    mask_stride = T * T if tree_mask.dim() == 3 else 0
+    q, k_cache, v_cache = (t if t.stride(3) == 1 else t.contiguous() for t in (q, k_cache, v_cache))
+    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
+    with _lib.on_device(q):
+        o = (_lib.check_out(out, (B, T, Hq, D), q.dtype, "tree_attention") if out is not None
+             else torch.empty(B, T, Hq, D, dtype=q.dtype, device=q.device))
+        if o.numel() == 0:
+            return o
+        qd, kd = _DT[q.dtype], _DT[k_cache.dtype]
+        need = int(_lib.fn("b2_tree_attn_workspace_size")(B, T, Hq, Hkv, D, keys, qd, kd))
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+        _lib.call("b2_tree_attn", q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), o.data_ptr(),
+                  None if page_table is None else page_table.data_ptr(), context_lens.data_ptr(),
+                  None if draft_lens is None else draft_lens.data_ptr(), tree_mask.data_ptr(), mask_stride,
+                  None if ws is None else ws.data_ptr(), B, T, Hq, Hkv, D, keys, ps, max_pages, k_cache.shape[0],
+                  _lib.strides_arg(q.stride()[:3]), _lib.strides_arg(k_cache.stride()[:3]),
+                  _lib.strides_arg(v_cache.stride()[:3]), _lib.strides_arg(o.stride()[:3]), scale, float(softcap),
+                  qd, kd, _stream())
+    return o
+
+
 def sliding_window_attention(Q, K_cache, V_cache, q_pos, seq_len, window_size, scale=None):
     """Reference sliding_window_attention (_msl_templates.py:3335-3431):
     Q [D] (or [H, D]), caches [S, D] (or [H, S, D]); keys
