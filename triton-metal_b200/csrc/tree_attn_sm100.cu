@@ -1,13 +1,896 @@
-// Attention of a tree of drafted tokens over a contiguous or paged KV cache.
+// Attention of a tree of drafted tokens over a contiguous or paged KV cache
+// (speculative decoding), sm_100a.
+//
+//   s = scale q.k  (softcap: s = cap tanh(s / cap)),  o = softmax(s | mask) v
+//
+// The rows of one (request, kv head) are its T drafted tokens times the
+// Hq / Hkv query heads: row r = t * rep + hh.  Each K/V row is needed by all of
+// them, so the cache is the traffic: with D = 128 and 16-bit values a key costs
+// 512 bytes and 512 FLOPs a row, which meets the HBM rate at ~250 rows.  Up to
+// there the copy stream sets the time, and the tensor cores have to keep up
+// with it at any number of rows, which 128-row tcgen05 tiles do.
+//
+// One persistent CTA per SM.  Work is cut in 128-key tiles; the tiles of all
+// (request, kv head, row tile) items stand in one line and every CTA takes an
+// equal run of it, whatever the requests' lengths (they are on the GPU only).
+// A run is a few segments, each inside one item; a segment that is not a whole
+// item leaves (m, l, unnormalised o) in the workspace, and a second kernel
+// joins those.
+//   warps 0-3   copy K, V and Q tiles with 16-byte cp.async into 128B-swizzled
+//               tiles (any page size and stride, zeros behind the last key), a
+//               ring of kRing tiles in the order K0 K1 V0 K2 V1 ...
+//   warps 4-11  two softmax warpgroups, one row per thread (TMEM lane = row)
+//   warp 12     TMEM owner and MMA issuer
+// TMEM as in the prefill kernel: unit u has S_u / P_u at column 256u and O_u at
+// 256u + 128.  With one row tile per item (SINGLE) the two units take the even
+// and the odd key tiles of the same rows, so that one unit's softmax runs under
+// the other's MMAs, and their (m, l, O) are joined from TMEM at the segment's
+// end; with more row tiles (PAIR) the units are two row tiles that share every
+// K/V tile.
 #include "attn_common.cuh"
+#include "fa_common.cuh"
 #include <math.h>
 
+namespace b2 {
+namespace tree {
+
+using namespace fa;
+
+constexpr int kThreads = 416;
+constexpr int BR = 128, BK = 128;          // rows and keys of a tile
+constexpr float kRescale = 8.f;            // log2 units: P holds up to 2^8
+
+template <int HD>
+struct Cfg {
+  static constexpr int kAtom = 128 * 128;             // 128 rows x 128 bytes
+  static constexpr int kTile = HD / 64 * kAtom;
+  static constexpr int kRing = HD == 128 ? 5 : 10;    // 160 KB of K and V tiles
+  // tiles a copying thread leaves in flight behind the one it hands over
+  static constexpr int kLag = HD == 128 ? 2 : 4;
+  static constexpr int kHead = 3072;                  // barriers and the (m, l) exchange
+  static constexpr int kSmem = kHead + (2 + kRing) * kTile;
+  static_assert(kSmem <= 232448, "shared memory");
+  static_assert(kLag < kRing, "a ring slot is handed over before it is waited for again");
+};
+
+struct Params {
+  const uint16_t *q, *k, *v;
+  uint16_t* o;
+  const int32_t *page_table, *ctx, *draft;
+  const uint8_t* mask;
+  float* ws;
+  int64_t mask_stride, n_pages;
+  int64_t qs[3], os[3], ks[3], vs[3];
+  int B, T, Hkv, rep, R, cap;   // R = T * rep rows; cap: keys a cache row holds
+  int n_rt;                     // row tiles (PAIR: pairs of them) of an item
+  uint32_t page_size;           // 0: contiguous
+  int max_pages;
+  float scale_log2;             // scale * log2 e
+  float cap_log2, cap_in;       // softcap * log2 e; 2 log2 e * scale / softcap
+  unsigned* err;
+};
+
+// ------------------------------------------------------------- schedule
+// Items of request b: hk-major, then row tile.  A row tile with drafted tokens
+// has all of the request's key tiles, one without has a single tile in which
+// nothing is visible (its rows become 0).
+struct Req {
+  int ctx, dl, tiles, full;  // key tiles, row tiles with drafted tokens
+  int per_head;              // tiles of one kv head
+};
+__device__ __forceinline__ Req request(const Params& p, int b, int rows_per_item) {
+  Req r;
+  attn::tree_lens(p.ctx, p.draft, b, p.T, p.cap, r.ctx, r.dl);
+  r.tiles = (r.ctx + r.dl + BK - 1) / BK;
+  r.full = (r.dl * p.rep + rows_per_item - 1) / rows_per_item;
+  r.per_head = r.full * r.tiles + (p.n_rt - r.full);
+  return r;
+}
+
+struct Segment {
+  int b, hk, rt, tile, n, of;  // n tiles from `tile` on, of an item with `of` tiles
+  int ctx, dl, keys;           // keys = ctx + dl, 0 when the item has no drafted token
+};
+
+// Walks the segments of the run [g, g1).
+struct Walk {
+  int64_t g, g1, start;  // start: first tile of request b
+  int b;
+  Req r;
+  __device__ __forceinline__ bool next(const Params& p, int rows_per_item, Segment& s) {
+    if (g >= g1) return false;
+    while (g >= start + (int64_t)r.per_head * p.Hkv) {
+      start += (int64_t)r.per_head * p.Hkv;
+      r = request(p, ++b, rows_per_item);
+    }
+    const uint32_t local = (uint32_t)(g - start);
+    s.b = b;
+    s.hk = local / (uint32_t)r.per_head;
+    const int rem = local - (uint32_t)s.hk * r.per_head;
+    const bool has = rem < r.full * r.tiles;
+    s.rt = has ? rem / r.tiles : r.full + rem - r.full * r.tiles;
+    s.tile = has ? rem - s.rt * r.tiles : 0;
+    s.of = has ? r.tiles : 1;
+    s.n = (int)min((int64_t)(s.of - s.tile), g1 - g);
+    s.ctx = r.ctx;
+    s.dl = has ? r.dl : 0;
+    s.keys = has ? r.ctx + r.dl : 0;
+    g += s.n;
+    return true;
+  }
+};
+
+// First tile of CTA c's run when G CTAs share W tiles (G <= W, so that no run
+// is empty).
+__device__ __forceinline__ int64_t run_start(int64_t c, int64_t W, int64_t G) { return c * W / G; }
+
+__device__ __forceinline__ int64_t warp_sum(int64_t x) {
+#pragma unroll
+  for (int off = 16; off; off >>= 1) x += __shfl_xor_sync(0xffffffffu, x, off);
+  return x;
+}
+
+// ------------------------------------------------------------- softmax
+// Row max of the raw scores of this thread's row, hidden keys left out.
+template <bool MASK>
+__device__ __forceinline__ float row_max_bits(uint32_t tS, const uint32_t (&vis)[4]) {
+  float mx = -INFINITY;
+#pragma unroll 1
+  for (int c = 0; c < 4; c += 2) {
+    uint32_t sv[64];
+    tc::tmem_ld_32x32b_x32(tS + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(sv));
+    tc::tmem_ld_32x32b_x32(tS + 32 * c + 32, *reinterpret_cast<uint32_t(*)[32]>(sv + 32));
+    tc::tmem_ld_wait();
+    const uint32_t w0 = c ? vis[2] : vis[0], w1 = c ? vis[3] : vis[1];
+#pragma unroll
+    for (int e = 0; e < 64; e += 2) {
+      float v0 = __uint_as_float(sv[e]), v1 = __uint_as_float(sv[e + 1]);
+      if constexpr (MASK) {
+        const uint32_t w = e < 32 ? w0 : w1;
+        if (!(w >> (e & 31) & 1)) v0 = -INFINITY;
+        if (!(w >> ((e + 1) & 31) & 1)) v1 = -INFINITY;
+      }
+      mx = max3(mx, v0, v1);
+    }
+  }
+  return mx;
+}
+
+__device__ __forceinline__ float rcp_approx(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// cap tanh(scale s / cap) - m in log2 units: tanh y = 1 - 2 / (1 + e^2y), good
+// to ~2e-7 (the one-instruction tanh is good to 2^-11, which a cap of 50 turns
+// into 0.02 in the exponent)
+__device__ __forceinline__ float capped(float s, float cap_in, float cap_log2, float m) {
+  return fmaf(-2.f * cap_log2, rcp_approx(1.f + ex2(s * cap_in)), cap_log2 - m);
+}
+
+// p = exp2(score - m) as 16-bit pairs over the S columns; returns their sum.
+// P rounded to 16 bits (half a step of its own size) is what the MMA takes; the
+// sum l is taken before that, in 32 bits.
+template <bool MASK, int FMT, bool CAP>
+__device__ __forceinline__ float exp_to_p_bits(uint32_t tS, const uint32_t (&vis)[4], float mref, const Params& p) {
+  uint64_t rs = 0;
+  const uint64_t sc2 = f2_pack(p.scale_log2, p.scale_log2), nm2 = f2_pack(-mref, -mref);
+#pragma unroll 1
+  for (int c = 0; c < 4; c += 2) {
+    uint32_t sv[64];
+    tc::tmem_ld_32x32b_x32(tS + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(sv));
+    tc::tmem_ld_32x32b_x32(tS + 32 * c + 32, *reinterpret_cast<uint32_t(*)[32]>(sv + 32));
+    tc::tmem_ld_wait();
+    const uint32_t w0 = c ? vis[2] : vis[0], w1 = c ? vis[3] : vis[1];
+    uint32_t pk[32];
+#pragma unroll
+    for (int e = 0; e < 32; ++e) {
+      float p0, p1;
+      uint64_t x;
+      if constexpr (CAP) {
+        x = f2_pack(capped(__uint_as_float(sv[2 * e]), p.cap_in, p.cap_log2, mref),
+                    capped(__uint_as_float(sv[2 * e + 1]), p.cap_in, p.cap_log2, mref));
+      } else {
+        x = fma_f2((uint64_t)sv[2 * e] | ((uint64_t)sv[2 * e + 1] << 32), sc2, nm2);
+      }
+      if (e % 3 == 2) {  // a third of the exponentials on the FMA pipe, as in the prefill kernel
+        const uint64_t y = exp2_poly_f2(x);
+        p0 = f2_lo(y);
+        p1 = f2_hi(y);
+      } else {
+        p0 = ex2(f2_lo(x));
+        p1 = ex2(f2_hi(x));
+      }
+      if constexpr (MASK) {
+        const uint32_t w = e < 16 ? w0 : w1;
+        if (!(w >> ((2 * e) & 31) & 1)) p0 = 0.f;
+        if (!(w >> ((2 * e + 1) & 31) & 1)) p1 = 0.f;
+      }
+      rs = add_f2(rs, f2_pack(p0, p1));
+      if constexpr (FMT == kF16) {
+        __half2 hv = __floats2half2_rn(p0, p1);
+        pk[e] = *reinterpret_cast<uint32_t*>(&hv);
+      } else {
+        __nv_bfloat162 hv = __floats2bfloat162_rn(p0, p1);
+        pk[e] = *reinterpret_cast<uint32_t*>(&hv);
+      }
+    }
+    tmem_st_32x32b_x32(tS + 16 * c, pk);
+  }
+  return f2_lo(rs) + f2_hi(rs);
+}
+
+// Visible keys of this thread's row among the 128 from kv0 on, as bits.  The
+// warp reads its tokens' mask rows together (lane = key) and every lane keeps
+// the ballots of its own token.
+__device__ __forceinline__ void visible_bits(uint32_t (&vis)[4], const uint8_t* mask, int T, int t, int t0, int t1,
+                                             int kv0, int ctx, int dl, bool row_ok) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) vis[w] = 0;
+  for (int tt = t0; tt <= t1; ++tt) {
+    const uint8_t* row = mask + (int64_t)tt * T;
+    bool see[4];
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const int j = kv0 + 32 * w + lane - ctx;
+      see[w] = j < 0 || (j < dl && row[j] != 0);
+    }
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const uint32_t bits = __ballot_sync(0xffffffffu, see[w]);
+      if (tt == t) vis[w] = bits;
+    }
+  }
+  if (!row_ok) vis[0] = vis[1] = vis[2] = vis[3] = 0;
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// sum of a flag over the 256 softmax threads: a barrier and a vote in one, so
+// that all of them leave together
+__device__ __forceinline__ bool any_of_softmax(bool x) {
+  uint32_t r;
+  asm volatile(
+      "{\n .reg .pred p, q;\n setp.ne.b32 p, %1, 0;\n barrier.cta.red.or.pred q, 1, 256, p;\n selp.u32 %0, 1, 0, q;\n}"
+      : "=r"(r)
+      : "r"((uint32_t)x)
+      : "memory");
+  return r != 0;
+}
+__device__ __forceinline__ void softmax_sync() { asm volatile("barrier.cta.sync 2, 256;" ::: "memory"); }
+
+template <int FMT>
+__device__ __forceinline__ bool not_finite16(uint32_t h) {
+  constexpr uint32_t e = FMT == kF16 ? 0x7C00u : 0x7F80u;
+  return (h & e) == e;
+}
+template <int FMT>
+__device__ __forceinline__ float widen16(uint16_t h) {
+  if constexpr (FMT == kF16) return __half2float(__ushort_as_half(h));
+  else return __uint_as_float((uint32_t)h << 16);
+}
+template <int FMT>
+__device__ __forceinline__ uint32_t narrow2(float a, float b) {
+  if constexpr (FMT == kF16) {
+    __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<uint32_t*>(&h);
+  } else {
+    __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<uint32_t*>(&h);
+  }
+}
+
+// Element offset of key `pos` of request b and kv head hk in K or V; false when
+// its page is none of the cache's.
+__device__ __forceinline__ bool key_offset(const Params& p, int b, int hk, int pos, int64_t& ko, int64_t& vo) {
+  if (p.page_size) {
+    const uint32_t pi = (uint32_t)pos / p.page_size, at = (uint32_t)pos - pi * p.page_size;
+    const int pg = p.page_table[(int64_t)b * p.max_pages + pi];
+    ko = pg * p.ks[0] + at * p.ks[1] + hk * p.ks[2];
+    vo = pg * p.vs[0] + at * p.vs[1] + hk * p.vs[2];
+    return pg >= 0 && pg < p.n_pages;
+  }
+  ko = b * p.ks[0] + hk * p.ks[1] + (int64_t)pos * p.ks[2];
+  vo = b * p.vs[0] + hk * p.vs[1] + (int64_t)pos * p.vs[2];
+  return true;
+}
+
+// ring index of K_i and V_i within a segment of n tiles: K0 K1 V0 K2 V1 ... V(n-1)
+__device__ __forceinline__ int k_at(int i) { return i == 0 ? 0 : 2 * i - 1; }
+__device__ __forceinline__ int v_at(int i, int n) { return i == n - 1 ? 2 * n - 1 : 2 * i + 2; }
+
+template <int HD, int FMT, bool PAIR, bool CAP>
+__global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p) {
+  using C = Cfg<HD>;
+  constexpr int NS = C::kRing, LAG = C::kLag;
+  constexpr int kRows = PAIR ? 2 * BR : BR;  // rows of an item
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem_raw);
+  uint64_t* empty = full + NS;
+  uint64_t* s_full = empty + NS;      // [2]
+  uint64_t* p_ready = s_full + 2;     // [2]
+  uint64_t* o_done = p_ready + 2;     // [2]
+  uint64_t* epi_done = o_done + 2;    // [2] by segment parity
+  uint64_t* drain = epi_done + 2;
+  int64_t* s_run = reinterpret_cast<int64_t*>(drain + 1);    // [16] scan of the schedule
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(s_run + 16);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
+  volatile uint32_t* s_bad = reinterpret_cast<volatile uint32_t*>(tmem_holder + 2);  // [2] by segment parity
+  int* s_b = reinterpret_cast<int*>(tmem_holder + 4);
+  float2* s_ml = reinterpret_cast<float2*>(smem_raw + 512);  // [2][128]
+  static_assert((2 * NS + 9 + 16) * 8 + 5 * 4 <= 512 && 512 + 2 * 128 * 8 <= C::kHead - 512, "header");
+  // tiles start on the next 1024-byte boundary behind the header
+  const uint32_t pad = (1024 - ((raw + 2560) & 1023)) & 1023;
+  uint8_t* sQ = smem_raw + 2560 + pad;  // 2 tiles: PAIR both row tiles, else this and the next segment's
+  uint8_t* sRing = sQ + 2 * C::kTile;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+  if (tid == 0) {
+    for (int i = 0; i < NS; ++i) {
+      mbar_init(&full[i], 128);
+      mbar_init(&empty[i], 1);
+    }
+    for (int u = 0; u < 2; ++u) {
+      mbar_init(&s_full[u], 1);
+      mbar_init(&p_ready[u], 4);
+      mbar_init(&o_done[u], 1);
+      mbar_init(&epi_done[u], 8);
+      s_bad[u] = 0xffffffffu;
+    }
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 12) {
+    tc::tmem_alloc(tmem_holder, 512);
+    tc::tmem_relinquish();
+  }
+  // this CTA's run: the number of tiles, then the request its first tile is in
+  int64_t sum = 0;
+  for (int b = tid; b < p.B; b += kThreads) sum += (int64_t)request(p, b, kRows).per_head * p.Hkv;
+  sum = warp_sum(sum);
+  if (lane == 0) s_run[warp] = sum;
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  const uint32_t tmem = *tmem_holder;
+  int64_t W = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) W += s_run[w];
+  const int64_t G = min((int64_t)gridDim.x, W);
+  Walk walk;
+  walk.g = walk.g1 = 0;
+  if (blockIdx.x < G) {
+    walk.g = run_start(blockIdx.x, W, G);
+    walk.g1 = run_start(blockIdx.x + 1, W, G);
+  }
+  bool fits = 2560 + pad + (2 + NS) * C::kTile <= (uint32_t)C::kSmem;
+  if (!fits && tid == 0) atomicCAS(p.err, 0u, 0xB2400001u);
+  const bool some = walk.g < walk.g1 && fits;
+  if (some) {
+    int64_t before = 0;
+    for (int b0 = 0; b0 < p.B; b0 += kThreads) {
+      const int b = b0 + tid;
+      const int64_t mine = b < p.B ? (int64_t)request(p, b, kRows).per_head * p.Hkv : 0;
+      int64_t inc = mine;
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) {
+        const int64_t a = __shfl_up_sync(0xffffffffu, inc, off);
+        if (lane >= off) inc += a;
+      }
+      __syncthreads();  // s_run of the round before is read
+      if (lane == 31) s_run[warp] = inc;
+      __syncthreads();
+      int64_t start = before + inc - mine;
+      for (int w = 0; w < kThreads / 32; ++w) {
+        if (w < warp) start += s_run[w];
+        before += s_run[w];
+      }
+      if (mine > 0 && start <= walk.g && walk.g < start + mine) {
+        *s_b = b;
+        s_run[15] = start;
+      }
+      if (before > walk.g) break;  // the same for every thread
+    }
+    __syncthreads();
+    walk.b = *s_b;
+    walk.start = s_run[15];
+    walk.r = request(p, walk.b, kRows);
+  }
+
+  Segment sg;
+  if (some && warp < 4) {
+    // --------------------------------- copies ---------------------------------
+    constexpr int CH = HD / 8, RPP = 32 / CH;  // 16-byte chunks of a row, rows a warp copies at once
+    const int cc = lane % CH, rsub = lane / CH;
+    uint32_t seq = 0, handed = 0;  // tiles issued / handed over
+    uint32_t end0 = 0, end1 = 0;   // seq at the end of the last segment and of the one before
+    uint64_t meta = 0;             // 12 bits a tile in flight: first drafted row of a V tile (255: none), parity
+    bool ok = true;
+    auto chunk_at = [&](uint32_t tile, int r) {
+      return tile + (cc >> 3) * C::kAtom + r * 128 + (((cc & 7) ^ (r & 7)) << 4);
+    };
+    uint32_t seg = 0;
+    // A drafted token's V that is infinite or NaN must reach only the rows that
+    // see the token, but in P V a weight of 0 would make NaN of it: such values
+    // are zeroed here and added for those rows at the segment's end.
+    auto hand_over = [&](uint32_t m) {
+      const uint32_t slot = handed % NS;
+      const int first = m & 255;
+      if (first < 128) {
+        bool bad = false;
+        const uint32_t tile = smem_u32(sRing) + slot * C::kTile;
+        for (int i = 0; i < 32 / RPP; ++i) {
+          const int r = 32 * warp + RPP * i + rsub;
+          if (r < first) continue;
+          uint4* at = reinterpret_cast<uint4*>(sRing + (chunk_at(tile, r) - smem_u32(sRing)));
+          uint4 x = *at;
+          uint32_t* w = reinterpret_cast<uint32_t*>(&x);
+          bool hit = false;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            if (not_finite16<FMT>(w[e])) w[e] &= 0xffff0000u, hit = true;
+            if (not_finite16<FMT>(w[e] >> 16)) w[e] &= 0x0000ffffu, hit = true;
+          }
+          if (hit) *at = x;
+          bad |= hit;
+        }
+        // tagged with the segment, so that nobody has to clear it
+        if (bad) s_bad[(m >> 8) & 1] = seg - ((seg & 1) != ((m >> 8) & 1));
+      }
+      tc::fence_proxy_async_smem();
+      mbar_arrive(&full[slot]);
+      ++handed;
+    };
+    auto begin = [&]() {  // the slot of the next tile, once it is free
+      const uint32_t slot = seq % NS;
+      ok = __all_sync(0xffffffffu, wait_abort(&empty[slot], ((seq / NS) & 1) ^ 1, p.err, 0xB2400002u, abort_flag));
+      return smem_u32(sRing) + slot * C::kTile;
+    };
+    auto end = [&](uint32_t m) {
+      cp_async_commit();
+      meta = meta << 12 | m;
+      ++seq;
+      if (seq - handed > LAG) {
+        cp_async_wait<LAG>();
+        hand_over((uint32_t)(meta >> (12 * LAG)) & 0xfff);
+      }
+    };
+    auto drain_all = [&]() {
+      cp_async_wait<0>();
+      while (handed != seq) hand_over((uint32_t)(meta >> (12 * (seq - handed - 1))) & 0xfff);
+    };
+    auto copy_tile = [&](uint32_t tile, const uint16_t* base, int64_t off) {  // off < 0: zeros
+#pragma unroll
+      for (int i = 0; i < 32 / RPP; ++i) {
+        const int64_t o = __shfl_sync(0xffffffffu, off, RPP * i + rsub);
+        const int r = 32 * warp + RPP * i + rsub;
+        cp_async16(chunk_at(tile, r), base + (o < 0 ? 0 : o) + cc * 8, o >= 0);
+      }
+    };
+    while (ok && walk.next(p, kRows, sg)) {
+      if (PAIR ? seg >= 1 : seg >= 2) {
+        // Q of the segment before (PAIR) or of the one before that is free once
+        // its epilogue is over; that waits for its last tile, which must not be
+        // among those still to be handed over
+        if (handed < (PAIR ? end0 : end1)) drain_all();
+        const uint32_t prev = seg - (PAIR ? 1 : 2);
+        ok = __all_sync(0xffffffffu,
+                        wait_abort(&epi_done[prev & 1], (prev >> 1) & 1, p.err, 0xB2400003u, abort_flag));
+        if (!ok) break;
+      }
+      // this lane's key of each tile, one tile ahead
+      int64_t ko, vo, ko1 = -1, vo1 = -1;
+      auto locate = [&](int tile, int64_t& a, int64_t& c) {
+        const int pos = (sg.tile + tile) * BK + 32 * warp + lane;
+        a = c = -1;
+        if (tile < sg.n && pos < sg.keys && !key_offset(p, sg.b, sg.hk, pos, a, c)) {
+          atomicCAS(p.err, 0u, attn::kErrPage);
+          a = c = -1;
+        }
+      };
+      locate(0, ko, vo);
+      uint32_t tile = begin();
+      if (!ok) break;
+#pragma unroll 1
+      for (int u = 0; u < (PAIR ? 2 : 1); ++u) {
+        const int rt = PAIR ? 2 * sg.rt + u : sg.rt;
+        const int row = rt * BR + 32 * warp + lane;
+        int64_t off = -1;
+        if (row < p.R) {
+          const int t = row / p.rep;
+          off = sg.b * p.qs[0] + (int64_t)t * p.qs[1] + (int64_t)(sg.hk * p.rep + row - t * p.rep) * p.qs[2];
+        }
+        copy_tile(smem_u32(sQ) + (PAIR ? u : seg & 1) * C::kTile, p.q, off);
+      }
+      copy_tile(tile, p.k, ko);
+      end(255);
+      for (int i = 0; i < sg.n && ok; ++i) {
+        if (i + 1 < sg.n) {
+          locate(i + 1, ko1, vo1);
+          tile = begin();
+          if (!ok) break;
+          copy_tile(tile, p.k, ko1);
+          end(255);
+        }
+        tile = begin();
+        if (!ok) break;
+        copy_tile(tile, p.v, vo);
+        const int first = max(sg.ctx - (sg.tile + i) * BK, 0);
+        end((first < 128 && sg.dl > 0 ? first : 255) | (seg & 1) << 8);
+        vo = vo1;
+      }
+      end1 = end0;
+      end0 = seq;
+      ++seg;
+    }
+    --seg;  // hand_over tags what is left with the last segment
+    cp_async_wait<0>();
+    if (ok) drain_all();
+  } else if (some && warp == 12) {
+    // ----------------------------------- MMA -----------------------------------
+    if (lane == 0) {
+      constexpr uint32_t idS = idesc_fmt(BR, BK, FMT, false), idPV = idesc_fmt(BR, HD, FMT, true);
+      bool ok = true;
+      uint32_t base = 0, seg = 0, pc[2] = {0, 0};  // ring tiles before the segment; P tiles waited for
+      auto take = [&](int at, unsigned code) {
+        const uint32_t n = base + at;
+        ok = ok && wait_abort(&full[n % NS], (n / NS) & 1, p.err, code, abort_flag);
+        if (ok) tc::fence_after_sync();
+        return sRing + (n % NS) * C::kTile;
+      };
+      auto release = [&](int at) { tc::commit(&empty[(base + at) % NS]); };
+      auto issue_s = [&](int u, const uint8_t* k) {
+        const uint8_t* q = sQ + (PAIR ? u : seg & 1) * C::kTile;
+#pragma unroll
+        for (int kk = 0; kk < HD / 16; ++kk)
+          mma_ss<FMT>(tmem + 256 * u, tc::desc_kmajor_sw128(q + (kk >> 2) * C::kAtom + (kk & 3) * 32),
+                      tc::desc_kmajor_sw128(k + (kk >> 2) * C::kAtom + (kk & 3) * 32), idS, kk != 0);
+        tc::commit(&s_full[u]);
+      };
+      auto issue_pv = [&](int u, const uint8_t* v, bool first) {
+#pragma unroll
+        for (int kk = 0; kk < BK / 16; ++kk)
+          mma_ts<FMT>(tmem + 256 * u + 128, tmem + 256 * u + kk * 8,
+                      tc::smem_desc(v + kk * 16 * 128, C::kAtom, 1024, tc::kSwizzle128B), idPV, !first || kk != 0);
+      };
+      auto wait_p = [&](int u) {
+        ok = ok && wait_abort(&p_ready[u], pc[u] & 1, p.err, 0xB2400006u, abort_flag);
+        ++pc[u];
+        if (ok) tc::fence_after_sync();
+      };
+      while (ok && walk.next(p, kRows, sg)) {
+        const int n = sg.n;
+        const int units = PAIR && (2 * sg.rt + 1) * BR < p.R ? 2 : 1;  // PAIR: row tiles of this item
+        if constexpr (PAIR) {
+          const uint8_t* k = take(0, 0xB2400004u);
+          if (!ok) break;
+          for (int u = 0; u < units; ++u) issue_s(u, k);
+          release(0);
+          for (int j = 0; j < n && ok; ++j) {
+            const uint8_t* v = take(v_at(j, n), 0xB2400005u);
+            const bool more = j + 1 < n;
+            if (ok && more) k = take(k_at(j + 1), 0xB2400004u);
+            for (int u = 0; u < units && ok; ++u) {
+              wait_p(u);
+              if (!ok) break;
+              issue_pv(u, v, j == 0);
+              if (!more) tc::commit(&o_done[u]);
+              else issue_s(u, k);
+            }
+            if (!ok) break;
+            release(v_at(j, n));
+            if (more) release(k_at(j + 1));
+          }
+        } else {
+          for (int j = 0; j < min(n, 2) && ok; ++j) {
+            const uint8_t* k = take(k_at(j), 0xB2400004u);
+            if (!ok) break;
+            issue_s(j, k);
+            release(k_at(j));
+          }
+          for (int j = 0; j < n && ok; ++j) {
+            const int u = j & 1;
+            const uint8_t* v = take(v_at(j, n), 0xB2400005u);
+            if (ok) wait_p(u);
+            if (!ok) break;
+            issue_pv(u, v, j < 2);
+            release(v_at(j, n));
+            if (j + 2 >= n) {
+              tc::commit(&o_done[u]);
+            } else {
+              const uint8_t* k = take(k_at(j + 2), 0xB2400004u);
+              if (!ok) break;
+              issue_s(u, k);
+              release(k_at(j + 2));
+            }
+          }
+        }
+        base += 2 * n;
+        ++seg;
+      }
+      if (!ok) {
+        tc::commit(drain);
+        mbar_wait(drain, 0, p.err, 0xB2400008u);
+      }
+    }
+  } else if (some) {
+    // --------------------------------- softmax ---------------------------------
+    const int u = (warp - 4) >> 2, qw = warp & 3, r = qw * 32 + lane;
+    const uint32_t lane_off = (uint32_t)(qw * 32) << 16;
+    const uint32_t tS = tmem + 256 * u + lane_off, tO = tmem + 128 + lane_off;  // tO: of unit 0
+    uint32_t sc = 0, oc[2] = {0, 0}, seg = 0;  // S tiles / O accumulators waited for
+    bool ok = true;
+    while (walk.next(p, kRows, sg)) {
+      const int rt = PAIR ? 2 * sg.rt + u : sg.rt;
+      const int units = PAIR ? ((2 * sg.rt + 1) * BR < p.R ? 2 : 1) : min(sg.n, 2);
+      const int row = rt * BR + r, t = row / p.rep;
+      const bool row_ok = row < p.R && t < sg.dl;
+      // tokens of this warp; a warp without one leaves its P rows as they are
+      // (their O is never read)
+      const int t0 = (rt * BR + qw * 32) / p.rep, t1 = min((rt * BR + qw * 32 + 31) / p.rep, sg.dl - 1);
+      const bool warp_ok = t0 < sg.dl && rt * BR + qw * 32 < p.R;
+      const uint8_t* mask = p.mask + sg.b * p.mask_stride;
+      float m_used = -INFINITY, l = 0.f;
+      bool first = true;
+      const int step = PAIR ? 1 : 2;
+      for (int j = PAIR ? (u < units ? 0 : sg.n) : u; j < sg.n && ok; j += step) {
+        ok = __all_sync(0xffffffffu, wait_abort(&s_full[u], sc & 1, p.err, 0xB2400009u, abort_flag));
+        ++sc;
+        if (!ok) break;
+        tc::fence_after_sync();
+        if (warp_ok) {
+          const int kv0 = (sg.tile + j) * BK;
+          const bool masked = kv0 + BK > sg.ctx;
+          uint32_t vis[4];
+          if (masked) visible_bits(vis, mask, p.T, t, t0, t1, kv0, sg.ctx, sg.dl, row_ok);
+          float mx = masked ? row_max_bits<true>(tS, vis) : row_max_bits<false>(tS, vis);
+          // scale > 0 and tanh keep the order
+          if constexpr (CAP) mx = mx == -INFINITY ? mx : capped(mx, p.cap_in, p.cap_log2, 0.f);
+          else mx *= p.scale_log2;
+          const bool need = mx > m_used + kRescale;
+          const float alpha = need ? (m_used == -INFINITY ? 0.f : ex2(m_used - mx)) : 1.f;
+          if (need) {
+            l *= alpha;
+            m_used = mx;
+          }
+          if (__any_sync(0xffffffffu, need) && !first) {
+            const uint32_t mine = tO + 256 * u;
+#pragma unroll 1
+            for (int c = 0; c < HD / 32; ++c) {
+              uint32_t o[32];
+              tc::tmem_ld_32x32b_x32(mine + 32 * c, o);
+              tc::tmem_ld_wait();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+              tmem_st_32x32b_x32(mine + 32 * c, o);
+            }
+          }
+          const float mref = m_used == -INFINITY ? 0.f : m_used;
+          l += masked ? exp_to_p_bits<true, FMT, CAP>(tS, vis, mref, p) : exp_to_p_bits<false, FMT, CAP>(tS, vis, mref, p);
+          tmem_st_wait();
+        }
+        first = false;
+        tc::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_ready[u]);
+      }
+      // ------------------------------ segment end ------------------------------
+      // This thread writes row r: SINGLE, columns of half u from both units'
+      // accumulators; PAIR, all columns of its own.
+      float M = m_used, L = l, f0 = 1.f, f1 = 0.f;
+      if constexpr (!PAIR) {
+        s_ml[u * 128 + r] = make_float2(m_used, l);
+        softmax_sync();
+        const float2 ot = s_ml[(u ^ 1) * 128 + r];
+        M = fmaxf(m_used, ot.x);
+        const float ref = M == -INFINITY ? 0.f : M;
+        const float fa = m_used == -INFINITY ? 0.f : ex2(m_used - ref);
+        const float fb = ot.x == -INFINITY ? 0.f : ex2(ot.x - ref);
+        L = l * fa + ot.y * fb;
+        f0 = u ? fb : fa;
+        f1 = u ? fa : fb;
+      }
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        if ((PAIR && x != u) || x >= units) continue;
+        ok = ok && __all_sync(0xffffffffu, wait_abort(&o_done[x], oc[x] & 1, p.err, 0xB240000Au, abort_flag));
+        ++oc[x];
+      }
+      if (ok && (!PAIR || u < units)) {
+        tc::fence_after_sync();
+        const bool whole = sg.n == sg.of;  // else a partial: before the run's first item border, or behind its last
+        const bool bad = s_bad[seg & 1] == seg;
+        const float inv = L > 0.f || L != L ? 1.f / L : 0.f;
+        constexpr int kCols = PAIR ? HD : HD / 2;
+        const int c0 = PAIR ? 0 : u * kCols;
+        uint16_t* out = nullptr;
+        float* part = nullptr;
+        const int prow = PAIR ? u * BR + r : r;
+        if (whole) {
+          if (row < p.R) out = p.o + sg.b * p.os[0] + (int64_t)t * p.os[1] + (int64_t)(sg.hk * p.rep + row - t * p.rep) * p.os[2];
+        } else {
+          const int64_t slot = 2 * (int64_t)blockIdx.x + (sg.tile == 0 ? 1 : 0);
+          float* w = p.ws + slot * (kRows * (HD + 2));
+          if (PAIR || u == 0) {
+            w[kRows * HD + prow] = row_ok ? M : -INFINITY;
+            w[kRows * HD + kRows + prow] = row_ok ? L : 0.f;
+          }
+          part = w + prow * HD;
+        }
+#pragma unroll 1
+        for (int c = c0; c < c0 + kCols; c += 32) {
+          float o[32];
+          if constexpr (PAIR) {
+            tc::tmem_ld_32x32b_x32(tO + 256 * u + c, *reinterpret_cast<uint32_t(*)[32]>(o));
+            tc::tmem_ld_wait();
+          } else {
+            float o1[32];
+            tc::tmem_ld_32x32b_x32(tO + c, *reinterpret_cast<uint32_t(*)[32]>(o));
+            if (units == 2) tc::tmem_ld_32x32b_x32(tO + 256 + c, *reinterpret_cast<uint32_t(*)[32]>(o1));
+            tc::tmem_ld_wait();
+            // a factor of 0 belongs to a unit that saw nothing of this row: drop it
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+              float x = f0 == 0.f ? 0.f : o[e] * f0;
+              if (units == 2 && f1 != 0.f) x = fmaf(o1[e], f1, x);
+              o[e] = x;
+            }
+          }
+          if (bad && row_ok) {
+            const int j0 = max(sg.tile * BK - sg.ctx, 0), j1 = min((sg.tile + sg.n) * BK - sg.ctx, sg.dl);
+            for (int j = j0; j < j1; ++j) {
+              int64_t ko, vo;
+              if (!mask[(int64_t)t * p.T + j] || !key_offset(p, sg.b, sg.hk, sg.ctx + j, ko, vo)) continue;
+#pragma unroll
+              for (int e = 0; e < 32; ++e) {
+                const uint16_t h = p.v[vo + c + e];
+                if (not_finite16<FMT>(h)) o[e] += widen16<FMT>(h);
+              }
+            }
+          }
+          if (!row_ok || L == 0.f) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = 0.f;
+          }
+          if (out) {
+            uint4* dst = reinterpret_cast<uint4*>(out + c);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              dst[e] = make_uint4(narrow2<FMT>(o[8 * e] * inv, o[8 * e + 1] * inv),
+                                  narrow2<FMT>(o[8 * e + 2] * inv, o[8 * e + 3] * inv),
+                                  narrow2<FMT>(o[8 * e + 4] * inv, o[8 * e + 5] * inv),
+                                  narrow2<FMT>(o[8 * e + 6] * inv, o[8 * e + 7] * inv));
+          }
+          if (part) {
+            float4* dst = reinterpret_cast<float4*>(part + c);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) dst[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+          }
+        }
+      }
+      ++seg;
+      // both warpgroups have read the accumulators: the next segment may overwrite them
+      tc::fence_before_sync();
+      if (any_of_softmax(!ok)) break;
+      if (lane == 0) mbar_arrive(&epi_done[(seg - 1) & 1]);
+    }
+  }
+
+  tc::fence_before_sync();
+  __syncthreads();
+  if (warp == 12) {
+    tc::fence_after_sync();
+    tc::tmem_dealloc(tmem, 512);
+  }
+}
+
+// Joins the partials of the items that several CTAs shared:
+// o = sum_c 2^{m_c - M} o_c / sum_c 2^{m_c - M} l_c.  One CTA per item and kJoin
+// rows, a warp per row.
+constexpr int kJoin = 16;
+template <int HD, int FMT, bool PAIR>
+__global__ void __launch_bounds__(128) tree_join_kernel(const Params p, int64_t G) {
+  constexpr int kRows = PAIR ? 2 * BR : BR;
+  __shared__ int64_t s_w[4], s_before[4];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int b = blockIdx.y, rt = blockIdx.x % p.n_rt, hk = blockIdx.x / p.n_rt % p.Hkv;
+  const int row0 = blockIdx.x / p.n_rt / p.Hkv * kJoin;
+  int64_t W = 0, before = 0;
+  for (int i = tid; i < p.B; i += 128) {
+    const int64_t n = (int64_t)request(p, i, kRows).per_head * p.Hkv;
+    W += n;
+    if (i < b) before += n;
+  }
+  W = warp_sum(W);
+  before = warp_sum(before);
+  if (lane == 0) {
+    s_w[warp] = W;
+    s_before[warp] = before;
+  }
+  __syncthreads();
+  W = s_w[0] + s_w[1] + s_w[2] + s_w[3];
+  before = s_before[0] + s_before[1] + s_before[2] + s_before[3];
+  const Req r = request(p, b, kRows);
+  if (rt >= r.full) return;  // one tile: written by its CTA
+  const int64_t g0 = before + (int64_t)hk * r.per_head + (int64_t)rt * r.tiles, g1 = g0 + r.tiles;
+  G = min(G, W);
+  // CTA of tile g: the last one whose run starts at or before it
+  const int64_t ca = ((g0 + 1) * G + W - 1) / W - 1, cz = (g1 * G + W - 1) / W - 1;
+  if (ca == cz) return;  // a single segment: written by its CTA
+  constexpr int V = HD / 32;  // columns a lane
+  const int64_t stride = kRows * (HD + 2);
+  for (int i = warp; i < kJoin; i += 4) {
+    const int in = row0 + i, row = rt * kRows + in;
+    if (in >= kRows || row >= p.R) return;
+    float M = -INFINITY;
+    for (int64_t c = ca; c <= cz; ++c) M = fmaxf(M, p.ws[(2 * c + (c == ca)) * stride + kRows * HD + in]);
+    const float ref = M == -INFINITY ? 0.f : M;
+    float acc[V], L = 0.f;
+#pragma unroll
+    for (int e = 0; e < V; ++e) acc[e] = 0.f;
+    for (int64_t c = ca; c <= cz; ++c) {
+      const float* w = p.ws + (2 * c + (c == ca)) * stride;
+      const float l = w[kRows * HD + kRows + in];
+      if (l == 0.f) continue;
+      const float f = ex2(w[kRows * HD + in] - ref);
+      L = fmaf(f, l, L);
+      float x[V];
+      if constexpr (V == 4) *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(w + in * HD + lane * V);
+      else *reinterpret_cast<float2*>(x) = *reinterpret_cast<const float2*>(w + in * HD + lane * V);
+#pragma unroll
+      for (int e = 0; e < V; ++e) acc[e] = fmaf(f, x[e], acc[e]);
+    }
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+    const int t = row / p.rep;
+    uint16_t* o = p.o + b * p.os[0] + (int64_t)t * p.os[1] + (int64_t)(hk * p.rep + row - t * p.rep) * p.os[2] + lane * V;
+    uint32_t h[V / 2];
+#pragma unroll
+    for (int e = 0; e < V / 2; ++e) h[e] = narrow2<FMT>(acc[2 * e] * inv, acc[2 * e + 1] * inv);
+    if constexpr (V == 4) *reinterpret_cast<uint2*>(o) = make_uint2(h[0], h[1]);
+    else *reinterpret_cast<uint32_t*>(o) = h[0];
+  }
+}
+
+template <int HD, int FMT, bool PAIR, bool CAP>
+static void launch(const Params& p, cudaStream_t st) {
+  const int G = num_sms();
+  set_max_smem((const void*)tree_kernel<HD, FMT, PAIR, CAP>, Cfg<HD>::kSmem);
+  tree_kernel<HD, FMT, PAIR, CAP><<<G, kThreads, Cfg<HD>::kSmem, st>>>(p);
+  const int rows = min(PAIR ? 2 * BR : BR, p.R);
+  const dim3 grid((unsigned)(p.n_rt * p.Hkv * ((rows + kJoin - 1) / kJoin)), p.B);
+  tree_join_kernel<HD, FMT, PAIR><<<grid, 128, 0, st>>>(p, G);
+}
+
+}  // namespace tree
+}  // namespace b2
+
 using namespace b2;
+
+// The tensor-core kernel takes 16-bit queries and cache of one type with head
+// dim 64 or 128; the rest runs on the CUDA cores.
+static bool tree_tc(int64_t D, int q_dtype, int kv_dtype) {
+  return q_dtype == kv_dtype && q_dtype != B2_F32 && (D == 64 || D == 128);
+}
 
 extern "C" size_t b2_tree_attn_workspace_size(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D,
                                               int64_t max_keys, int q_dtype, int kv_dtype) {
   if (B <= 0 || T <= 0 || Hq <= 0 || Hkv <= 0 || D <= 0 || max_keys <= 0) return 0;
-  return attn::simt_workspace(B, T, Hq, Hkv, D, max_keys);
+  const size_t simt = attn::simt_workspace(B, T, Hq, Hkv, D, max_keys);
+  if (!tree_tc(D, q_dtype, kv_dtype)) return simt;
+  // two partials a CTA; the larger of both kernels' needs, since strides and
+  // alignment, which also decide, come with the call
+  const int64_t rows = T * (Hq / Hkv) > tree::BR ? 2 * tree::BR : tree::BR;
+  const size_t tc = (size_t)2 * num_sms() * rows * (D + 2) * sizeof(float);
+  return tc > simt ? tc : simt;
 }
 
 extern "C" int b2_tree_attn(const void* q, const void* k, const void* v, void* o, const int32_t* page_table,
@@ -69,6 +952,61 @@ extern "C" int b2_tree_attn(const void* q, const void* k, const void* v, void* o
   B2_CHECK_ARG(p.err, B2_ERR_LAUNCH, "tree_attn: no device");
   const size_t need = b2_tree_attn_workspace_size(B, T, Hq, Hkv, D, max_keys, q_dtype, kv_dtype);
   B2_CHECK_ARG(need == 0 || workspace, B2_ERR_INVALID, "tree_attn: workspace required");
+  cudaStream_t st = (cudaStream_t)stream;
+  const int64_t rep = Hq / Hkv, R = T * rep;
+  bool wide = aligned(q, 16) && aligned(k, 16) && aligned(v, 16) && aligned(o, 16) && aligned(workspace, 16);
+  for (int i = 0; i < 3; ++i)
+    wide = wide && q_strides[i] % 8 == 0 && k_strides[i] % 8 == 0 && v_strides[i] % 8 == 0 && o_strides[i] % 8 == 0;
+  const bool pair = R > tree::BR;
+  const int64_t n_rt = pair ? (R + 2 * tree::BR - 1) / (2 * tree::BR) : 1;
+  // scale > 0: the row maximum is taken before the scale
+  if (tree_tc(D, q_dtype, kv_dtype) && wide && scale > 0.f && max_keys > 0 &&
+      Hkv * n_rt * ((max_keys + tree::BK - 1) / tree::BK) <= (1 << 30) && n_rt * Hkv <= (1 << 24)) {
+    tree::Params t = {};
+    t.q = (const uint16_t*)q;
+    t.k = (const uint16_t*)k;
+    t.v = (const uint16_t*)v;
+    t.o = (uint16_t*)o;
+    t.page_table = page_table;
+    t.ctx = context_lens;
+    t.draft = draft_lens;
+    t.mask = tree_mask;
+    t.ws = (float*)workspace;
+    t.mask_stride = mask_stride;
+    t.n_pages = n_pages;
+    for (int i = 0; i < 3; ++i) {
+      t.qs[i] = q_strides[i];
+      t.os[i] = o_strides[i];
+      t.ks[i] = k_strides[i];
+      t.vs[i] = v_strides[i];
+    }
+    t.B = (int)B;
+    t.T = (int)T;
+    t.Hkv = (int)Hkv;
+    t.rep = (int)rep;
+    t.R = (int)R;
+    t.cap = (int)max_keys;
+    t.n_rt = (int)n_rt;
+    t.page_size = (uint32_t)page_size;
+    t.max_pages = (int)max_pages;
+    t.scale_log2 = scale * attn::kLog2e;
+    t.cap_log2 = softcap * attn::kLog2e;
+    t.cap_in = softcap > 0.f ? 2.f * attn::kLog2e * scale / softcap : 0.f;
+    t.err = p.err;
+#define B2_TREE(HD, FMT)                                              \
+  do {                                                                \
+    if (pair && softcap > 0.f) tree::launch<HD, FMT, true, true>(t, st);   \
+    else if (pair) tree::launch<HD, FMT, true, false>(t, st);         \
+    else if (softcap > 0.f) tree::launch<HD, FMT, false, true>(t, st);     \
+    else tree::launch<HD, FMT, false, false>(t, st);                  \
+  } while (0)
+    if (D == 128 && q_dtype == B2_F16) B2_TREE(128, fa::kF16);
+    else if (D == 128) B2_TREE(128, fa::kBF16);
+    else if (q_dtype == B2_F16) B2_TREE(64, fa::kF16);
+    else B2_TREE(64, fa::kBF16);
+#undef B2_TREE
+    return launch_status("tree_attn");
+  }
   p.ws = need ? (float*)workspace : nullptr;
-  return attn::launch_simt(p, q_dtype, kv_dtype, (cudaStream_t)stream, "tree_attn");
+  return attn::launch_simt(p, q_dtype, kv_dtype, st, "tree_attn");
 }
