@@ -173,6 +173,32 @@ B2_API int b2_flash_attn_fwd_window(const void* q, const void* k, const void* v,
                                     float scale, int64_t window, int dtype, void* stream);
 
 /*
+ * FlashAttention forward with more masks and score forms (the reference has
+ * the causal mask only).  Tensors, strides and dtypes as in b2_flash_attn_fwd.
+ *   s = scale q.k; softcap > 0: s = softcap tanh(s / softcap);
+ *   alibi_slopes fp32 [Hq] or NULL: s -= slope[h] |query - key|.
+ *   causal, window (> 0 needs causal): as in b2_flash_attn_fwd_window.
+ *   doc_offsets int32 [B, n_docs + 1] ascending, or NULL (needs Sq == Skv):
+ *     tokens off[d] .. off[d + 1] - 1 are document d; a query sees only keys of
+ *     its document.  Tokens in no document (padding) see nothing.
+ *   prefix_lens int32 [B, n_docs] (without documents [B]) or NULL (needs causal,
+ *     no window): the first prefix_lens tokens of a document are seen by all
+ *     of its queries, the rest causally.
+ * Rows that see nothing give 0, and hidden keys do not count whatever their
+ * values.  fp16 / bf16 with D = 64 or 128 and 16-byte aligned rows run on
+ * tcgen05, the rest (fp32 kept in fp32) on the CUDA cores; D <= 256.
+ */
+B2_API int b2_flash_attn_fwd_scored(const void* q, const void* k, const void* v, void* o,
+                                    int64_t B, int64_t Hq, int64_t Hkv,
+                                    int64_t Sq, int64_t Skv, int64_t D,
+                                    const int64_t* q_strides, const int64_t* k_strides,
+                                    const int64_t* v_strides, const int64_t* o_strides,
+                                    float scale, int causal, int64_t window, float softcap,
+                                    const float* alibi_slopes, const int32_t* doc_offsets,
+                                    int64_t n_docs, const int32_t* prefix_lens, int dtype,
+                                    void* stream);
+
+/*
  * Decode attention: one query token per head over a KV cache, split-KV.
  * Replaces kv_cache_attention, gqa_attention, batched_kv_decode,
  * paged_attention, multi_head_paged_attention and fp16_kv_attention
@@ -202,6 +228,23 @@ B2_API int b2_decode_attn(const void* q, const void* k, const void* v, void* o,
                           const int64_t* v_strides, const int32_t* q_pos,
                           int64_t window, const float* rope_freqs, float scale,
                           int q_dtype, int kv_dtype, void* stream);
+
+/*
+ * b2_decode_attn with capped and biased scores: softcap > 0: s = softcap
+ * tanh(s / softcap); alibi_slopes fp32 [Hq] or NULL: s -= slope[h] |q_pos -
+ * key|.  n_pages: pages of a paged cache; a page number outside [0, n_pages)
+ * reads as zeros and is recorded in the device error word.
+ */
+B2_API int b2_decode_attn_scored(const void* q, const void* k, const void* v, void* o,
+                                 const int32_t* page_table, const int32_t* seq_lens,
+                                 void* workspace, int64_t B, int64_t Hq, int64_t Hkv,
+                                 int64_t D, int64_t max_seq_len, int64_t page_size,
+                                 int64_t max_pages, int64_t n_pages,
+                                 const int64_t* k_strides, const int64_t* v_strides,
+                                 const int32_t* q_pos, int64_t window,
+                                 const float* rope_freqs, float scale, float softcap,
+                                 const float* alibi_slopes, int q_dtype, int kv_dtype,
+                                 void* stream);
 
 /*
  * repeat_kv (make_repeat_kv_kernel, _msl_templates.py:3434-3480):

@@ -34,11 +34,37 @@ def _strides(t):
     return t, _lib.strides_arg(t.stride()[:3])
 
 
-def flash_attention(q, k, v, causal=False, scale=None, out=None, window=0):
+def _score_args(Hq, device, softcap, alibi_slopes):
+    """Checked softcap and slopes (fp32 [Hq] on the device) of capped / biased scores."""
+    if softcap < 0 or not math.isfinite(softcap):
+        raise B2ShapeError("softcap must be a finite number >= 0")
+    if alibi_slopes is None:
+        return None
+    if alibi_slopes.dtype != torch.float32 or tuple(alibi_slopes.shape) != (Hq,):
+        raise B2ShapeError(f"alibi_slopes must be fp32 [{Hq}]")
+    if alibi_slopes.device != device:
+        raise B2ShapeError(f"alibi_slopes is on {alibi_slopes.device}, not on {device}")
+    return alibi_slopes.contiguous()
+
+
+def flash_attention(q, k, v, causal=False, scale=None, out=None, window=0, softcap=0.0, alibi_slopes=None,
+                    doc_offsets=None, prefix_lens=None):
     """O = softmax(scale Q K^T [causal]) V for [B, H, S, D] tensors (GQA when Hq > Hkv).
 
     window > 0 (needs causal): query s sees keys s - window + 1 .. s only
-    (Mistral-style sliding window)."""
+    (Mistral-style sliding window).
+
+    softcap > 0 caps the scores: softcap * tanh(scale q.k / softcap).
+    alibi_slopes fp32 [Hq] subtracts slope * |query - key| from them (after the cap).
+    doc_offsets int32 [B, n_docs + 1], ascending: several documents packed in a
+    row, tokens offsets[d] .. offsets[d + 1] - 1 each; a query sees only its own
+    document (a padded batch is one document a row).  Tokens in no document see
+    nothing and give 0.
+    prefix_lens int32 [B], or [B, n_docs] with documents (needs causal, no
+    window): the first tokens of a document that all of its queries see.
+    With any of these, hidden keys do not count whatever their values, fp32
+    inputs are computed in fp32 on the CUDA cores at every head dim, and scale
+    may have any sign."""
     for t in (q, k, v):
         if not t.is_cuda:
             raise B2ShapeError("b200kern ops take CUDA tensors (there is no CPU path)")
@@ -62,14 +88,47 @@ def flash_attention(q, k, v, causal=False, scale=None, out=None, window=0):
     if o.stride(3) != 1:
         raise B2ShapeError("out must have a contiguous last dimension")
     os_ = _lib.strides_arg(o.stride()[:3])
+    if window and (not causal or window < 0):
+        raise B2ShapeError("a sliding window needs causal=True and window > 0")
+    if softcap or alibi_slopes is not None or doc_offsets is not None or prefix_lens is not None:
+        return _flash_scored(q, k, v, o, qs, ks, vs, os_, causal, scale, window, softcap, alibi_slopes, doc_offsets,
+                             prefix_lens)
     if window:
-        if not causal or window < 0:
-            raise B2ShapeError("a sliding window needs causal=True and window > 0")
         _lib.call("b2_flash_attn_fwd_window", q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
                   B, Hq, Hkv, Sq, Skv, D, qs, ks, vs, os_, float(scale), int(window), _DT[q.dtype], _stream())
         return o
     _lib.call("b2_flash_attn_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
               B, Hq, Hkv, Sq, Skv, D, qs, ks, vs, os_, float(scale), int(bool(causal)), _DT[q.dtype], _stream())
+    return o
+
+
+def _flash_scored(q, k, v, o, qs, ks, vs, os_, causal, scale, window, softcap, alibi_slopes, doc_offsets, prefix_lens):
+    B, Hq, Sq, D = q.shape
+    Hkv, Skv = k.shape[1], k.shape[2]
+    if (causal or doc_offsets is not None) and Sq != Skv:
+        raise B2ShapeError("causal and doc_offsets need as many queries as keys")
+    slopes = _score_args(Hq, q.device, softcap, alibi_slopes)
+    n_docs = 0
+    if doc_offsets is not None:
+        if doc_offsets.dtype != torch.int32 or doc_offsets.dim() != 2 or doc_offsets.shape[0] != B \
+                or doc_offsets.shape[1] < 2:
+            raise B2ShapeError(f"doc_offsets must be int32 [{B}, n_docs + 1] with n_docs >= 1")
+        doc_offsets = doc_offsets.contiguous()
+        n_docs = doc_offsets.shape[1] - 1
+    if prefix_lens is not None:
+        want = (B, n_docs) if n_docs else (B,)
+        if prefix_lens.dtype != torch.int32 or tuple(prefix_lens.shape) != want:
+            raise B2ShapeError(f"prefix_lens must be int32 {list(want)}")
+        if not causal or window:
+            raise B2ShapeError("prefix_lens needs causal=True and no window")
+        prefix_lens = prefix_lens.contiguous()
+    _lib.check_device(q, k=k, v=v, out=o, doc_offsets=doc_offsets, prefix_lens=prefix_lens)
+    p = lambda t: None if t is None else t.data_ptr()
+    with _lib.on_device(q):
+        if o.numel():
+            _lib.call("b2_flash_attn_fwd_scored", p(q), p(k), p(v), p(o), B, Hq, Hkv, Sq, Skv, D, qs, ks, vs, os_,
+                      float(scale), int(bool(causal)), int(window), float(softcap), p(slopes), p(doc_offsets), n_docs,
+                      p(prefix_lens), _DT[q.dtype], _stream())
     return o
 
 
@@ -105,7 +164,7 @@ def _seq_lens(seq_lens, B, device):
 
 
 def decode_attention(q, k_cache, v_cache, seq_lens, scale=None, page_table=None, out=None, q_pos=None, window=0,
-                     rope_freqs=None):
+                     rope_freqs=None, softcap=0.0, alibi_slopes=None):
     """o[B, Hq, D] = softmax(scale q K^T) V over the first seq_lens[b] keys.
 
     Contiguous cache: k/v [B, Hkv, S, D] (any strides, last dim contiguous).
@@ -114,7 +173,10 @@ def decode_attention(q, k_cache, v_cache, seq_lens, scale=None, page_table=None,
     The cache dtype may differ from q's (e.g. fp16 KV with fp32 queries).
     q_pos [B] (default seq_len - 1); window > 0 keeps the keys
     [max(0, q_pos + 1 - window), min(q_pos + 1, seq_len)) (sliding window);
-    rope_freqs [D/2] rotates q at q_pos and each key at its position (RoPE)."""
+    rope_freqs [D/2] rotates q at q_pos and each key at its position (RoPE).
+    softcap > 0 caps the scores, softcap * tanh(scale q.k / softcap);
+    alibi_slopes fp32 [Hq] then subtracts slope * |q_pos - key|.  A page number
+    outside a paged cache reads as zeros and shows in b2_device_error."""
     for t in (q, k_cache, v_cache):
         if not t.is_cuda:
             raise B2ShapeError("b200kern ops take CUDA tensors (there is no CPU path)")
@@ -153,10 +215,13 @@ def decode_attention(q, k_cache, v_cache, seq_lens, scale=None, page_table=None,
         fr = torch.as_tensor(rope_freqs, dtype=torch.float32).to(q.device).contiguous()
         if fr.numel() != D // 2:
             raise B2ShapeError(f"rope_freqs must have D/2 = {D // 2} entries")
-    _lib.call("b2_decode_attn", q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), o.data_ptr(),
+    slopes = _score_args(Hq, q.device, softcap, alibi_slopes)
+    n_pages = k_cache.shape[0] if pt is not None else 0
+    _lib.call("b2_decode_attn_scored", q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), o.data_ptr(),
               None if pt is None else pt.data_ptr(), lens.data_ptr(), ws.data_ptr(), B, Hq, Hkv, D, S, ps,
-              max_pages, _lib.strides_arg(ks), _lib.strides_arg(vs), None if qp is None else qp.data_ptr(),
-              int(window), None if fr is None else fr.data_ptr(), scale, _DT[q.dtype], _DT[k_cache.dtype],
+              max_pages, n_pages, _lib.strides_arg(ks), _lib.strides_arg(vs), None if qp is None else qp.data_ptr(),
+              int(window), None if fr is None else fr.data_ptr(), scale, float(softcap),
+              None if slopes is None else slopes.data_ptr(), _DT[q.dtype], _DT[k_cache.dtype],
               _stream())
     return o
 

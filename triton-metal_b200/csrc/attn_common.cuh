@@ -36,7 +36,7 @@ __device__ __forceinline__ void row_range(const RangeMask& m, int b, int row, in
     }
     d = a;
     lo = hi = 0;
-    if (d < m.n_docs && off[d] <= row) {
+    if (d < m.n_docs && off[d] <= row && row < off[d + 1]) {
       lo = max(off[d], 0);
       hi = min(off[d + 1], Skv);
     }

@@ -23,8 +23,11 @@
 // Options: q_pos [B] (default seq_len - 1) and window W > 0 restrict the
 // keys to [max(0, q_pos + 1 - W), min(q_pos + 1, seq_len)) (sliding window);
 // rope freqs [D/2] rotate q at q_pos and key j at j, pairs (2d, 2d + 1) by
-// angle pos * freqs[d], before the dot products (V is not rotated).
-#include "b2_common.cuh"
+// angle pos * freqs[d], before the dot products (V is not rotated); softcap
+// and slopes: s = softcap tanh(s / softcap), then s -= slope |q_pos - key| (both
+// after RoPE and scale).
+#include "attn_common.cuh"
+#include <math.h>
 #include <type_traits>
 
 namespace b2 {
@@ -49,7 +52,19 @@ struct Params {
   int window;            // > 0: sliding window
   int cap;               // keys a sequence may reach: max_seq_len (<= max_pages * page_size when paged)
   const float* rope;     // [D/2] RoPE frequencies or null
+  int64_t n_pages;       // page numbers outside [0, n_pages) read as zeros
+  float softcap;         // 0: none
+  const float* slopes;   // [Hq] or null
+  unsigned* err;
 };
+
+// Physical page of a key, or -1 (recorded) when it is none of the cache's.
+__device__ __forceinline__ int64_t key_page(const Params& p, int b, int pos) {
+  const int pg = p.page_table[(int64_t)b * p.max_pages + pos / p.page_size];
+  if (pg >= 0 && pg < p.n_pages) return pg;
+  atomicCAS(p.err, 0u, attn::kErrPage);
+  return -1;
+}
 
 // Key range [lo, hi) of sequence b and its query position.
 __device__ __forceinline__ void key_range(const Params& p, int b, int& lo, int& hi, int& qp) {
@@ -132,17 +147,21 @@ decode_split_kernel(const Params p) {
       float kv = 0.f, vv = 0.f;
       if (pos < s1) {
         int64_t ko, vo;
+        bool there = true;
         if constexpr (PAGED) {
-          const int pg = p.page_table[(int64_t)b * p.max_pages + pos / p.page_size];
+          const int64_t pg = key_page(p, b, pos);
           const int off = pos % p.page_size;
+          there = pg >= 0;
           ko = pg * p.ks[0] + off * p.ks[1] + hk * p.ks[2] + d;
           vo = pg * p.vs[0] + off * p.vs[1] + hk * p.vs[2] + d;
         } else {
           ko = b * p.ks[0] + hk * p.ks[1] + (int64_t)pos * p.ks[2] + d;
           vo = b * p.vs[0] + hk * p.vs[1] + (int64_t)pos * p.vs[2] + d;
         }
-        kv = ldf(kb + ko);
-        vv = ldf(vb + vo);
+        if (there) {
+          kv = ldf(kb + ko);
+          vv = ldf(vb + vo);
+        }
       }
       sK[j * LDK + d] = kv;
       sV[j * LDK + d] = vv;
@@ -170,6 +189,8 @@ decode_split_kernel(const Params p) {
         const int j = lane + 32 * u;
         float dot = 0.f;
         for (int d = 0; d < D; ++d) dot += sQ[hh * D + d] * sK[j * LDK + d];
+        if (p.softcap > 0.f) dot = p.softcap * attn::tanh_acc(__fdividef(dot, p.softcap));
+        if (p.slopes) dot -= p.slopes[hk * rep + hh] * fabsf((float)(qp - (t0 + j)));
         sc[u] = (t0 + j < s1) ? dot : -INFINITY;
       }
       float tmax = fmaxf(sc[0], sc[1]);
@@ -312,7 +333,8 @@ __device__ __forceinline__ uint32_t swz(int r, int c) {
   return (uint32_t)(r * D * 2 + ((c ^ (r & 7)) << 4));
 }
 
-template <typename T, int D, bool PAGED, bool ROPE>
+// SC: capped and / or biased scores
+template <typename T, int D, bool PAGED, bool ROPE, bool SC>
 __global__ void __launch_bounds__(kThreads, D == 256 ? 1 : 2)
 decode_tc_kernel(const Params p) {
   using C = TcCfg<D>;
@@ -357,14 +379,17 @@ decode_tc_kernel(const Params p) {
 #pragma unroll
     for (int i = 0; i < TK / C::kRowsPerPass; ++i) {
       const int r = r0 + i * C::kRowsPerPass, pos = base + r;
-      const bool ok = pos < s1;
+      bool ok = pos < s1;
       int64_t ko = 0, vo = 0;
       if (ok) {
         if constexpr (PAGED) {
-          const int pg = p.page_table[(int64_t)b * p.max_pages + pos / p.page_size];
+          const int64_t pg = key_page(p, b, pos);
           const int off = pos - (pos / p.page_size) * p.page_size;
-          ko = pg * p.ks[0] + off * p.ks[1] + hk * p.ks[2];
-          vo = pg * p.vs[0] + off * p.vs[1] + hk * p.vs[2];
+          if (pg >= 0) {
+            ko = pg * p.ks[0] + off * p.ks[1] + hk * p.ks[2];
+            vo = pg * p.vs[0] + off * p.vs[1] + hk * p.vs[2];
+          }
+          ok = pg >= 0;
         } else {
           ko = b * p.ks[0] + hk * p.ks[1] + (int64_t)pos * p.ks[2];
           vo = b * p.vs[0] + hk * p.vs[1] + (int64_t)pos * p.vs[2];
@@ -383,6 +408,16 @@ decode_tc_kernel(const Params p) {
 
   const float sl2 = p.scale * 1.4426950408889634f;  // scores in log2 units
   const int g = lane >> 2, tq = lane & 3;
+  // SC: tanh y = 1 - 2 / (1 + e^2y), as in the prefill kernel
+  const float cap_log2 = SC ? p.softcap * attn::kLog2e : 0.f;
+  const float cap_in = SC && p.softcap > 0.f ? 2.f * sl2 / p.softcap : 0.f;
+  float slope0 = 0.f, slope1 = 0.f;
+  if constexpr (SC) {
+    if (p.slopes) {
+      if (g < rep) slope0 = p.slopes[hk * rep + g] * attn::kLog2e;
+      if (g + 8 < rep) slope1 = p.slopes[hk * rep + g + 8] * attn::kLog2e;
+    }
+  }
   float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;  // rows g, g + 8
   float acc[D / 8][4];
 #pragma unroll
@@ -451,8 +486,14 @@ decode_tc_kernel(const Params p) {
     for (int j = 0; j < 2; ++j) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const bool ok = kpos + j * 8 + (e & 1) < s1;
-        s[j][e] = ok ? s[j][e] * sl2 : -INFINITY;
+        const int key = kpos + j * 8 + (e & 1);
+        const bool ok = key < s1;
+        float x = s[j][e] * sl2;
+        if constexpr (SC) {
+          if (p.softcap > 0.f) x = cap_log2 - 2.f * cap_log2 * __fdividef(1.f, 1.f + exp2f(s[j][e] * cap_in));
+          x -= (e < 2 ? slope0 : slope1) * fabsf((float)(qp - key));
+        }
+        s[j][e] = ok ? x : -INFINITY;
       }
       mx0 = fmaxf(mx0, fmaxf(s[j][0], s[j][1]));
       mx1 = fmaxf(mx1, fmaxf(s[j][2], s[j][3]));
@@ -574,11 +615,12 @@ extern "C" size_t b2_decode_attn_workspace_size(int64_t B, int64_t Hq, int64_t H
   return (size_t)B * Hq * ns * (D + 2) * sizeof(float);
 }
 
-extern "C" int b2_decode_attn(const void* q, const void* k, const void* v, void* o, const int32_t* page_table,
-                              const int32_t* seq_lens, void* workspace, int64_t B, int64_t Hq, int64_t Hkv, int64_t D,
-                              int64_t max_seq_len, int64_t page_size, int64_t max_pages, const int64_t* k_strides,
-                              const int64_t* v_strides, const int32_t* q_pos, int64_t window, const float* rope_freqs,
-                              float scale, int q_dtype, int kv_dtype, void* stream) {
+static int decode_impl(const void* q, const void* k, const void* v, void* o, const int32_t* page_table,
+                       const int32_t* seq_lens, void* workspace, int64_t B, int64_t Hq, int64_t Hkv, int64_t D,
+                       int64_t max_seq_len, int64_t page_size, int64_t max_pages, int64_t n_pages,
+                       const int64_t* k_strides, const int64_t* v_strides, const int32_t* q_pos, int64_t window,
+                       const float* rope_freqs, float scale, float softcap, const float* slopes, int q_dtype,
+                       int kv_dtype, void* stream) {
   B2_CHECK_ARG(q && k && v && o && seq_lens && k_strides && v_strides, B2_ERR_INVALID, "decode_attn: null pointer");
   B2_CHECK_ARG(B > 0 && Hq > 0 && Hkv > 0 && D > 0 && max_seq_len >= 0, B2_ERR_INVALID, "decode_attn: bad shape");
   B2_CHECK_ARG(Hq % Hkv == 0 && Hq / Hkv <= dec::kMaxRep, B2_ERR_UNSUPPORTED,
@@ -615,6 +657,11 @@ extern "C" int b2_decode_attn(const void* q, const void* k, const void* v, void*
   p.window = (int)(window > 0 ? window : 0);
   p.cap = (int)max_seq_len;
   p.rope = rope_freqs;
+  p.n_pages = n_pages;
+  p.softcap = softcap;
+  p.slopes = slopes;
+  p.err = device_error_word();
+  const bool scored = softcap > 0.f || slopes;
   B2_CHECK_ARG(!rope_freqs || D % 2 == 0, B2_ERR_INVALID, "decode_attn: RoPE needs an even head dim");
   // with a window every sequence has at most `window` keys: split that
   const int64_t eff_len = (window > 0 && window < max_seq_len) ? window : max_seq_len;
@@ -632,11 +679,16 @@ extern "C" int b2_decode_attn(const void* q, const void* k, const void* v, void*
   bool s16 = true;
   for (int i = 0; i < 3; ++i) s16 = s16 && p.ks[i] % 8 == 0 && p.vs[i] % 8 == 0;
   if (q_dtype == kv_dtype && q_dtype != B2_F32 && (D == 64 || D == 128 || D == 256) && a16 && s16) {
-#define B2_TC2(T, DD, PG, RP)                                                                                \
+#define B2_TC3(T, DD, PG, RP, SC)                                                                            \
   do {                                                                                                       \
     const int sm = dec::TcCfg<DD>::kSmem;                                                                    \
-    set_max_smem((const void*)dec::decode_tc_kernel<T, DD, PG, RP>, sm);                                     \
-    dec::decode_tc_kernel<T, DD, PG, RP><<<grid, dec::kThreads, sm, st>>>(p);                                \
+    set_max_smem((const void*)dec::decode_tc_kernel<T, DD, PG, RP, SC>, sm);                                 \
+    dec::decode_tc_kernel<T, DD, PG, RP, SC><<<grid, dec::kThreads, sm, st>>>(p);                            \
+  } while (0)
+#define B2_TC2(T, DD, PG, RP)                           \
+  do {                                                  \
+    if (scored) B2_TC3(T, DD, PG, RP, true);            \
+    else B2_TC3(T, DD, PG, RP, false);                  \
   } while (0)
 #define B2_TC(T, DD)                                    \
   do {                                                  \
@@ -664,6 +716,7 @@ extern "C" int b2_decode_attn(const void* q, const void* k, const void* v, void*
 #undef B2_TC_D
 #undef B2_TC
 #undef B2_TC2
+#undef B2_TC3
     return launch_status("decode_attn");
   }
   const size_t smem = dec::smem_bytes(p.D);
@@ -690,6 +743,31 @@ extern "C" int b2_decode_attn(const void* q, const void* k, const void* v, void*
 #undef B2_DEC_KV
 #undef B2_DEC
   return launch_status("decode_attn");
+}
+
+extern "C" int b2_decode_attn(const void* q, const void* k, const void* v, void* o, const int32_t* page_table,
+                              const int32_t* seq_lens, void* workspace, int64_t B, int64_t Hq, int64_t Hkv, int64_t D,
+                              int64_t max_seq_len, int64_t page_size, int64_t max_pages, const int64_t* k_strides,
+                              const int64_t* v_strides, const int32_t* q_pos, int64_t window, const float* rope_freqs,
+                              float scale, int q_dtype, int kv_dtype, void* stream) {
+  return decode_impl(q, k, v, o, page_table, seq_lens, workspace, B, Hq, Hkv, D, max_seq_len, page_size, max_pages,
+                     INT64_MAX, k_strides, v_strides, q_pos, window, rope_freqs, scale, 0.f, nullptr, q_dtype, kv_dtype,
+                     stream);
+}
+
+extern "C" int b2_decode_attn_scored(const void* q, const void* k, const void* v, void* o, const int32_t* page_table,
+                                     const int32_t* seq_lens, void* workspace, int64_t B, int64_t Hq, int64_t Hkv,
+                                     int64_t D, int64_t max_seq_len, int64_t page_size, int64_t max_pages,
+                                     int64_t n_pages, const int64_t* k_strides, const int64_t* v_strides,
+                                     const int32_t* q_pos, int64_t window, const float* rope_freqs, float scale,
+                                     float softcap, const float* alibi_slopes, int q_dtype, int kv_dtype,
+                                     void* stream) {
+  B2_CHECK_ARG(softcap >= 0.f && isfinite(softcap), B2_ERR_INVALID,
+               "decode_attn_scored: softcap must be finite and >= 0");
+  B2_CHECK_ARG(n_pages >= 0, B2_ERR_INVALID, "decode_attn_scored: bad shape");
+  return decode_impl(q, k, v, o, page_table, seq_lens, workspace, B, Hq, Hkv, D, max_seq_len, page_size, max_pages,
+                     n_pages, k_strides, v_strides, q_pos, window, rope_freqs, scale, softcap, alibi_slopes, q_dtype,
+                     kv_dtype, stream);
 }
 
 // ---------------------------------------------------------------------------

@@ -137,5 +137,180 @@ __device__ __forceinline__ uint64_t exp2_poly_f2(uint64_t x2) {
   return (uint64_t)lo | ((uint64_t)hi << 32);
 }
 
+// ---------------------------------------------------------------------------
+// Scores with a mask of one bit per key, a cap and a distance bias, for one
+// 128-key tile; this thread's row is its TMEM lane.  In log2 units:
+//   x = scale s            or  x = cap tanh(scale s / cap)
+//   x -= slope |row - key|
+// ---------------------------------------------------------------------------
+struct Score {
+  float scale_log2;        // scale * log2 e (> 0)
+  float cap_in, cap_log2;  // 2 log2 e scale / cap; cap * log2 e
+  float slope, dist;       // slope * log2 e; row - first key of the tile
+};
+
+__device__ __forceinline__ float rcp_approx(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// cap tanh(scale s / cap) + add: tanh y = 1 - 2 / (1 + e^2y), good to ~2e-7
+// (the one-instruction tanh is good to 2^-11, which a cap of 50 turns into 0.02
+// in the exponent)
+__device__ __forceinline__ float capped(float s, const Score& c, float add) {
+  return fmaf(-2.f * c.cap_log2, rcp_approx(1.f + ex2(s * c.cap_in)), c.cap_log2 + add);
+}
+
+// Score of two neighbouring keys (e and e + 1 in the tile), plus `add`.  Where
+// MASK is false all keys of the tile lie on one side of the row, so the bias is
+// linear in the key: slope carries its sign there (slope > 0: keys before the
+// row).
+template <bool MASK, bool CAP, bool BIAS>
+__device__ __forceinline__ uint64_t score_pair(uint32_t s0, uint32_t s1, int e, const Score& c, float add) {
+  uint64_t a = f2_pack(add, add);
+  if constexpr (BIAS) {
+    if constexpr (MASK) {
+      a = f2_pack(fmaf(-c.slope, fabsf(c.dist - (float)e), add), fmaf(-c.slope, fabsf(c.dist - (float)(e + 1)), add));
+    } else {
+      const float b = fmaf(-c.slope, c.dist, add);
+      a = fma_f2(f2_pack(c.slope, c.slope), f2_pack((float)e, (float)(e + 1)), f2_pack(b, b));
+    }
+  }
+  if constexpr (CAP)
+    return f2_pack(capped(__uint_as_float(s0), c, f2_lo(a)), capped(__uint_as_float(s1), c, f2_hi(a)));
+  return fma_f2((uint64_t)s0 | ((uint64_t)s1 << 32), f2_pack(c.scale_log2, c.scale_log2), a);
+}
+
+// Largest score of the row's visible keys (bits of vis), -inf without one.
+// Scale and cap keep the order, so without a bias the raw maximum is taken and
+// scored once.  With cap and bias both, the scores are left in the S columns
+// for score_exp, so that the cap is computed once.
+template <bool MASK, bool CAP, bool BIAS>
+__device__ __forceinline__ float score_max(uint32_t tS, const uint32_t (&vis)[4], const Score& sc) {
+  float mx = -INFINITY;
+#pragma unroll 1
+  for (int c = 0; c < 4; c += 2) {
+    uint32_t sv[64];
+    tc::tmem_ld_32x32b_x32(tS + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(sv));
+    tc::tmem_ld_32x32b_x32(tS + 32 * c + 32, *reinterpret_cast<uint32_t(*)[32]>(sv + 32));
+    tc::tmem_ld_wait();
+    const uint32_t w0 = c ? vis[2] : vis[0], w1 = c ? vis[3] : vis[1];
+    Score cc = sc;
+    cc.dist -= 32.f * c;
+#pragma unroll
+    for (int e = 0; e < 64; e += 2) {
+      float v0 = __uint_as_float(sv[e]), v1 = __uint_as_float(sv[e + 1]);
+      if constexpr (BIAS) {
+        const uint64_t x = score_pair<MASK, CAP, BIAS>(sv[e], sv[e + 1], e, cc, 0.f);
+        v0 = f2_lo(x);
+        v1 = f2_hi(x);
+        if constexpr (CAP) {
+          sv[e] = (uint32_t)x;
+          sv[e + 1] = (uint32_t)(x >> 32);
+        }
+      }
+      if constexpr (MASK) {
+        const uint32_t w = e < 32 ? w0 : w1;
+        if (!(w >> (e & 31) & 1)) v0 = -INFINITY;
+        if (!(w >> ((e + 1) & 31) & 1)) v1 = -INFINITY;
+      }
+      mx = max3(mx, v0, v1);
+    }
+    if constexpr (CAP && BIAS) {
+      tmem_st_32x32b_x32(tS + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(sv));
+      tmem_st_32x32b_x32(tS + 32 * c + 32, *reinterpret_cast<uint32_t(*)[32]>(sv + 32));
+    }
+  }
+  if constexpr (CAP && BIAS) tmem_st_wait();
+  if constexpr (!BIAS) {
+    if constexpr (CAP) mx = mx == -INFINITY ? mx : capped(mx, sc, 0.f);
+    else mx *= sc.scale_log2;
+  }
+  return mx;
+}
+
+// p = exp2(score - m) as 16-bit pairs over the S columns; returns their sum.
+// P rounded to 16 bits (half a step of its own size) is what the MMA takes; the
+// sum is taken before that, in 32 bits.
+template <bool MASK, int FMT, bool CAP, bool BIAS>
+__device__ __forceinline__ float score_exp(uint32_t tS, const uint32_t (&vis)[4], float mref, const Score& sc) {
+  uint64_t rs = 0;
+#pragma unroll 1
+  for (int c = 0; c < 4; c += 2) {
+    uint32_t sv[64];
+    tc::tmem_ld_32x32b_x32(tS + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(sv));
+    tc::tmem_ld_32x32b_x32(tS + 32 * c + 32, *reinterpret_cast<uint32_t(*)[32]>(sv + 32));
+    tc::tmem_ld_wait();
+    const uint32_t w0 = c ? vis[2] : vis[0], w1 = c ? vis[3] : vis[1];
+    Score cc = sc;
+    cc.dist -= 32.f * c;
+    uint32_t pk[32];
+#pragma unroll
+    for (int e = 0; e < 32; ++e) {
+      float p0, p1;
+      uint64_t x;
+      if constexpr (CAP && BIAS) x = add_f2((uint64_t)sv[2 * e] | ((uint64_t)sv[2 * e + 1] << 32), f2_pack(-mref, -mref));
+      else x = score_pair<MASK, CAP, BIAS>(sv[2 * e], sv[2 * e + 1], 2 * e, cc, -mref);
+      if (e % 3 == 2) {  // a third of the exponentials on the FMA pipe, as in the prefill kernel
+        const uint64_t y = exp2_poly_f2(x);
+        p0 = f2_lo(y);
+        p1 = f2_hi(y);
+      } else {
+        p0 = ex2(f2_lo(x));
+        p1 = ex2(f2_hi(x));
+      }
+      if constexpr (MASK) {
+        const uint32_t w = e < 16 ? w0 : w1;
+        if (!(w >> ((2 * e) & 31) & 1)) p0 = 0.f;
+        if (!(w >> ((2 * e + 1) & 31) & 1)) p1 = 0.f;
+      }
+      rs = add_f2(rs, f2_pack(p0, p1));
+      if constexpr (FMT == kF16) {
+        __half2 hv = __floats2half2_rn(p0, p1);
+        pk[e] = *reinterpret_cast<uint32_t*>(&hv);
+      } else {
+        __nv_bfloat162 hv = __floats2bfloat162_rn(p0, p1);
+        pk[e] = *reinterpret_cast<uint32_t*>(&hv);
+      }
+    }
+    tmem_st_32x32b_x32(tS + 16 * c, pk);
+  }
+  return f2_lo(rs) + f2_hi(rs);
+}
+
+template <int FMT>
+__device__ __forceinline__ bool not_finite16(uint32_t h) {  // of the low half
+  constexpr uint32_t e = FMT == kF16 ? 0x7C00u : 0x7F80u;
+  return (h & e) == e;
+}
+// Zeroes the 16-bit values of a chunk that are infinite or NaN; true if there were any.
+template <int FMT>
+__device__ __forceinline__ bool zero_not_finite(uint4& x) {
+  uint32_t* w = reinterpret_cast<uint32_t*>(&x);
+  bool hit = false;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if (not_finite16<FMT>(w[e])) w[e] &= 0xffff0000u, hit = true;
+    if (not_finite16<FMT>(w[e] >> 16)) w[e] &= 0x0000ffffu, hit = true;
+  }
+  return hit;
+}
+template <int FMT>
+__device__ __forceinline__ float widen16(uint16_t h) {
+  if constexpr (FMT == kF16) return __half2float(__ushort_as_half(h));
+  else return __uint_as_float((uint32_t)h << 16);
+}
+template <int FMT>
+__device__ __forceinline__ uint32_t narrow2(float a, float b) {
+  if constexpr (FMT == kF16) {
+    __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<uint32_t*>(&h);
+  } else {
+    __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<uint32_t*>(&h);
+  }
+}
+
 }  // namespace fa
 }  // namespace b2

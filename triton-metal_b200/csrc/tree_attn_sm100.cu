@@ -130,97 +130,7 @@ __device__ __forceinline__ int64_t warp_sum(int64_t x) {
   return x;
 }
 
-// ------------------------------------------------------------- softmax
-// Row max of the raw scores of this thread's row, hidden keys left out.
-template <bool MASK>
-__device__ __forceinline__ float row_max_bits(uint32_t tS, const uint32_t (&vis)[4]) {
-  float mx = -INFINITY;
-#pragma unroll 1
-  for (int c = 0; c < 4; c += 2) {
-    uint32_t sv[64];
-    tc::tmem_ld_32x32b_x32(tS + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(sv));
-    tc::tmem_ld_32x32b_x32(tS + 32 * c + 32, *reinterpret_cast<uint32_t(*)[32]>(sv + 32));
-    tc::tmem_ld_wait();
-    const uint32_t w0 = c ? vis[2] : vis[0], w1 = c ? vis[3] : vis[1];
-#pragma unroll
-    for (int e = 0; e < 64; e += 2) {
-      float v0 = __uint_as_float(sv[e]), v1 = __uint_as_float(sv[e + 1]);
-      if constexpr (MASK) {
-        const uint32_t w = e < 32 ? w0 : w1;
-        if (!(w >> (e & 31) & 1)) v0 = -INFINITY;
-        if (!(w >> ((e + 1) & 31) & 1)) v1 = -INFINITY;
-      }
-      mx = max3(mx, v0, v1);
-    }
-  }
-  return mx;
-}
-
-__device__ __forceinline__ float rcp_approx(float x) {
-  float y;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-// cap tanh(scale s / cap) - m in log2 units: tanh y = 1 - 2 / (1 + e^2y), good
-// to ~2e-7 (the one-instruction tanh is good to 2^-11, which a cap of 50 turns
-// into 0.02 in the exponent)
-__device__ __forceinline__ float capped(float s, float cap_in, float cap_log2, float m) {
-  return fmaf(-2.f * cap_log2, rcp_approx(1.f + ex2(s * cap_in)), cap_log2 - m);
-}
-
-// p = exp2(score - m) as 16-bit pairs over the S columns; returns their sum.
-// P rounded to 16 bits (half a step of its own size) is what the MMA takes; the
-// sum l is taken before that, in 32 bits.
-template <bool MASK, int FMT, bool CAP>
-__device__ __forceinline__ float exp_to_p_bits(uint32_t tS, const uint32_t (&vis)[4], float mref, const Params& p) {
-  uint64_t rs = 0;
-  const uint64_t sc2 = f2_pack(p.scale_log2, p.scale_log2), nm2 = f2_pack(-mref, -mref);
-#pragma unroll 1
-  for (int c = 0; c < 4; c += 2) {
-    uint32_t sv[64];
-    tc::tmem_ld_32x32b_x32(tS + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(sv));
-    tc::tmem_ld_32x32b_x32(tS + 32 * c + 32, *reinterpret_cast<uint32_t(*)[32]>(sv + 32));
-    tc::tmem_ld_wait();
-    const uint32_t w0 = c ? vis[2] : vis[0], w1 = c ? vis[3] : vis[1];
-    uint32_t pk[32];
-#pragma unroll
-    for (int e = 0; e < 32; ++e) {
-      float p0, p1;
-      uint64_t x;
-      if constexpr (CAP) {
-        x = f2_pack(capped(__uint_as_float(sv[2 * e]), p.cap_in, p.cap_log2, mref),
-                    capped(__uint_as_float(sv[2 * e + 1]), p.cap_in, p.cap_log2, mref));
-      } else {
-        x = fma_f2((uint64_t)sv[2 * e] | ((uint64_t)sv[2 * e + 1] << 32), sc2, nm2);
-      }
-      if (e % 3 == 2) {  // a third of the exponentials on the FMA pipe, as in the prefill kernel
-        const uint64_t y = exp2_poly_f2(x);
-        p0 = f2_lo(y);
-        p1 = f2_hi(y);
-      } else {
-        p0 = ex2(f2_lo(x));
-        p1 = ex2(f2_hi(x));
-      }
-      if constexpr (MASK) {
-        const uint32_t w = e < 16 ? w0 : w1;
-        if (!(w >> ((2 * e) & 31) & 1)) p0 = 0.f;
-        if (!(w >> ((2 * e + 1) & 31) & 1)) p1 = 0.f;
-      }
-      rs = add_f2(rs, f2_pack(p0, p1));
-      if constexpr (FMT == kF16) {
-        __half2 hv = __floats2half2_rn(p0, p1);
-        pk[e] = *reinterpret_cast<uint32_t*>(&hv);
-      } else {
-        __nv_bfloat162 hv = __floats2bfloat162_rn(p0, p1);
-        pk[e] = *reinterpret_cast<uint32_t*>(&hv);
-      }
-    }
-    tmem_st_32x32b_x32(tS + 16 * c, pk);
-  }
-  return f2_lo(rs) + f2_hi(rs);
-}
-
+// ------------------------------------------------------------- masks
 // Visible keys of this thread's row among the 128 from kv0 on, as bits.  The
 // warp reads its tokens' mask rows together (lane = key) and every lane keeps
 // the ballots of its own token.
@@ -265,27 +175,6 @@ __device__ __forceinline__ bool any_of_softmax(bool x) {
   return r != 0;
 }
 __device__ __forceinline__ void softmax_sync() { asm volatile("barrier.cta.sync 2, 256;" ::: "memory"); }
-
-template <int FMT>
-__device__ __forceinline__ bool not_finite16(uint32_t h) {
-  constexpr uint32_t e = FMT == kF16 ? 0x7C00u : 0x7F80u;
-  return (h & e) == e;
-}
-template <int FMT>
-__device__ __forceinline__ float widen16(uint16_t h) {
-  if constexpr (FMT == kF16) return __half2float(__ushort_as_half(h));
-  else return __uint_as_float((uint32_t)h << 16);
-}
-template <int FMT>
-__device__ __forceinline__ uint32_t narrow2(float a, float b) {
-  if constexpr (FMT == kF16) {
-    __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<uint32_t*>(&h);
-  } else {
-    __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<uint32_t*>(&h);
-  }
-}
 
 // Element offset of key `pos` of request b and kv head hk in K or V; false when
 // its page is none of the cache's.
@@ -433,13 +322,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p) {
           if (r < first) continue;
           uint4* at = reinterpret_cast<uint4*>(sRing + (chunk_at(tile, r) - smem_u32(sRing)));
           uint4 x = *at;
-          uint32_t* w = reinterpret_cast<uint32_t*>(&x);
-          bool hit = false;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            if (not_finite16<FMT>(w[e])) w[e] &= 0xffff0000u, hit = true;
-            if (not_finite16<FMT>(w[e] >> 16)) w[e] &= 0x0000ffffu, hit = true;
-          }
+          const bool hit = zero_not_finite<FMT>(x);
           if (hit) *at = x;
           bad |= hit;
         }
@@ -627,6 +510,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p) {
     const int u = (warp - 4) >> 2, qw = warp & 3, r = qw * 32 + lane;
     const uint32_t lane_off = (uint32_t)(qw * 32) << 16;
     const uint32_t tS = tmem + 256 * u + lane_off, tO = tmem + 128 + lane_off;  // tO: of unit 0
+    const Score score = {p.scale_log2, p.cap_in, p.cap_log2, 0.f, 0.f};
     uint32_t sc = 0, oc[2] = {0, 0}, seg = 0;  // S tiles / O accumulators waited for
     bool ok = true;
     while (walk.next(p, kRows, sg)) {
@@ -652,10 +536,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p) {
           const bool masked = kv0 + BK > sg.ctx;
           uint32_t vis[4];
           if (masked) visible_bits(vis, mask, p.T, t, t0, t1, kv0, sg.ctx, sg.dl, row_ok);
-          float mx = masked ? row_max_bits<true>(tS, vis) : row_max_bits<false>(tS, vis);
-          // scale > 0 and tanh keep the order
-          if constexpr (CAP) mx = mx == -INFINITY ? mx : capped(mx, p.cap_in, p.cap_log2, 0.f);
-          else mx *= p.scale_log2;
+          const float mx = masked ? score_max<true, CAP, false>(tS, vis, score) : score_max<false, CAP, false>(tS, vis, score);
           const bool need = mx > m_used + kRescale;
           const float alpha = need ? (m_used == -INFINITY ? 0.f : ex2(m_used - mx)) : 1.f;
           if (need) {
@@ -675,7 +556,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p) {
             }
           }
           const float mref = m_used == -INFINITY ? 0.f : m_used;
-          l += masked ? exp_to_p_bits<true, FMT, CAP>(tS, vis, mref, p) : exp_to_p_bits<false, FMT, CAP>(tS, vis, mref, p);
+          l += masked ? score_exp<true, FMT, CAP, false>(tS, vis, mref, score)
+                      : score_exp<false, FMT, CAP, false>(tS, vis, mref, score);
           tmem_st_wait();
         }
         first = false;
