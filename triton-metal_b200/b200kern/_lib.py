@@ -168,6 +168,21 @@ class on_device:
         return False
 
 
+def fast_call(name, entry, *args):
+    """The common case of an operator through _b2fast; None when it is not one
+    (or the binding is not built)."""
+    m = fast()
+    if m is None:
+        return None
+    try:
+        r = getattr(m, name)(*args)
+    except TypeError:  # an argument of another kind: the operator's own checks say which
+        return None
+    if r.__class__ is int:
+        check(r, entry)
+    return r
+
+
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 

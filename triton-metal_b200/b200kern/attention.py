@@ -65,6 +65,13 @@ def flash_attention(q, k, v, causal=False, scale=None, out=None, window=0, softc
     With any of these, hidden keys do not count whatever their values, fp32
     inputs are computed in fp32 on the CUDA cores at every head dim, and scale
     may have any sign."""
+    scored = softcap or alibi_slopes is not None or doc_offsets is not None or prefix_lens is not None
+    if scored:
+        r = _lib.fast_call("flash_scored", "b2_flash_attn_fwd_scored", q, k, v, causal,
+                           1.0 / math.sqrt(q.shape[-1]) if scale is None else scale, window, softcap, alibi_slopes,
+                           doc_offsets, prefix_lens, out)
+        if r is not None:
+            return r
     for t in (q, k, v):
         if not t.is_cuda:
             raise B2ShapeError("b200kern ops take CUDA tensors (there is no CPU path)")
@@ -90,7 +97,7 @@ def flash_attention(q, k, v, causal=False, scale=None, out=None, window=0, softc
     os_ = _lib.strides_arg(o.stride()[:3])
     if window and (not causal or window < 0):
         raise B2ShapeError("a sliding window needs causal=True and window > 0")
-    if softcap or alibi_slopes is not None or doc_offsets is not None or prefix_lens is not None:
+    if scored:
         return _flash_scored(q, k, v, o, qs, ks, vs, os_, causal, scale, window, softcap, alibi_slopes, doc_offsets,
                              prefix_lens)
     if window:
@@ -177,6 +184,11 @@ def decode_attention(q, k_cache, v_cache, seq_lens, scale=None, page_table=None,
     softcap > 0 caps the scores, softcap * tanh(scale q.k / softcap);
     alibi_slopes fp32 [Hq] then subtracts slope * |q_pos - key|.  A page number
     outside a paged cache reads as zeros and shows in b2_device_error."""
+    if q_pos is None and rope_freqs is None and not window and isinstance(seq_lens, torch.Tensor):
+        r = _lib.fast_call("decode_attention", "b2_decode_attn_scored", q, k_cache, v_cache, seq_lens, page_table,
+                           1.0 / math.sqrt(q.shape[-1]) if scale is None else scale, softcap, alibi_slopes, out)
+        if r is not None:
+            return r
     for t in (q, k_cache, v_cache):
         if not t.is_cuda:
             raise B2ShapeError("b200kern ops take CUDA tensors (there is no CPU path)")
@@ -246,6 +258,10 @@ def tree_attention(q, k_cache, v_cache, context_lens, tree_mask, draft_lens=None
     a page number outside the cache reads as zeros and shows in
     b2_device_error.  Hidden keys do not count, whatever their values.
     """
+    r = _lib.fast_call("tree_attention", "b2_tree_attn", q, k_cache, v_cache, context_lens, tree_mask, draft_lens,
+                       page_table, 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale, softcap, out)
+    if r is not None:
+        return r
     if q.dim() != 4 or k_cache.dim() != 4 or k_cache.shape != v_cache.shape:
         raise B2ShapeError("tree_attention takes q [B, T, Hq, D] and two 4-d caches of one shape")
     if q.dtype not in _DT or k_cache.dtype not in _DT or v_cache.dtype != k_cache.dtype:

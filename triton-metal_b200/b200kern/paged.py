@@ -45,6 +45,10 @@ def build_page_table(context_lens, new_lens, page_size, free_pages, page_table, 
     with the pages they would open.  One launch, no synchronisation; a step
     captured in a CUDA graph follows the lengths of each replay.
     """
+    r = _lib.fast_call("build_page_table", "b2_build_page_table", context_lens, new_lens, page_size, free_pages,
+                       page_table, max_tokens)
+    if r is not None:
+        return r
     _lens(context_lens, "context_lens")
     _lens(new_lens, "new_lens")
     _lens(free_pages, "free_pages")
@@ -94,6 +98,9 @@ def store_kv(k, v, k_pages, v_pages, slots):
     occur once in a call; which of several rows for one slot stays is not
     defined.  Nothing else of the cache is touched.
     """
+    r = _lib.fast_call("store_kv", "b2_store_kv", k, v, k_pages, v_pages, slots)
+    if r is not None:
+        return r
     for name, t in (("k", k), ("v", v)):
         if t.dim() != 3 or t.shape != k.shape or t.dtype != k.dtype:
             raise B2ShapeError("k and v must be [N, Hkv, D] of one shape and dtype")
