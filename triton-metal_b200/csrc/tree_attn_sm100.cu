@@ -39,6 +39,7 @@ using namespace fa;
 constexpr int kThreads = 416;
 constexpr int BR = 128, BK = 128;          // rows and keys of a tile
 constexpr float kRescale = 8.f;            // log2 units: P holds up to 2^8
+constexpr int kItemCost = 2;               // what starting and ending an item costs, in tiles
 
 template <int HD>
 struct Cfg {
@@ -73,17 +74,19 @@ struct Params {
 // ------------------------------------------------------------- schedule
 // Items of request b: hk-major, then row tile.  A row tile with drafted tokens
 // has all of the request's key tiles, one without has a single tile in which
-// nothing is visible (its rows become 0).
+// nothing is visible (its rows become 0).  The line that the CTAs share is made
+// of units: kItemCost units that stand for an item's start and end, then its
+// tiles.
 struct Req {
   int ctx, dl, tiles, full;  // key tiles, row tiles with drafted tokens
-  int per_head;              // tiles of one kv head
+  int per_head;              // units of one kv head
 };
 __device__ __forceinline__ Req request(const Params& p, int b, int rows_per_item) {
   Req r;
   attn::tree_lens(p.ctx, p.draft, b, p.T, p.cap, r.ctx, r.dl);
   r.tiles = (r.ctx + r.dl + BK - 1) / BK;
   r.full = (r.dl * p.rep + rows_per_item - 1) / rows_per_item;
-  r.per_head = r.full * r.tiles + (p.n_rt - r.full);
+  r.per_head = r.full * (r.tiles + kItemCost) + (p.n_rt - r.full) * (1 + kItemCost);
   return r;
 }
 
@@ -92,37 +95,47 @@ struct Segment {
   int ctx, dl, keys;           // keys = ctx + dl, 0 when the item has no drafted token
 };
 
-// Walks the segments of the run [g, g1).
+// Walks the segments of the run [g, g1) of units.
 struct Walk {
-  int64_t g, g1, start;  // start: first tile of request b
+  int64_t g, g1, start;  // start: first unit of request b
   int b;
   Req r;
   __device__ __forceinline__ bool next(const Params& p, int rows_per_item, Segment& s) {
-    if (g >= g1) return false;
-    while (g >= start + (int64_t)r.per_head * p.Hkv) {
-      start += (int64_t)r.per_head * p.Hkv;
-      r = request(p, ++b, rows_per_item);
+    while (g < g1) {
+      while (g >= start + (int64_t)r.per_head * p.Hkv) {
+        start += (int64_t)r.per_head * p.Hkv;
+        r = request(p, ++b, rows_per_item);
+      }
+      const uint32_t local = (uint32_t)(g - start);
+      s.b = b;
+      s.hk = local / (uint32_t)r.per_head;
+      int rem = local - (uint32_t)s.hk * r.per_head;
+      const int size = r.tiles + kItemCost;
+      const bool has = rem < r.full * size;
+      if (!has) rem -= r.full * size;
+      s.of = has ? r.tiles : 1;
+      s.rt = rem / (s.of + kItemCost);
+      const int at = rem - s.rt * (s.of + kItemCost);  // unit within the item
+      if (!has) s.rt += r.full;
+      const int end = (int)min((int64_t)(s.of + kItemCost), at + (g1 - g));
+      s.tile = max(at - kItemCost, 0);
+      s.n = max(end - kItemCost, 0) - s.tile;
+      s.ctx = r.ctx;
+      s.dl = has ? r.dl : 0;
+      s.keys = has ? r.ctx + r.dl : 0;
+      g += end - at;
+      if (s.n > 0) return true;  // else the run ends before the item's first tile
     }
-    const uint32_t local = (uint32_t)(g - start);
-    s.b = b;
-    s.hk = local / (uint32_t)r.per_head;
-    const int rem = local - (uint32_t)s.hk * r.per_head;
-    const bool has = rem < r.full * r.tiles;
-    s.rt = has ? rem / r.tiles : r.full + rem - r.full * r.tiles;
-    s.tile = has ? rem - s.rt * r.tiles : 0;
-    s.of = has ? r.tiles : 1;
-    s.n = (int)min((int64_t)(s.of - s.tile), g1 - g);
-    s.ctx = r.ctx;
-    s.dl = has ? r.dl : 0;
-    s.keys = has ? r.ctx + r.dl : 0;
-    g += s.n;
-    return true;
+    return false;
   }
 };
 
-// First tile of CTA c's run when G CTAs share W tiles (G <= W, so that no run
+// First unit of CTA c's run when G CTAs share W units (G <= W, so that no run
 // is empty).
-__device__ __forceinline__ int64_t run_start(int64_t c, int64_t W, int64_t G) { return c * W / G; }
+__device__ __forceinline__ int64_t run_start(int64_t c, int64_t W, int64_t G) {
+  const int64_t n = c * W;
+  return n >> 32 == 0 ? (uint32_t)n / (uint32_t)G : n / G;
+}
 
 __device__ __forceinline__ int64_t warp_sum(int64_t x) {
 #pragma unroll
@@ -131,29 +144,51 @@ __device__ __forceinline__ int64_t warp_sum(int64_t x) {
 }
 
 // ------------------------------------------------------------- masks
-// Visible keys of this thread's row among the 128 from kv0 on, as bits.  The
-// warp reads its tokens' mask rows together (lane = key) and every lane keeps
-// the ballots of its own token.
-__device__ __forceinline__ void visible_bits(uint32_t (&vis)[4], const uint8_t* mask, int T, int t, int t0, int t1,
-                                             int kv0, int ctx, int dl, bool row_ok) {
+// Drafted tokens j0 .. j0 + 127 that this thread's row sees, as bits.  The warp
+// reads the mask rows of its tokens t0 .. t1 together (lane = drafted token),
+// eight rows in flight, and every lane keeps the ballots of its own token t.
+__device__ __forceinline__ void draft_bits(uint32_t (&bits)[4], const uint8_t* mask, int T, int t, int t0, int t1,
+                                           int j0, int dl, bool row_ok) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
-  for (int w = 0; w < 4; ++w) vis[w] = 0;
-  for (int tt = t0; tt <= t1; ++tt) {
-    const uint8_t* row = mask + (int64_t)tt * T;
-    bool see[4];
+  for (int w = 0; w < 4; ++w) bits[w] = 0;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const int j = kv0 + 32 * w + lane - ctx;
-      see[w] = j < 0 || (j < dl && row[j] != 0);
-    }
+  for (int w = 0; w < 4; ++w) {
+    const int j = j0 + 32 * w + lane;
+    if (j0 + 32 * w >= dl) break;  // the same for the warp
+    for (int tt = t0; tt <= t1; tt += 8) {
+      bool see[8];
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const uint32_t bits = __ballot_sync(0xffffffffu, see[w]);
-      if (tt == t) vis[w] = bits;
+      for (int i = 0; i < 8; ++i) see[i] = j >= 0 && j < dl && tt + i <= t1 && mask[(int64_t)(tt + i) * T + j] != 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t b = __ballot_sync(0xffffffffu, see[i]);
+        if (tt + i == t) bits[w] = b;
+      }
     }
   }
-  if (!row_ok) vis[0] = vis[1] = vis[2] = vis[3] = 0;
+  if (!row_ok) bits[0] = bits[1] = bits[2] = bits[3] = 0;
+}
+
+// Visible keys among the 128 from drafted token j0 (negative: context) on, from
+// the bits of the first 128 drafted tokens.
+__device__ __forceinline__ void visible_bits(uint32_t (&vis)[4], const uint32_t (&bits)[4], int j0, bool row_ok) {
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const int j = j0 + 32 * w;
+    uint32_t x;
+    if (j <= -32) {
+      x = 0xffffffffu;
+    } else if (j < 0) {
+      x = ((1u << -j) - 1) | bits[0] << -j;
+    } else {
+      const int i = j >> 5;
+      const uint32_t lo = i == 0 ? bits[0] : i == 1 ? bits[1] : i == 2 ? bits[2] : i == 3 ? bits[3] : 0;
+      const uint32_t hi = i == 0 ? bits[1] : i == 1 ? bits[2] : i == 2 ? bits[3] : 0;
+      x = __funnelshift_r(lo, hi, j & 31);
+    }
+    vis[w] = row_ok ? x : 0;
+  }
 }
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
@@ -176,12 +211,16 @@ __device__ __forceinline__ bool any_of_softmax(bool x) {
 }
 __device__ __forceinline__ void softmax_sync() { asm volatile("barrier.cta.sync 2, 256;" ::: "memory"); }
 
-// Element offset of key `pos` of request b and kv head hk in K or V; false when
-// its page is none of the cache's.
-__device__ __forceinline__ bool key_offset(const Params& p, int b, int hk, int pos, int64_t& ko, int64_t& vo) {
+// Page table entry of key `pos` of request b (contiguous: 0).
+__device__ __forceinline__ int key_page(const Params& p, int b, int pos) {
+  return p.page_size ? p.page_table[(int64_t)b * p.max_pages + (uint32_t)pos / p.page_size] : 0;
+}
+
+// Element offset of key `pos` of request b and kv head hk in K or V, given its
+// page; false when that is none of the cache's.
+__device__ __forceinline__ bool key_offset(const Params& p, int b, int hk, int pos, int pg, int64_t& ko, int64_t& vo) {
   if (p.page_size) {
-    const uint32_t pi = (uint32_t)pos / p.page_size, at = (uint32_t)pos - pi * p.page_size;
-    const int pg = p.page_table[(int64_t)b * p.max_pages + pi];
+    const uint32_t at = (uint32_t)pos % p.page_size;
     ko = pg * p.ks[0] + at * p.ks[1] + hk * p.ks[2];
     vo = pg * p.vs[0] + at * p.vs[1] + hk * p.vs[2];
     return pg >= 0 && pg < p.n_pages;
@@ -222,6 +261,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p) {
   uint8_t* sRing = sQ + 2 * C::kTile;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
+  // the joining kernel may start (it waits for this one's end)
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (tid == 0) {
     for (int i = 0; i < NS; ++i) {
       mbar_init(&full[i], 128);
@@ -242,18 +283,38 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p) {
     tc::tmem_alloc(tmem_holder, 512);
     tc::tmem_relinquish();
   }
-  // this CTA's run: the number of tiles, then the request its first tile is in
-  int64_t sum = 0;
-  for (int b = tid; b < p.B; b += kThreads) sum += (int64_t)request(p, b, kRows).per_head * p.Hkv;
-  sum = warp_sum(sum);
-  if (lane == 0) s_run[warp] = sum;
+  // this CTA's run, and the request that its first unit is in: a scan over the
+  // requests' units, in rounds of one request a thread
+  int64_t mine = 0;
+  if (tid < p.B) mine = (int64_t)request(p, tid, kRows).per_head * p.Hkv;
+  auto scan = [&](int64_t x, int64_t& total) {  // sum over the threads before this one
+    int64_t inc = x;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const int64_t a = __shfl_up_sync(0xffffffffu, inc, off);
+      if (lane >= off) inc += a;
+    }
+    __syncthreads();  // s_run of the round before is read
+    if (lane == 31) s_run[warp] = inc;
+    __syncthreads();
+    int64_t before = inc - x;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < kThreads / 32; ++w) {
+      if (w < warp) before += s_run[w];
+      total += s_run[w];
+    }
+    return before;
+  };
   tc::fence_before_sync();
-  __syncthreads();
+  int64_t round = 0, start = scan(mine, round), W = round;
   tc::fence_after_sync();
   const uint32_t tmem = *tmem_holder;
-  int64_t W = 0;
-#pragma unroll
-  for (int w = 0; w < kThreads / 32; ++w) W += s_run[w];
+  for (int b0 = kThreads; b0 < p.B; b0 += kThreads) {
+    int64_t t;
+    scan(b0 + tid < p.B ? (int64_t)request(p, b0 + tid, kRows).per_head * p.Hkv : 0, t);
+    W += t;
+  }
   const int64_t G = min((int64_t)gridDim.x, W);
   Walk walk;
   walk.g = walk.g1 = 0;
@@ -265,28 +326,17 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p) {
   if (!fits && tid == 0) atomicCAS(p.err, 0u, 0xB2400001u);
   const bool some = walk.g < walk.g1 && fits;
   if (some) {
-    int64_t before = 0;
-    for (int b0 = 0; b0 < p.B; b0 += kThreads) {
-      const int b = b0 + tid;
-      const int64_t mine = b < p.B ? (int64_t)request(p, b, kRows).per_head * p.Hkv : 0;
-      int64_t inc = mine;
-#pragma unroll
-      for (int off = 1; off < 32; off <<= 1) {
-        const int64_t a = __shfl_up_sync(0xffffffffu, inc, off);
-        if (lane >= off) inc += a;
+    int64_t before = 0;  // units of the rounds before
+    for (int b0 = 0;; b0 += kThreads) {
+      if (b0) {
+        mine = b0 + tid < p.B ? (int64_t)request(p, b0 + tid, kRows).per_head * p.Hkv : 0;
+        start = before + scan(mine, round);
       }
-      __syncthreads();  // s_run of the round before is read
-      if (lane == 31) s_run[warp] = inc;
-      __syncthreads();
-      int64_t start = before + inc - mine;
-      for (int w = 0; w < kThreads / 32; ++w) {
-        if (w < warp) start += s_run[w];
-        before += s_run[w];
-      }
-      if (mine > 0 && start <= walk.g && walk.g < start + mine) {
-        *s_b = b;
+      if (start <= walk.g && walk.g < start + mine) {
+        *s_b = b0 + tid;
         s_run[15] = start;
       }
+      before += round;
       if (before > walk.g) break;  // the same for every thread
     }
     __syncthreads();
@@ -296,8 +346,12 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p) {
   }
 
   Segment sg;
+  // Registers: 13 warps are launched with 128 a thread (53,248); the copying
+  // warpgroup gives some up to the two softmax warpgroups, which would spill:
+  // 128 x 88 + 256 x 144 + 32 x 128 = 52,224.
   if (some && warp < 4) {
     // --------------------------------- copies ---------------------------------
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     constexpr int CH = HD / 8, RPP = 32 / CH;  // 16-byte chunks of a row, rows a warp copies at once
     const int cc = lane % CH, rsub = lane / CH;
     uint32_t seq = 0, handed = 0;  // tiles issued / handed over
@@ -370,17 +424,20 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p) {
                         wait_abort(&epi_done[prev & 1], (prev >> 1) & 1, p.err, 0xB2400003u, abort_flag));
         if (!ok) break;
       }
-      // this lane's key of each tile, one tile ahead
+      // this lane's key of each tile, one tile ahead, and its page, two ahead
       int64_t ko, vo, ko1 = -1, vo1 = -1;
-      auto locate = [&](int tile, int64_t& a, int64_t& c) {
-        const int pos = (sg.tile + tile) * BK + 32 * warp + lane;
+      auto key = [&](int tile) { return (sg.tile + tile) * BK + 32 * warp + lane; };
+      auto page = [&](int tile) { return tile < sg.n && key(tile) < sg.keys ? key_page(p, sg.b, key(tile)) : 0; };
+      auto locate = [&](int tile, int pg, int64_t& a, int64_t& c) {
         a = c = -1;
-        if (tile < sg.n && pos < sg.keys && !key_offset(p, sg.b, sg.hk, pos, a, c)) {
+        if (key(tile) < sg.keys && !key_offset(p, sg.b, sg.hk, key(tile), pg, a, c)) {
           atomicCAS(p.err, 0u, attn::kErrPage);
           a = c = -1;
         }
       };
-      locate(0, ko, vo);
+      const int pg0 = page(0);
+      int pg1 = page(1);
+      locate(0, pg0, ko, vo);
       uint32_t tile = begin();
       if (!ok) break;
 #pragma unroll 1
@@ -398,7 +455,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p) {
       end(255);
       for (int i = 0; i < sg.n && ok; ++i) {
         if (i + 1 < sg.n) {
-          locate(i + 1, ko1, vo1);
+          locate(i + 1, pg1, ko1, vo1);
+          pg1 = page(i + 2);
           tile = begin();
           if (!ok) break;
           copy_tile(tile, p.k, ko1);
@@ -507,6 +565,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p) {
     }
   } else if (some) {
     // --------------------------------- softmax ---------------------------------
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 144;");
     const int u = (warp - 4) >> 2, qw = warp & 3, r = qw * 32 + lane;
     const uint32_t lane_off = (uint32_t)(qw * 32) << 16;
     const uint32_t tS = tmem + 256 * u + lane_off, tO = tmem + 128 + lane_off;  // tO: of unit 0
@@ -523,6 +582,11 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p) {
       const int t0 = (rt * BR + qw * 32) / p.rep, t1 = min((rt * BR + qw * 32 + 31) / p.rep, sg.dl - 1);
       const bool warp_ok = t0 < sg.dl && rt * BR + qw * 32 < p.R;
       const uint8_t* mask = p.mask + sg.b * p.mask_stride;
+      // mask bits of the first 128 drafted tokens, read while the first keys are
+      // still on their way (wider trees read theirs tile by tile)
+      uint32_t drafted[4] = {0, 0, 0, 0};
+      if (warp_ok && (sg.tile + sg.n) * BK > sg.ctx)
+        draft_bits(drafted, mask, p.T, t, t0, t1, 0, min(sg.dl, 128), row_ok);
       float m_used = -INFINITY, l = 0.f;
       bool first = true;
       const int step = PAIR ? 1 : 2;
@@ -535,7 +599,17 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p) {
           const int kv0 = (sg.tile + j) * BK;
           const bool masked = kv0 + BK > sg.ctx;
           uint32_t vis[4];
-          if (masked) visible_bits(vis, mask, p.T, t, t0, t1, kv0, sg.ctx, sg.dl, row_ok);
+          if (masked) {
+            if (sg.dl <= 128 || kv0 + BK <= sg.ctx + 128) {
+              visible_bits(vis, drafted, kv0 - sg.ctx, row_ok);
+            } else {
+              draft_bits(vis, mask, p.T, t, t0, t1, kv0 - sg.ctx, sg.dl, row_ok);
+              uint32_t before[4];
+              visible_bits(before, drafted, kv0 - sg.ctx, row_ok);
+#pragma unroll
+              for (int w = 0; w < 4; ++w) vis[w] |= before[w];
+            }
+          }
           const float mx = masked ? score_max<true, CAP, false>(tS, vis, score) : score_max<false, CAP, false>(tS, vis, score);
           const bool need = mx > m_used + kRescale;
           const float alpha = need ? (m_used == -INFINITY ? 0.f : ex2(m_used - mx)) : 1.f;
@@ -587,27 +661,43 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p) {
         ok = ok && __all_sync(0xffffffffu, wait_abort(&o_done[x], oc[x] & 1, p.err, 0xB240000Au, abort_flag));
         ++oc[x];
       }
-      if (ok && (!PAIR || u < units)) {
+      if (ok && (!PAIR || u < units) && rt * BR + qw * 32 < p.R) {
         tc::fence_after_sync();
         const bool whole = sg.n == sg.of;  // else a partial: before the run's first item border, or behind its last
         const bool bad = s_bad[seg & 1] == seg;
         const float inv = L > 0.f || L != L ? 1.f / L : 0.f;
         constexpr int kCols = PAIR ? HD : HD / 2;
         const int c0 = PAIR ? 0 : u * kCols;
-        uint16_t* out = nullptr;
-        float* part = nullptr;
-        const int prow = PAIR ? u * BR + r : r;
+        // Rows leave through shared memory (Q's tile, which the segment no longer
+        // needs): 32 rows of SB bytes a warp, so that a store instruction writes
+        // whole 128-byte lines instead of 16 bytes of 32 rows.
+        constexpr int SB = HD == 128 || PAIR ? 128 : 64, CPR = SB / 16;
+        uint8_t* stage = sQ + (PAIR ? u : seg & 1) * C::kTile + (PAIR ? qw : 4 * u + qw) * 32 * SB;
+        auto staged = [&](int rr, int ch) { return reinterpret_cast<uint4*>(stage + rr * SB + ((ch ^ (rr / (8 / CPR) & (CPR - 1))) << 4)); };
+        uint8_t* dst = nullptr;  // of this lane's row
         if (whole) {
-          if (row < p.R) out = p.o + sg.b * p.os[0] + (int64_t)t * p.os[1] + (int64_t)(sg.hk * p.rep + row - t * p.rep) * p.os[2];
+          if (row < p.R)
+            dst = reinterpret_cast<uint8_t*>(p.o + sg.b * p.os[0] + (int64_t)t * p.os[1] + (int64_t)(sg.hk * p.rep + row - t * p.rep) * p.os[2]);
         } else {
           const int64_t slot = 2 * (int64_t)blockIdx.x + (sg.tile == 0 ? 1 : 0);
           float* w = p.ws + slot * (kRows * (HD + 2));
+          const int prow = PAIR ? u * BR + r : r;
           if (PAIR || u == 0) {
             w[kRows * HD + prow] = row_ok ? M : -INFINITY;
             w[kRows * HD + kRows + prow] = row_ok ? L : 0.f;
           }
-          part = w + prow * HD;
+          if (row < p.R) dst = reinterpret_cast<uint8_t*>(w + prow * HD);
         }
+        auto flush = [&](int at) {  // SB bytes of every row, to byte `at` of it
+          __syncwarp();
+#pragma unroll
+          for (int k = 0; k < CPR; ++k) {
+            const int rr = k * (32 / CPR) + lane / CPR, ch = lane % CPR;
+            uint8_t* to = reinterpret_cast<uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dst), rr));
+            if (to) *reinterpret_cast<uint4*>(to + at + ch * 16) = *staged(rr, ch);
+          }
+          __syncwarp();
+        };
 #pragma unroll 1
         for (int c = c0; c < c0 + kCols; c += 32) {
           float o[32];
@@ -631,7 +721,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p) {
             const int j0 = max(sg.tile * BK - sg.ctx, 0), j1 = min((sg.tile + sg.n) * BK - sg.ctx, sg.dl);
             for (int j = j0; j < j1; ++j) {
               int64_t ko, vo;
-              if (!mask[(int64_t)t * p.T + j] || !key_offset(p, sg.b, sg.hk, sg.ctx + j, ko, vo)) continue;
+              if (!mask[(int64_t)t * p.T + j]) continue;
+              if (!key_offset(p, sg.b, sg.hk, sg.ctx + j, key_page(p, sg.b, sg.ctx + j), ko, vo)) continue;
 #pragma unroll
               for (int e = 0; e < 32; ++e) {
                 const uint16_t h = p.v[vo + c + e];
@@ -643,19 +734,25 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p) {
 #pragma unroll
             for (int e = 0; e < 32; ++e) o[e] = 0.f;
           }
-          if (out) {
-            uint4* dst = reinterpret_cast<uint4*>(out + c);
+          if (whole) {  // 64 bytes of the row
+            const int first = (c - c0) % (SB / 2) / 8;
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              dst[e] = make_uint4(narrow2<FMT>(o[8 * e] * inv, o[8 * e + 1] * inv),
-                                  narrow2<FMT>(o[8 * e + 2] * inv, o[8 * e + 3] * inv),
-                                  narrow2<FMT>(o[8 * e + 4] * inv, o[8 * e + 5] * inv),
-                                  narrow2<FMT>(o[8 * e + 6] * inv, o[8 * e + 7] * inv));
-          }
-          if (part) {
-            float4* dst = reinterpret_cast<float4*>(part + c);
+              *staged(lane, first + e) = make_uint4(narrow2<FMT>(o[8 * e] * inv, o[8 * e + 1] * inv),
+                                                    narrow2<FMT>(o[8 * e + 2] * inv, o[8 * e + 3] * inv),
+                                                    narrow2<FMT>(o[8 * e + 4] * inv, o[8 * e + 5] * inv),
+                                                    narrow2<FMT>(o[8 * e + 6] * inv, o[8 * e + 7] * inv));
+            if (first + 4 == CPR) flush((c + 32) * 2 - SB);
+          } else {  // 128 bytes
 #pragma unroll
-            for (int e = 0; e < 8; ++e) dst[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+            for (int h = 0; h < 8 / CPR; ++h) {
+#pragma unroll
+              for (int e = 0; e < CPR; ++e) {
+                const float* x = o + h * (SB / 4) + 4 * e;
+                *staged(lane, e) = make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+              }
+              flush(c * 4 + h * SB);
+            }
           }
         }
       }
@@ -675,9 +772,19 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p) {
   }
 }
 
+// floor((a + b - 1) / b): 32-bit where it fits, since a 64-bit division costs
+// about as much as a load from L2
+__device__ __forceinline__ int64_t ceil_div(int64_t a, int64_t b) {
+  const int64_t n = a + b - 1;
+  if (n >> 32 == 0) return (uint32_t)n / (uint32_t)b;
+  return n / b;
+}
+
 // Joins the partials of the items that several CTAs shared:
 // o = sum_c 2^{m_c - M} o_c / sum_c 2^{m_c - M} l_c.  One CTA per item and kJoin
-// rows, a warp per row.
+// rows, four rows a warp, whose loads are in flight together.  Launched while
+// the first kernel still runs (programmatic dependent launch): it finds its
+// place in the schedule, then waits for that kernel's end.
 constexpr int kJoin = 16;
 template <int HD, int FMT, bool PAIR>
 __global__ void __launch_bounds__(128) tree_join_kernel(const Params p, int64_t G) {
@@ -685,7 +792,7 @@ __global__ void __launch_bounds__(128) tree_join_kernel(const Params p, int64_t 
   __shared__ int64_t s_w[4], s_before[4];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int b = blockIdx.y, rt = blockIdx.x % p.n_rt, hk = blockIdx.x / p.n_rt % p.Hkv;
-  const int row0 = blockIdx.x / p.n_rt / p.Hkv * kJoin;
+  const int row0 = blockIdx.x / p.n_rt / p.Hkv * kJoin + warp * 4;
   int64_t W = 0, before = 0;
   for (int i = tid; i < p.B; i += 128) {
     const int64_t n = (int64_t)request(p, i, kRows).per_head * p.Hkv;
@@ -702,41 +809,59 @@ __global__ void __launch_bounds__(128) tree_join_kernel(const Params p, int64_t 
   W = s_w[0] + s_w[1] + s_w[2] + s_w[3];
   before = s_before[0] + s_before[1] + s_before[2] + s_before[3];
   const Req r = request(p, b, kRows);
+  // before any way out, so that this kernel never ends before the first one
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   if (rt >= r.full) return;  // one tile: written by its CTA
-  const int64_t g0 = before + (int64_t)hk * r.per_head + (int64_t)rt * r.tiles, g1 = g0 + r.tiles;
+  const int64_t g0 = before + (int64_t)hk * r.per_head + (int64_t)rt * (r.tiles + kItemCost) + kItemCost;
+  const int64_t g1 = g0 + r.tiles;  // the item's tiles as units
   G = min(G, W);
-  // CTA of tile g: the last one whose run starts at or before it
-  const int64_t ca = ((g0 + 1) * G + W - 1) / W - 1, cz = (g1 * G + W - 1) / W - 1;
+  // CTA of unit g: the last one whose run starts at or before it
+  const int ca = (int)ceil_div((g0 + 1) * G, W) - 1, cz = (int)ceil_div(g1 * G, W) - 1;
   if (ca == cz) return;  // a single segment: written by its CTA
   constexpr int V = HD / 32;  // columns a lane
   const int64_t stride = kRows * (HD + 2);
-  for (int i = warp; i < kJoin; i += 4) {
-    const int in = row0 + i, row = rt * kRows + in;
-    if (in >= kRows || row >= p.R) return;
-    float M = -INFINITY;
-    for (int64_t c = ca; c <= cz; ++c) M = fmaxf(M, p.ws[(2 * c + (c == ca)) * stride + kRows * HD + in]);
-    const float ref = M == -INFINITY ? 0.f : M;
-    float acc[V], L = 0.f;
+  float m[4], l[4], acc[4][V];
 #pragma unroll
-    for (int e = 0; e < V; ++e) acc[e] = 0.f;
-    for (int64_t c = ca; c <= cz; ++c) {
-      const float* w = p.ws + (2 * c + (c == ca)) * stride;
-      const float l = w[kRows * HD + kRows + in];
-      if (l == 0.f) continue;
-      const float f = ex2(w[kRows * HD + in] - ref);
-      L = fmaf(f, l, L);
-      float x[V];
-      if constexpr (V == 4) *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(w + in * HD + lane * V);
-      else *reinterpret_cast<float2*>(x) = *reinterpret_cast<const float2*>(w + in * HD + lane * V);
+  for (int i = 0; i < 4; ++i) {
+    m[i] = -INFINITY;
+    l[i] = 0.f;
 #pragma unroll
-      for (int e = 0; e < V; ++e) acc[e] = fmaf(f, x[e], acc[e]);
+    for (int e = 0; e < V; ++e) acc[i][e] = 0.f;
+  }
+  // rows behind the item's last (row0 + 4 > kRows cannot be) hold (-inf, 0)
+  // partials or are not stored below
+  for (int c = ca; c <= cz; ++c) {
+    const float* w = p.ws + (2 * (int64_t)c + (c == ca)) * stride;
+    float mc[4], lc[4], x[4][V];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      mc[i] = w[kRows * HD + row0 + i];
+      lc[i] = w[kRows * HD + kRows + row0 + i];
+      const float* o = w + (row0 + i) * HD + lane * V;
+      if constexpr (V == 4) *reinterpret_cast<float4*>(x[i]) = *reinterpret_cast<const float4*>(o);
+      else *reinterpret_cast<float2*>(x[i]) = *reinterpret_cast<const float2*>(o);
     }
-    const float inv = L == 0.f ? 0.f : 1.f / L;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (lc[i] == 0.f) continue;  // saw nothing
+      const float mn = fmaxf(m[i], mc[i]), ref = mn == -INFINITY ? 0.f : mn;
+      const float fa = m[i] == -INFINITY ? 0.f : ex2(m[i] - ref), fb = ex2(mc[i] - ref);
+      m[i] = mn;
+      l[i] = l[i] * fa + lc[i] * fb;
+#pragma unroll
+      for (int e = 0; e < V; ++e) acc[i][e] = acc[i][e] * fa + x[i][e] * fb;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = rt * kRows + row0 + i;
+    if (row >= p.R) return;
+    const float inv = l[i] == 0.f ? 0.f : 1.f / l[i];
     const int t = row / p.rep;
     uint16_t* o = p.o + b * p.os[0] + (int64_t)t * p.os[1] + (int64_t)(hk * p.rep + row - t * p.rep) * p.os[2] + lane * V;
     uint32_t h[V / 2];
 #pragma unroll
-    for (int e = 0; e < V / 2; ++e) h[e] = narrow2<FMT>(acc[2 * e] * inv, acc[2 * e + 1] * inv);
+    for (int e = 0; e < V / 2; ++e) h[e] = narrow2<FMT>(acc[i][2 * e] * inv, acc[i][2 * e + 1] * inv);
     if constexpr (V == 4) *reinterpret_cast<uint2*>(o) = make_uint2(h[0], h[1]);
     else *reinterpret_cast<uint32_t*>(o) = h[0];
   }
@@ -749,7 +874,16 @@ static void launch(const Params& p, cudaStream_t st) {
   tree_kernel<HD, FMT, PAIR, CAP><<<G, kThreads, Cfg<HD>::kSmem, st>>>(p);
   const int rows = min(PAIR ? 2 * BR : BR, p.R);
   const dim3 grid((unsigned)(p.n_rt * p.Hkv * ((rows + kJoin - 1) / kJoin)), p.B);
-  tree_join_kernel<HD, FMT, PAIR><<<grid, 128, 0, st>>>(p, G);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(128);
+  cfg.stream = st;
+  cudaLaunchAttribute early;
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &early;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, tree_join_kernel<HD, FMT, PAIR>, p, (int64_t)G);
 }
 
 }  // namespace tree
