@@ -9,6 +9,24 @@ namespace b2 {
 namespace fa {
 
 constexpr int kF16 = 0, kBF16 = 1, kTF32 = 2;  // operand formats (tcgen05 instruction descriptor codes)
+constexpr int BQ = 128, BKV = 128;
+constexpr int kKStages = 3, kVStages = 2;
+
+// Tile geometry of the tcgen05 path for head dim HD and operand format FMT
+// (kTF32: fp32 q / k / v read as tf32, fp32 output).  A tile is BQ rows of HD
+// elements in 128-byte swizzle atoms; one MMA k-step is 32 bytes of K.
+template <int HD_, int FMT_>
+struct FaCfg {
+  static constexpr int HD = HD_, FMT = FMT_;
+  static constexpr int ES = FMT == kTF32 ? 4 : 2;   // element bytes
+  static constexpr int KSTEP = 32 / ES;             // K elements per MMA
+  static constexpr int AE = 128 / ES;               // elements per swizzle row
+  static constexpr int NATOM = HD / AE;
+  static constexpr int kAtom = BQ * 128;            // bytes of one atom column
+  static constexpr int kTile = NATOM * kAtom;
+  static constexpr size_t kSmem = (size_t)kTile * (2 + kKStages + kVStages) + 1024 + 256;
+  static_assert(HD % AE == 0, "head dim must fill whole swizzle rows");
+};
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -146,6 +164,7 @@ __device__ __forceinline__ uint64_t exp2_poly_f2(uint64_t x2) {
 struct Score {
   float scale_log2;        // scale * log2 e (> 0)
   float cap_in, cap_log2;  // 2 log2 e scale / cap; cap * log2 e
+  float z_in;              // scale / cap
   float slope, dist;       // slope * log2 e; row - first key of the tile
 };
 
@@ -162,64 +181,133 @@ __device__ __forceinline__ float capped(float s, const Score& c, float add) {
   return fmaf(-2.f * c.cap_log2, rcp_approx(1.f + ex2(s * c.cap_in)), c.cap_log2 + add);
 }
 
-// Score of two neighbouring keys (e and e + 1 in the tile), plus `add`.  Where
-// MASK is false all keys of the tile lie on one side of the row, so the bias is
-// linear in the key: slope carries its sign there (slope > 0: keys before the
-// row).
-template <bool MASK, bool CAP, bool BIAS>
+// The same for two scores of at most kSmallCap of the cap, on the FMA pipe: the
+// two MUFU operations a score of the form above would set the pace of the
+// softmax.  tanh z = z p(z^2), this file's own minimax fit on [-3/4, 3/4]
+// (largest error 2.4e-7 in fp32).
+constexpr float kSmallCap = 0.75f;
+__device__ __forceinline__ uint64_t mul_f2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t capped_small(uint64_t s, const Score& c, uint64_t add) {
+  const uint64_t z = mul_f2(s, f2_pack(c.z_in, c.z_in)), w = mul_f2(z, z);
+  uint64_t q = fma_f2(f2_pack(0.01231883f, 0.01231883f), w, f2_pack(-0.049280446f, -0.049280446f));
+  q = fma_f2(q, w, f2_pack(0.13226092f, 0.13226092f));
+  q = fma_f2(q, w, f2_pack(-0.33323076f, -0.33323076f));
+  q = fma_f2(q, w, f2_pack(0.9999972f, 0.9999972f));
+  return fma_f2(mul_f2(z, f2_pack(c.cap_log2, c.cap_log2)), q, add);
+}
+// Whether all of the warp's N x 32 scores may take capped_small.
+template <int N>
+__device__ __forceinline__ bool all_small(const uint32_t (&sv)[N], const Score& c) {
+  float am = 0.f;
+#pragma unroll
+  for (int e = 0; e < N; e += 2) am = max3(am, fabsf(__uint_as_float(sv[e])), fabsf(__uint_as_float(sv[e + 1])));
+  return !__any_sync(0xffffffffu, !(am * c.z_in <= kSmallCap));
+}
+
+// Score of two neighbouring keys (e and e + 1 from where c.dist counts), plus
+// `add`.  ABS: keys on both sides of the row.  Otherwise all keys of the tile
+// lie on one side, the bias is linear in the key and slope carries its sign
+// (slope > 0: keys before the row).
+template <bool ABS, bool CAP, bool BIAS, bool SMALL>
 __device__ __forceinline__ uint64_t score_pair(uint32_t s0, uint32_t s1, int e, const Score& c, float add) {
   uint64_t a = f2_pack(add, add);
   if constexpr (BIAS) {
-    if constexpr (MASK) {
+    if constexpr (ABS) {
       a = f2_pack(fmaf(-c.slope, fabsf(c.dist - (float)e), add), fmaf(-c.slope, fabsf(c.dist - (float)(e + 1)), add));
     } else {
       const float b = fmaf(-c.slope, c.dist, add);
       a = fma_f2(f2_pack(c.slope, c.slope), f2_pack((float)e, (float)(e + 1)), f2_pack(b, b));
     }
   }
+  const uint64_t s = (uint64_t)s0 | ((uint64_t)s1 << 32);
+  if constexpr (CAP && SMALL) return capped_small(s, c, a);
   if constexpr (CAP)
     return f2_pack(capped(__uint_as_float(s0), c, f2_lo(a)), capped(__uint_as_float(s1), c, f2_hi(a)));
-  return fma_f2((uint64_t)s0 | ((uint64_t)s1 << 32), f2_pack(c.scale_log2, c.scale_log2), a);
+  return fma_f2(s, f2_pack(c.scale_log2, c.scale_log2), a);
 }
 
-// Largest score of the row's visible keys (bits of vis), -inf without one.
-// Scale and cap keep the order, so without a bias the raw maximum is taken and
-// scored once.  With cap and bias both, the scores are left in the S columns
-// for score_exp, so that the cap is computed once.
+// Scores of the N columns in sv, left in sv (cap and bias both: computed once).
+template <bool ABS, bool SMALL, int N>
+__device__ __forceinline__ void score_chunk(uint32_t (&sv)[N], const Score& c) {
+#pragma unroll
+  for (int e = 0; e < N; e += 2) {
+    const uint64_t x = score_pair<ABS, true, true, SMALL>(sv[e], sv[e + 1], e, c, 0.f);
+    sv[e] = (uint32_t)x;
+    sv[e + 1] = (uint32_t)(x >> 32);
+  }
+}
+
+// Largest score (without a bias: largest raw score) of N columns; BITS: of those
+// with a bit in w (N = 32).
+template <bool BITS, bool ABS, bool CAP, bool BIAS, int N>
+__device__ __forceinline__ float max_chunk(uint32_t (&sv)[N], uint32_t w, const Score& c, float mx) {
+  if constexpr (CAP && BIAS) {
+    if (all_small(sv, c)) score_chunk<ABS, true>(sv, c);
+    else score_chunk<ABS, false>(sv, c);
+  }
+#pragma unroll
+  for (int e = 0; e < N; e += 2) {
+    float v0 = __uint_as_float(sv[e]), v1 = __uint_as_float(sv[e + 1]);
+    if constexpr (BIAS && !CAP) {
+      const uint64_t x = score_pair<ABS, CAP, BIAS, false>(sv[e], sv[e + 1], e, c, 0.f);
+      v0 = f2_lo(x);
+      v1 = f2_hi(x);
+    }
+    if constexpr (BITS) {
+      if (!(w >> e & 1)) v0 = -INFINITY;
+      if (!(w >> (e + 1) & 1)) v1 = -INFINITY;
+    }
+    mx = max3(mx, v0, v1);
+  }
+  return mx;
+}
+
+__device__ __forceinline__ uint32_t word_of(const uint32_t (&vis)[4], int c) {
+  return c == 0 ? vis[0] : c == 1 ? vis[1] : c == 2 ? vis[2] : vis[3];
+}
+
+// Largest score of the row's visible keys, -inf without one.  Scale and cap
+// keep the order, so without a bias the raw maximum is taken and scored once.
+// With cap and bias both, the scores are left in the S columns for score_exp.
+// MASK: visible keys as bits; of the four 32-key pieces those that no row of the
+// warp sees are passed over, and those that all of its rows see whole cost no
+// more than in an unmasked tile (on a diagonal or at a document's border one
+// piece in four is mixed).
 template <bool MASK, bool CAP, bool BIAS>
 __device__ __forceinline__ float score_max(uint32_t tS, const uint32_t (&vis)[4], const Score& sc) {
   float mx = -INFINITY;
+  if constexpr (MASK) {
 #pragma unroll 1
-  for (int c = 0; c < 4; c += 2) {
-    uint32_t sv[64];
-    tc::tmem_ld_32x32b_x32(tS + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(sv));
-    tc::tmem_ld_32x32b_x32(tS + 32 * c + 32, *reinterpret_cast<uint32_t(*)[32]>(sv + 32));
-    tc::tmem_ld_wait();
-    const uint32_t w0 = c ? vis[2] : vis[0], w1 = c ? vis[3] : vis[1];
-    Score cc = sc;
-    cc.dist -= 32.f * c;
-#pragma unroll
-    for (int e = 0; e < 64; e += 2) {
-      float v0 = __uint_as_float(sv[e]), v1 = __uint_as_float(sv[e + 1]);
-      if constexpr (BIAS) {
-        const uint64_t x = score_pair<MASK, CAP, BIAS>(sv[e], sv[e + 1], e, cc, 0.f);
-        v0 = f2_lo(x);
-        v1 = f2_hi(x);
-        if constexpr (CAP) {
-          sv[e] = (uint32_t)x;
-          sv[e + 1] = (uint32_t)(x >> 32);
-        }
-      }
-      if constexpr (MASK) {
-        const uint32_t w = e < 32 ? w0 : w1;
-        if (!(w >> (e & 31) & 1)) v0 = -INFINITY;
-        if (!(w >> ((e + 1) & 31) & 1)) v1 = -INFINITY;
-      }
-      mx = max3(mx, v0, v1);
+    for (int c = 0; c < 4; ++c) {
+      const uint32_t w = word_of(vis, c);
+      if (!__any_sync(0xffffffffu, w != 0)) continue;
+      uint32_t sv[32];
+      tc::tmem_ld_32x32b_x32(tS + 32 * c, sv);
+      tc::tmem_ld_wait();
+      Score cc = sc;
+      cc.dist -= 32.f * c;
+      if (__all_sync(0xffffffffu, w == 0xffffffffu)) mx = max_chunk<false, true, CAP, BIAS>(sv, w, cc, mx);
+      else mx = max_chunk<true, true, CAP, BIAS>(sv, w, cc, mx);
+      if constexpr (CAP && BIAS) tmem_st_32x32b_x32(tS + 32 * c, sv);
     }
-    if constexpr (CAP && BIAS) {
-      tmem_st_32x32b_x32(tS + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(sv));
-      tmem_st_32x32b_x32(tS + 32 * c + 32, *reinterpret_cast<uint32_t(*)[32]>(sv + 32));
+  } else {
+#pragma unroll 1
+    for (int c = 0; c < 4; c += 2) {
+      uint32_t sv[64];
+      tc::tmem_ld_32x32b_x32(tS + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(sv));
+      tc::tmem_ld_32x32b_x32(tS + 32 * c + 32, *reinterpret_cast<uint32_t(*)[32]>(sv + 32));
+      tc::tmem_ld_wait();
+      Score cc = sc;
+      cc.dist -= 32.f * c;
+      mx = max_chunk<false, false, CAP, BIAS>(sv, 0, cc, mx);
+      if constexpr (CAP && BIAS) {
+        tmem_st_32x32b_x32(tS + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(sv));
+        tmem_st_32x32b_x32(tS + 32 * c + 32, *reinterpret_cast<uint32_t(*)[32]>(sv + 32));
+      }
     }
   }
   if constexpr (CAP && BIAS) tmem_st_wait();
@@ -230,51 +318,88 @@ __device__ __forceinline__ float score_max(uint32_t tS, const uint32_t (&vis)[4]
   return mx;
 }
 
+// p = exp2(score - m) of N columns as 16-bit pairs; their sum goes to rs.
+template <bool BITS, bool ABS, int FMT, bool CAP, bool BIAS, bool SMALL, int N>
+__device__ __forceinline__ void exp_chunk(const uint32_t (&sv)[N], uint32_t (&pk)[N / 2], uint64_t& rs, uint32_t w,
+                                          const Score& c, float mref) {
+#pragma unroll
+  for (int e = 0; e < N / 2; ++e) {
+    float p0, p1;
+    uint64_t x;
+    if constexpr (CAP && BIAS) x = add_f2((uint64_t)sv[2 * e] | ((uint64_t)sv[2 * e + 1] << 32), f2_pack(-mref, -mref));
+    else x = score_pair<ABS, CAP, BIAS, SMALL>(sv[2 * e], sv[2 * e + 1], 2 * e, c, -mref);
+    if (e % 3 == 2) {  // a third of the exponentials on the FMA pipe, as in the prefill kernel
+      const uint64_t y = exp2_poly_f2(x);
+      p0 = f2_lo(y);
+      p1 = f2_hi(y);
+    } else {
+      p0 = ex2(f2_lo(x));
+      p1 = ex2(f2_hi(x));
+    }
+    if constexpr (BITS) {
+      if (!(w >> (2 * e) & 1)) p0 = 0.f;
+      if (!(w >> (2 * e + 1) & 1)) p1 = 0.f;
+    }
+    rs = add_f2(rs, f2_pack(p0, p1));
+    if constexpr (FMT == kF16) {
+      __half2 hv = __floats2half2_rn(p0, p1);
+      pk[e] = *reinterpret_cast<uint32_t*>(&hv);
+    } else {
+      __nv_bfloat162 hv = __floats2bfloat162_rn(p0, p1);
+      pk[e] = *reinterpret_cast<uint32_t*>(&hv);
+    }
+  }
+}
+template <bool BITS, bool ABS, int FMT, bool CAP, bool BIAS, int N>
+__device__ __forceinline__ void exp_chunk_any(const uint32_t (&sv)[N], uint32_t (&pk)[N / 2], uint64_t& rs, uint32_t w,
+                                              const Score& c, float mref) {
+  if constexpr (CAP && !BIAS) {
+    if (all_small(sv, c)) {
+      exp_chunk<BITS, ABS, FMT, CAP, BIAS, true>(sv, pk, rs, w, c, mref);
+      return;
+    }
+  }
+  exp_chunk<BITS, ABS, FMT, CAP, BIAS, false>(sv, pk, rs, w, c, mref);
+}
+
 // p = exp2(score - m) as 16-bit pairs over the S columns; returns their sum.
 // P rounded to 16 bits (half a step of its own size) is what the MMA takes; the
 // sum is taken before that, in 32 bits.
 template <bool MASK, int FMT, bool CAP, bool BIAS>
 __device__ __forceinline__ float score_exp(uint32_t tS, const uint32_t (&vis)[4], float mref, const Score& sc) {
   uint64_t rs = 0;
+  if constexpr (MASK) {
 #pragma unroll 1
-  for (int c = 0; c < 4; c += 2) {
-    uint32_t sv[64];
-    tc::tmem_ld_32x32b_x32(tS + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(sv));
-    tc::tmem_ld_32x32b_x32(tS + 32 * c + 32, *reinterpret_cast<uint32_t(*)[32]>(sv + 32));
-    tc::tmem_ld_wait();
-    const uint32_t w0 = c ? vis[2] : vis[0], w1 = c ? vis[3] : vis[1];
-    Score cc = sc;
-    cc.dist -= 32.f * c;
-    uint32_t pk[32];
+    for (int c = 0; c < 4; ++c) {
+      const uint32_t w = word_of(vis, c);
+      uint32_t pk[16];
+      if (!__any_sync(0xffffffffu, w != 0)) {
 #pragma unroll
-    for (int e = 0; e < 32; ++e) {
-      float p0, p1;
-      uint64_t x;
-      if constexpr (CAP && BIAS) x = add_f2((uint64_t)sv[2 * e] | ((uint64_t)sv[2 * e + 1] << 32), f2_pack(-mref, -mref));
-      else x = score_pair<MASK, CAP, BIAS>(sv[2 * e], sv[2 * e + 1], 2 * e, cc, -mref);
-      if (e % 3 == 2) {  // a third of the exponentials on the FMA pipe, as in the prefill kernel
-        const uint64_t y = exp2_poly_f2(x);
-        p0 = f2_lo(y);
-        p1 = f2_hi(y);
+        for (int e = 0; e < 16; ++e) pk[e] = 0;
       } else {
-        p0 = ex2(f2_lo(x));
-        p1 = ex2(f2_hi(x));
+        uint32_t sv[32];
+        tc::tmem_ld_32x32b_x32(tS + 32 * c, sv);
+        tc::tmem_ld_wait();
+        Score cc = sc;
+        cc.dist -= 32.f * c;
+        if (__all_sync(0xffffffffu, w == 0xffffffffu)) exp_chunk_any<false, true, FMT, CAP, BIAS>(sv, pk, rs, w, cc, mref);
+        else exp_chunk_any<true, true, FMT, CAP, BIAS>(sv, pk, rs, w, cc, mref);
       }
-      if constexpr (MASK) {
-        const uint32_t w = e < 16 ? w0 : w1;
-        if (!(w >> ((2 * e) & 31) & 1)) p0 = 0.f;
-        if (!(w >> ((2 * e + 1) & 31) & 1)) p1 = 0.f;
-      }
-      rs = add_f2(rs, f2_pack(p0, p1));
-      if constexpr (FMT == kF16) {
-        __half2 hv = __floats2half2_rn(p0, p1);
-        pk[e] = *reinterpret_cast<uint32_t*>(&hv);
-      } else {
-        __nv_bfloat162 hv = __floats2bfloat162_rn(p0, p1);
-        pk[e] = *reinterpret_cast<uint32_t*>(&hv);
-      }
+      tmem_st_32x32b_x16(tS + 16 * c, pk);
     }
-    tmem_st_32x32b_x32(tS + 16 * c, pk);
+  } else {
+#pragma unroll 1
+    for (int c = 0; c < 4; c += 2) {
+      uint32_t sv[64];
+      tc::tmem_ld_32x32b_x32(tS + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(sv));
+      tc::tmem_ld_32x32b_x32(tS + 32 * c + 32, *reinterpret_cast<uint32_t(*)[32]>(sv + 32));
+      tc::tmem_ld_wait();
+      Score cc = sc;
+      cc.dist -= 32.f * c;
+      uint32_t pk[32];
+      exp_chunk_any<false, false, FMT, CAP, BIAS>(sv, pk, rs, 0, cc, mref);
+      tmem_st_32x32b_x32(tS + 16 * c, pk);
+    }
   }
   return f2_lo(rs) + f2_hi(rs);
 }
@@ -312,5 +437,56 @@ __device__ __forceinline__ uint32_t narrow2(float a, float b) {
   }
 }
 
+// 4-D tensor map coordinates: (d, s, h, b)
+__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, int d, int s, int h, int b,
+                                            uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
+          smem_u32(dst)),
+      "l"(map), "r"(d), "r"(s), "r"(h), "r"(b), "r"(smem_u32(bar))
+      : "memory");
+}
+
 }  // namespace fa
+
+// dims (d, s, h, b), element strides (b, h, s); box = one swizzle row
+// (box_d elements = 128 bytes) x 128 rows.
+// mn_major_tf32: the 128-byte swizzle with 32-byte atomicity that the MMA's
+// MN-major tf32 operand layout (SWIZZLE_128B_BASE32B) expects (V of the tf32 path).
+static bool make_tmap_4d(CUtensorMap* map, const void* base, int dtype, int64_t D, int64_t S, int64_t H, int64_t B,
+                         const int64_t* strides_elems, bool mn_major_tf32 = false) {
+  // dims (d, s, h, b); strides in bytes for s, h, b
+  typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                               const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                               CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static EncodeFn fn = nullptr;
+  if (!fn) {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      return false;
+    fn = reinterpret_cast<EncodeFn>(p);
+  }
+  const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)S, (cuuint64_t)H, (cuuint64_t)B};
+  const cuuint64_t es = dtype == B2_F32 ? 4 : 2;
+  const cuuint64_t strides[3] = {(cuuint64_t)strides_elems[2] * es, (cuuint64_t)strides_elems[1] * es,
+                                 (cuuint64_t)strides_elems[0] * es};
+  const cuuint32_t box[4] = {(cuuint32_t)(128 / es), 128, 1, 1};
+  const cuuint32_t estr[4] = {1, 1, 1, 1};
+  const CUtensorMapDataType dt = dtype == B2_F32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                 : dtype == B2_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                   : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  return fn(map, dt, 4, const_cast<void*>(base),
+            dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            mn_major_tf32 ? CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B : CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// element strides whose byte values are multiples of 16 (TMA)
+static bool strides_ok(const int64_t* s, int dtype) {
+  const int64_t m = dtype == B2_F32 ? 4 : 8;
+  return s[0] % m == 0 && s[1] % m == 0 && s[2] % m == 0;
+}
+
 }  // namespace b2

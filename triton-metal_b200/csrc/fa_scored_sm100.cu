@@ -1,29 +1,500 @@
 // FlashAttention forward with document and prefix masks, capped scores and a
-// distance bias: key ranges per row and score forms on the kernels of
-// fa_fwd_kernel.cuh (16-bit, head dim 64 / 128, tcgen05) and attn_simt.cu (the
-// rest, fp32 arithmetic).  The reference has causal masking only
+// distance bias: key ranges per row and score forms, on tcgen05 here (16-bit,
+// head dim 64 / 128) and on the CUDA cores in attn_simt.cu (the rest, fp32
+// arithmetic).  The reference has causal masking only
 // (_msl_templates.py:1610-1619).
 //
 //   s = scale q.k;  softcap: s = softcap tanh(s / softcap);  s -= slope |i - j|
 //
 // Every mask is one key range per query row (attn::row_range), so a Q tile
-// visits the KV tiles from its rows' first visible key to their last and only
+// visits the KV tiles from its rows' first visible key to their last, and only
 // tiles at the ranges' ends are masked.  Capped and biased scores cost softmax
-// issue slots, not memory: the cap takes two more MUFU operations a score, the
-// bias one more paired FMA.
-#include "fa_fwd_kernel.cuh"
+// issue slots, not memory.
+#include "attn_common.cuh"
+#include "fa_common.cuh"
+#include <limits.h>
 #include <math.h>
 
 namespace b2 {
+namespace scored {
 
-template <int HD, int FMT, bool CAP, bool BIAS>
-static void launch_scored(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const fa::Params& p,
-                          dim3 grid, cudaStream_t st) {
-  using Cf = fa::FaCfg<HD, FMT>;
-  set_max_smem((const void*)fa::fa_fwd2_kernel<HD, FMT, true, CAP, BIAS>, (int)Cf::kSmem);
-  fa::fa_fwd2_kernel<HD, FMT, true, CAP, BIAS><<<grid, fa::kThreads2, Cf::kSmem, st>>>(tq, tk, tv, p);
+using namespace fa;
+
+// ---------------------------------------------------------------------------
+// The pipeline of the plain prefill kernel (fa_fwd_sm100.cu: two Q tiles in
+// ping-pong, P in TMEM), made persistent: with short documents a unit (a pair
+// of Q tiles of one head) has a handful of KV tiles, and what counts is how
+// soon the next one starts.  One CTA per SM walks units; the next unit's Q, K
+// and V are loaded and its first S is computed while this one's last softmax
+// and output are under way.
+//   warp 0      TMA
+//   warp 1      TMEM owner, MMA issuer
+//   warps 2-3   key ranges of the next unit (which KV tiles its Q tiles visit,
+//               which of them are masked), and V: a tile in which some row must
+//               not see some key has its infinities and NaN zeroed, since a
+//               weight of 0 would make NaN of them; rows that do see such a
+//               value get it added at the end
+//   warps 4-11  two softmax warpgroups, one per Q tile, one row per thread
+// ---------------------------------------------------------------------------
+constexpr int kThreads = 384;
+constexpr float kRescale = 8.f;  // log2 units
+
+struct Params {
+  int B, Hq, Hkv, Sq, Skv, q_tiles;
+  int per, n_units;        // Q tiles of a unit (1 where pairs would not fill the SMs); units of a head
+  attn::RangeMask range;
+  float scale_log2, cap_in, cap_log2, z_in;
+  const float* slopes;     // [Hq]
+  void* o;
+  int64_t os_b, os_h, os_s;
+  const uint16_t* v;       // V again, for values that are not finite
+  int64_t vs_b, vs_h, vs_s;
+  unsigned* err;
+};
+
+// Unit of a CTA's turn: the rows furthest back first (causal rows: the longest),
+// heads of one kv head next to one another (their K/V stays in L2), turns in
+// alternating direction so that nobody gets the longest of each.
+struct Unit {
+  int b, h, q0;  // q0: first row
+};
+__device__ __forceinline__ bool unit_of(const Params& p, int turn, Unit& u) {
+  const int64_t G = gridDim.x, n = (int64_t)p.n_units * p.Hq * p.B;
+  const int64_t at = turn * G + (turn & 1 ? G - 1 - blockIdx.x : blockIdx.x);
+  if (at >= n) return false;
+  const uint32_t heads = (uint32_t)p.Hq * p.B, x = (uint32_t)at;
+  const uint32_t row = x / heads, bh = x - row * heads;
+  u.b = bh / (uint32_t)p.Hq;
+  u.h = bh - u.b * p.Hq;
+  u.q0 = (p.n_units - 1 - (int)row) * p.per * BQ;
+  return true;
 }
 
+// What warps 2-3 find out about a unit's two Q tiles.
+struct Info {
+  int kb[2], nkv[2];            // KV tiles visited: kb .. nkv - 1
+  int lo_most[2], hi_least[2];  // keys that every row of the tile sees
+  __device__ __forceinline__ bool active(int u, int j) const { return j >= kb[u] && j < nkv[u]; }
+  __device__ __forceinline__ bool masked(int u, int j) const { return j * BKV < lo_most[u] || j * BKV + BKV > hi_least[u]; }
+  __device__ __forceinline__ int first() const {
+    return nkv[0] == 0 ? kb[1] : nkv[1] == 0 ? kb[0] : min(kb[0], kb[1]);
+  }
+  __device__ __forceinline__ int last() const { return max(nkv[0], nkv[1]); }
+};
+
+// Bits of the keys of [lo, hi) among the 128 from kv0 on.
+__device__ __forceinline__ void range_bits(uint32_t (&vis)[4], int lo, int hi, int kv0) {
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const int a = min(max(lo - kv0 - 32 * w, 0), 32), z = min(max(hi - kv0 - 32 * w, 0), 32);
+    const uint32_t below_z = z == 32 ? 0xffffffffu : (1u << z) - 1, below_a = a == 32 ? 0xffffffffu : (1u << a) - 1;
+    vis[w] = below_z & ~below_a;
+  }
+}
+
+template <int HD, int FMT, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(kThreads, 1)
+scored_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+              const __grid_constant__ CUtensorMap tmV, const Params p) {
+  using Cf = FaCfg<HD, FMT>;
+  constexpr int kTile = Cf::kTile, kAtom = Cf::kAtom;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  uint8_t* sQ = smem;  // 2 tiles
+  uint8_t* sK = sQ + 2 * kTile;
+  uint8_t* sV = sK + kKStages * kTile;
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(sV + kVStages * kTile);
+  uint64_t* q_empty = q_full + 1;
+  uint64_t* k_full = q_empty + 1;
+  uint64_t* k_empty = k_full + kKStages;
+  uint64_t* v_full = k_empty + kKStages;
+  uint64_t* v_clean = v_full + kVStages;
+  uint64_t* v_empty = v_clean + kVStages;
+  uint64_t* s_full = v_empty + kVStages;      // [2] per Q tile
+  uint64_t* p_ready = s_full + 2;             // [2]
+  uint64_t* o_done = p_ready + 2;             // [2]
+  uint64_t* info_full = o_done + 2;           // [2] by unit parity
+  uint64_t* info_empty = info_full + 2;       // [2]
+  uint64_t* drain = info_empty + 2;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(drain + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
+  volatile int* s_bad = reinterpret_cast<volatile int*>(tmem_holder + 2);      // [4]: unit with a bad V value
+  int4* s_info = reinterpret_cast<int4*>(q_full + 32);                         // [2 parities][2 warps][2 tiles]
+  static_assert(2 + 2 * kKStages + 3 * kVStages + 11 + 3 <= 32, "barriers");
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
+    for (int i = 0; i < kKStages; ++i) {
+      mbar_init(&k_full[i], 1);
+      mbar_init(&k_empty[i], 1);
+    }
+    for (int i = 0; i < kVStages; ++i) {
+      mbar_init(&v_full[i], 1);
+      mbar_init(&v_clean[i], 64);
+      mbar_init(&v_empty[i], 1);
+    }
+    for (int u = 0; u < 2; ++u) {
+      mbar_init(&s_full[u], 1);
+      mbar_init(&p_ready[u], 4);
+      mbar_init(&o_done[u], 1);
+      mbar_init(&info_full[u], 64);
+      mbar_init(&info_empty[u], 10);  // TMA, MMA, 8 softmax warps
+    }
+    for (int i = 0; i < 4; ++i) s_bad[i] = -1;
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tc::tmem_alloc(tmem_holder, 512);
+    tc::tmem_relinquish();
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  const uint32_t tmem = *tmem_holder;
+
+  // The info of turn k, once it is there; every reader says that it has it.
+  auto read_info = [&](int k, Info& f) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int4 a = s_info[(k & 1) * 4 + u], b = s_info[(k & 1) * 4 + 2 + u];
+      const int lo = min(a.x, b.x), hi = max(a.z, b.z);
+      f.lo_most[u] = max(a.y, b.y);
+      f.hi_least[u] = min(a.w, b.w);
+      // A row that sees anything sees itself or everything, so the two tiles'
+      // spans touch and the pair's union has no gap.
+      f.kb[u] = hi > 0 ? lo / BKV : 0;
+      f.nkv[u] = (hi + BKV - 1) / BKV;
+    }
+  };
+
+  Unit un;
+  Info f;
+  if (warp == 0) {
+    // ---------------------------------- TMA ----------------------------------
+    if (lane == 0) {
+      int kst = 0, vst = 0;
+      uint32_t kph = 0, vph = 0, qn = 0;  // qn: units with anything to load
+      bool ok = true;
+      for (int k = 0; ok && unit_of(p, k, un); ++k) {
+        ok = wait_abort(&info_full[k & 1], (k >> 1) & 1, p.err, 0xB2600001u, abort_flag);
+        if (!ok) break;
+        read_info(k, f);
+        mbar_arrive(&info_empty[k & 1]);
+        const int jb = f.first(), je = f.last();
+        if (je == 0) continue;
+        const int hk = un.h / (p.Hq / p.Hkv);
+        ok = wait_abort(q_empty, (qn & 1) ^ 1, p.err, 0xB2600002u, abort_flag);
+        if (!ok) break;
+        ++qn;
+        mbar_arrive_expect_tx(q_full, ((f.nkv[0] > 0) + (f.nkv[1] > 0)) * kTile);
+        for (int u = 0; u < 2; ++u)
+          if (f.nkv[u] > 0)
+#pragma unroll
+            for (int a = 0; a < Cf::NATOM; ++a)
+              tma_load_4d(sQ + u * kTile + a * kAtom, &tmQ, a * Cf::AE, un.q0 + u * BQ, un.h, un.b, q_full);
+        for (int j = jb; j < je; ++j) {
+          ok = wait_abort(&k_empty[kst], kph ^ 1, p.err, 0xB2600003u, abort_flag);
+          if (!ok) break;
+          mbar_arrive_expect_tx(&k_full[kst], kTile);
+#pragma unroll
+          for (int a = 0; a < Cf::NATOM; ++a)
+            tma_load_4d(sK + kst * kTile + a * kAtom, &tmK, a * Cf::AE, j * BKV, hk, un.b, &k_full[kst]);
+          ok = wait_abort(&v_empty[vst], vph ^ 1, p.err, 0xB2600004u, abort_flag);
+          if (!ok) break;
+          mbar_arrive_expect_tx(&v_full[vst], kTile);
+#pragma unroll
+          for (int a = 0; a < Cf::NATOM; ++a)
+            tma_load_4d(sV + vst * kTile + a * kAtom, &tmV, a * Cf::AE, j * BKV, hk, un.b, &v_full[vst]);
+          if (++kst == kKStages) { kst = 0; kph ^= 1; }
+          if (++vst == kVStages) { vst = 0; vph ^= 1; }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ---------------------------------- MMA ----------------------------------
+    if (lane == 0) {
+      constexpr uint32_t idS = idesc_fmt(BQ, BKV, FMT, false);
+      constexpr uint32_t idPV = idesc_fmt(BQ, HD, FMT, true);
+      int kst = 0, vst = 0;
+      uint32_t kph = 0, vph = 0, qn = 0, pc[2] = {0, 0};
+      bool ok = true;
+      auto issue_s = [&](int u) {
+#pragma unroll
+        for (int kk = 0; kk < HD / Cf::KSTEP; ++kk) {
+          const uint64_t da = tc::desc_kmajor_sw128(sQ + u * kTile + (kk >> 2) * kAtom + (kk & 3) * 32);
+          const uint64_t db = tc::desc_kmajor_sw128(sK + kst * kTile + (kk >> 2) * kAtom + (kk & 3) * 32);
+          mma_ss<FMT>(tmem + 256 * u, da, db, idS, kk != 0);
+        }
+        tc::commit(&s_full[u]);
+      };
+      auto wait_k = [&]() {
+        ok = ok && wait_abort(&k_full[kst], kph, p.err, 0xB2600005u, abort_flag);
+        if (ok) tc::fence_after_sync();
+        return ok;
+      };
+      auto free_k = [&]() {
+        tc::commit(&k_empty[kst]);
+        if (++kst == kKStages) { kst = 0; kph ^= 1; }
+      };
+      for (int k = 0; ok && unit_of(p, k, un); ++k) {
+        ok = wait_abort(&info_full[k & 1], (k >> 1) & 1, p.err, 0xB2600006u, abort_flag);
+        if (!ok) break;
+        read_info(k, f);
+        mbar_arrive(&info_empty[k & 1]);
+        const int jb = f.first(), je = f.last();
+        if (je == 0) continue;
+        ok = wait_abort(q_full, qn & 1, p.err, 0xB2600007u, abort_flag);
+        if (!ok) break;
+        ++qn;
+        // S of the first KV tile.  Its columns hold the last P of the unit before,
+        // whose PV was issued earlier: MMAs of one thread run in order.
+        if (!wait_k()) break;
+        for (int u = 0; u < 2; ++u)
+          if (f.active(u, jb)) issue_s(u);
+        free_k();
+        for (int j = jb; j < je && ok; ++j) {
+          if (j == je - 1) tc::commit(q_empty);  // every S of the unit is issued
+          ok = wait_abort(&v_clean[vst], vph, p.err, 0xB2600008u, abort_flag);
+          if (!ok) break;
+          bool have_k = false;
+          for (int u = 0; u < 2 && ok; ++u) {
+            if (f.active(u, j)) {
+              ok = wait_abort(&p_ready[u], pc[u] & 1, p.err, 0xB2600009u, abort_flag);
+              if (!ok) break;
+              ++pc[u];
+              tc::fence_after_sync();
+#pragma unroll
+              for (int kk = 0; kk < BKV / Cf::KSTEP; ++kk)
+                mma_ts<FMT>(tmem + 256 * u + 128, tmem + 256 * u + kk * 8,
+                            tc::smem_desc(sV + vst * kTile + kk * Cf::KSTEP * 128, kAtom, 1024, tc::kSwizzle128B), idPV,
+                            (j != f.kb[u]) || kk != 0);
+              if (j == f.nkv[u] - 1) tc::commit(&o_done[u]);
+            }
+            if (f.active(u, j + 1)) {
+              if (!have_k && !wait_k()) break;
+              have_k = true;
+              issue_s(u);
+            }
+          }
+          if (!ok) break;
+          tc::commit(&v_empty[vst]);
+          if (++vst == kVStages) { vst = 0; vph ^= 1; }
+          if (have_k) free_k();
+        }
+      }
+      if (!ok) {
+        tc::commit(drain);
+        mbar_wait(drain, 0, p.err, 0xB260000Au);
+      }
+    }
+  } else if (warp < 4) {
+    // ------------------------- key ranges, V of masked tiles -------------------------
+    const int t = threadIdx.x - 64;
+    auto find = [&](int k) {  // info of turn k; true when there is such a turn
+      Unit n;
+      if (!unit_of(p, k, n)) return true;
+      if (k >= 2 && !__all_sync(0xffffffffu, wait_abort(&info_empty[k & 1], ((k >> 1) - 1) & 1, p.err, 0xB260000Bu, abort_flag)))
+        return false;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        // smallest / largest first key, largest / smallest end; a row that sees
+        // nothing makes every tile a masked one
+        int4 x = make_int4(INT_MAX, 0, 0, INT_MAX);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int row = n.q0 + u * BQ + i * 64 + t;
+          if (u < p.per && row < p.Sq) {
+            int lo, hi;
+            attn::row_range(p.range, n.b, row, p.Skv, lo, hi);
+            const bool sees = hi > lo;
+            if (sees) x.x = min(x.x, lo);
+            x.y = sees ? max(x.y, lo) : INT_MAX;
+            if (sees) x.z = max(x.z, hi);
+            x.w = sees ? min(x.w, hi) : 0;
+          }
+        }
+        x.x = __reduce_min_sync(0xffffffffu, x.x);
+        x.y = __reduce_max_sync(0xffffffffu, x.y);
+        x.z = __reduce_max_sync(0xffffffffu, x.z);
+        x.w = __reduce_min_sync(0xffffffffu, x.w);
+        if (lane == 0) s_info[(k & 1) * 4 + (warp - 2) * 2 + u] = x;
+      }
+      __syncwarp();
+      mbar_arrive(&info_full[k & 1]);
+      return true;
+    };
+    int vst = 0;
+    uint32_t vph = 0;
+    bool ok = find(0);
+    for (int k = 0; ok && unit_of(p, k, un); ++k) {
+      // before the next info may replace this one's neighbour: the other warp's half
+      ok = __all_sync(0xffffffffu, wait_abort(&info_full[k & 1], (k >> 1) & 1, p.err, 0xB260000Cu, abort_flag));
+      if (!ok) break;
+      read_info(k, f);
+      ok = find(k + 1);
+      const int jb = f.first(), je = f.last();
+      for (int j = jb; j < je && ok; ++j) {
+        // every tile passes through here, so that these warps are never a ring
+        // turn behind a stage (a parity wait cannot tell that)
+        ok = __all_sync(0xffffffffu, wait_abort(&v_full[vst], vph, p.err, 0xB260000Du, abort_flag));
+        if (!ok) break;
+        if ((f.active(0, j) && f.masked(0, j)) || (f.active(1, j) && f.masked(1, j))) {
+          uint4* tile = reinterpret_cast<uint4*>(sV + vst * kTile);
+          bool bad = false;
+#pragma unroll 8
+          for (int i = t; i < kTile / 16; i += 64) {
+            uint4 x = tile[i];
+            if (zero_not_finite<FMT>(x)) {
+              tile[i] = x;
+              bad = true;
+            }
+          }
+          // four turns of flags: warps 4-11 have left turn k - 4 when info k + 1
+          // could be made
+          if (bad) s_bad[k & 3] = k;
+          tc::fence_proxy_async_smem();
+        }
+        mbar_arrive(&v_clean[vst]);
+        if (++vst == kVStages) { vst = 0; vph ^= 1; }
+      }
+    }
+  } else {
+    // -------------------------------- softmax --------------------------------
+    const int u = (warp - 4) >> 2, qw = warp & 3, r = qw * 32 + lane;
+    const uint32_t lane_off = (uint32_t)(qw * 32) << 16;
+    const uint32_t tS = tmem + 256 * u + lane_off, tO = tS + 128;
+    Score score = {p.scale_log2, p.cap_in, p.cap_log2, p.z_in, 0.f, 0.f};
+    uint32_t sc = 0, oc = 0;  // S tiles / outputs waited for
+    bool ok = true;
+    for (int k = 0; ok && unit_of(p, k, un); ++k) {
+      const int q0 = un.q0 + u * BQ, qpos = q0 + r;
+      const bool exists = u < p.per && qpos < p.Sq;
+      int row_lo = 0, row_hi = 0;
+      if (exists) attn::row_range(p.range, un.b, qpos, p.Skv, row_lo, row_hi);
+      float slope = 0.f;
+      if constexpr (BIAS) slope = p.slopes[un.h] * attn::kLog2e;
+      ok = __all_sync(0xffffffffu, wait_abort(&info_full[k & 1], (k >> 1) & 1, p.err, 0xB260000Eu, abort_flag));
+      if (!ok) break;
+      read_info(k, f);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&info_empty[k & 1]);
+      const int kb = f.kb[u], nkv = f.nkv[u];
+      float m_used = -INFINITY, l = 0.f;
+      for (int j = kb; j < nkv; ++j) {
+        ok = __all_sync(0xffffffffu, wait_abort(&s_full[u], sc & 1, p.err, 0xB260000Fu, abort_flag));
+        if (!ok) break;
+        ++sc;
+        tc::fence_after_sync();
+        const int kv0 = j * BKV;
+        bool need_mask = f.masked(u, j);
+        if constexpr (BIAS) {
+          // the bias is linear over the tile unless the tile's rows lie in it
+          const bool before = kv0 + BKV - 1 <= q0, behind = kv0 >= q0 + BQ - 1;
+          need_mask = need_mask || !(before || behind);
+          score.dist = (float)(qpos - kv0);
+          score.slope = need_mask || before ? slope : -slope;
+        }
+        uint32_t vis[4] = {0, 0, 0, 0};
+        if (need_mask) range_bits(vis, row_lo, row_hi, kv0);
+        const float mx = need_mask ? score_max<true, CAP, BIAS>(tS, vis, score) : score_max<false, CAP, BIAS>(tS, vis, score);
+        // lazy, warp-uniform rescale of O (O_u is quiescent: PV_u(j-1) finished)
+        const bool need = mx > m_used + kRescale;
+        const float alpha = need ? ((m_used == -INFINITY) ? 0.f : ex2(m_used - mx)) : 1.f;
+        if (need) {
+          l *= alpha;
+          m_used = mx;
+        }
+        if (__any_sync(0xffffffffu, need) && j > kb) {
+#pragma unroll 1
+          for (int c = 0; c < HD / 32; ++c) {
+            uint32_t o[32];
+            tc::tmem_ld_32x32b_x32(tO + 32 * c, o);
+            tc::tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+            tmem_st_32x32b_x32(tO + 32 * c, o);
+          }
+        }
+        const float mref = (m_used == -INFINITY) ? 0.f : m_used;
+        l += need_mask ? score_exp<true, FMT, CAP, BIAS>(tS, vis, mref, score)
+                       : score_exp<false, FMT, CAP, BIAS>(tS, vis, mref, score);
+        tmem_st_wait();
+        tc::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_ready[u]);
+      }
+      if (!ok) break;
+      // O_u / l -> global (rows beyond Sq are not stored)
+      uint16_t* orow = reinterpret_cast<uint16_t*>(p.o) + un.b * p.os_b + un.h * p.os_h + (int64_t)qpos * p.os_s;
+      if (nkv == kb) {  // no row of the tile sees anything: zeros
+        if (exists)
+          for (int e = 0; e < HD / 8; ++e) reinterpret_cast<uint4*>(orow)[e] = make_uint4(0, 0, 0, 0);
+        continue;
+      }
+      ok = __all_sync(0xffffffffu, wait_abort(&o_done[u], oc & 1, p.err, 0xB2600010u, abort_flag));
+      if (!ok) break;
+      ++oc;
+      tc::fence_after_sync();
+      const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+      const bool bad = s_bad[k & 3] == k;
+      const int hk = un.h / (p.Hq / p.Hkv);
+#pragma unroll 1
+      for (int c = 0; c < HD / 32; ++c) {
+        float o[32];
+        tc::tmem_ld_32x32b_x32(tO + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(o));
+        tc::tmem_ld_wait();
+        if (bad) {
+          for (int key = row_lo; key < row_hi; ++key) {
+            const uint16_t* v = p.v + un.b * p.vs_b + hk * p.vs_h + (int64_t)key * p.vs_s + 32 * c;
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+              const uint16_t x = v[e];
+              if (not_finite16<FMT>(x)) o[e] += widen16<FMT>(x);
+            }
+          }
+        }
+        if (l == 0.f) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = 0.f;
+        }
+        if (exists) {
+          uint4* dst = reinterpret_cast<uint4*>(orow + 32 * c);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            dst[e] = make_uint4(narrow2<FMT>(o[8 * e] * inv, o[8 * e + 1] * inv),
+                                narrow2<FMT>(o[8 * e + 2] * inv, o[8 * e + 3] * inv),
+                                narrow2<FMT>(o[8 * e + 4] * inv, o[8 * e + 5] * inv),
+                                narrow2<FMT>(o[8 * e + 6] * inv, o[8 * e + 7] * inv));
+        }
+      }
+      // the next unit's first PV overwrites O_u once this warpgroup hands over a P
+      tc::fence_before_sync();
+    }
+  }
+
+  tc::fence_before_sync();
+  __syncthreads();
+  if (warp == 1) {
+    tc::fence_after_sync();
+    tc::tmem_dealloc(tmem, 512);
+  }
+}
+
+template <int HD, int FMT, bool CAP, bool BIAS>
+static void launch(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const Params& p,
+                   cudaStream_t st) {
+  constexpr int smem = 7 * FaCfg<HD, FMT>::kTile + 1024 + 512;
+  const int64_t units = (int64_t)p.n_units * p.Hq * p.B;
+  const int grid = (int)(units < num_sms() ? units : num_sms());
+  set_max_smem((const void*)scored_kernel<HD, FMT, CAP, BIAS>, smem);
+  scored_kernel<HD, FMT, CAP, BIAS><<<grid, kThreads, smem, st>>>(tq, tk, tv, p);
+}
+
+}  // namespace scored
 }  // namespace b2
 
 using namespace b2;
@@ -68,18 +539,22 @@ extern "C" int b2_flash_attn_fwd_scored(const void* q, const void* k, const void
   // scale > 0: the row maximum is taken before the scale.  fp32 stays fp32 here
   // (the plain kernel reads it as tf32 at head dim 64).
   unsigned* err = device_error_word();
-  if (wide && (D == 64 || D == 128) && dtype != B2_F32 && scale > 0.f && Skv > 0 && err) {
+  if (wide && (D == 64 || D == 128) && dtype != B2_F32 && scale > 0.f && Skv > 0 && err &&
+      B * Hq * ((Sq + fa::BQ - 1) / fa::BQ) <= (1 << 30)) {
     CUtensorMap tq, tk, tv;
     if (make_tmap_4d(&tq, q, dtype, D, Sq, Hq, B, qs) && make_tmap_4d(&tk, k, dtype, D, Skv, Hkv, B, ks) &&
         make_tmap_4d(&tv, v, dtype, D, Skv, Hkv, B, vs)) {
-      fa::Params p = {};
+      scored::Params p = {};
       p.B = (int)B;
       p.Hq = (int)Hq;
       p.Hkv = (int)Hkv;
       p.Sq = (int)Sq;
       p.Skv = (int)Skv;
       p.q_tiles = (int)((Sq + fa::BQ - 1) / fa::BQ);
-      p.scale_log2 = scale * fa::kLog2e;
+      // Q-tile pairs, or single Q tiles when the pairs would not fill the SMs
+      p.per = (int64_t)((p.q_tiles + 1) / 2) * Hq * B < num_sms() ? 1 : 2;
+      p.n_units = (p.q_tiles + p.per - 1) / p.per;
+      p.scale_log2 = scale * attn::kLog2e;
       p.o = o;
       p.os_b = os[0];
       p.os_h = os[1];
@@ -87,20 +562,19 @@ extern "C" int b2_flash_attn_fwd_scored(const void* q, const void* k, const void
       p.err = err;
       p.range = range;
       p.slopes = alibi_slopes;
-      p.cap_log2 = softcap * fa::kLog2e;
-      p.cap_in = softcap > 0.f ? 2.f * fa::kLog2e * scale / softcap : 0.f;
+      p.cap_log2 = softcap * attn::kLog2e;
+      p.cap_in = softcap > 0.f ? 2.f * attn::kLog2e * scale / softcap : 0.f;
+      p.z_in = softcap > 0.f ? scale / softcap : 0.f;
       p.v = (const uint16_t*)v;
       p.vs_b = vs[0];
       p.vs_h = vs[1];
       p.vs_s = vs[2];
-      p.single = (int64_t)((p.q_tiles + 1) / 2) * Hq * B < num_sms() ? 1 : 0;
-      const dim3 grid(p.single ? p.q_tiles : (p.q_tiles + 1) / 2, (unsigned)Hq, (unsigned)B);
-#define B2_SCORED(HD, FMT)                                                                     \
-  do {                                                                                         \
-    if (softcap > 0.f && alibi_slopes) launch_scored<HD, FMT, true, true>(tq, tk, tv, p, grid, st);   \
-    else if (softcap > 0.f) launch_scored<HD, FMT, true, false>(tq, tk, tv, p, grid, st);      \
-    else if (alibi_slopes) launch_scored<HD, FMT, false, true>(tq, tk, tv, p, grid, st);       \
-    else launch_scored<HD, FMT, false, false>(tq, tk, tv, p, grid, st);                        \
+#define B2_SCORED(HD, FMT)                                                                             \
+  do {                                                                                                 \
+    if (softcap > 0.f && alibi_slopes) scored::launch<HD, FMT, true, true>(tq, tk, tv, p, st);         \
+    else if (softcap > 0.f) scored::launch<HD, FMT, true, false>(tq, tk, tv, p, st);                   \
+    else if (alibi_slopes) scored::launch<HD, FMT, false, true>(tq, tk, tv, p, st);                    \
+    else scored::launch<HD, FMT, false, false>(tq, tk, tv, p, st);                                     \
   } while (0)
       if (D == 128 && dtype == B2_F16) B2_SCORED(128, fa::kF16);
       else if (D == 128) B2_SCORED(128, fa::kBF16);

@@ -67,7 +67,7 @@ struct Params {
   uint32_t page_size;           // 0: contiguous
   int max_pages;
   float scale_log2;             // scale * log2 e
-  float cap_log2, cap_in;       // softcap * log2 e; 2 log2 e * scale / softcap
+  float cap_log2, cap_in, z_in; // softcap * log2 e; 2 log2 e * scale / softcap; scale / softcap
   unsigned* err;
 };
 
@@ -148,7 +148,7 @@ __device__ __forceinline__ int64_t warp_sum(int64_t x) {
 // reads the mask rows of its tokens t0 .. t1 together (lane = drafted token),
 // eight rows in flight, and every lane keeps the ballots of its own token t.
 __device__ __forceinline__ void draft_bits(uint32_t (&bits)[4], const uint8_t* mask, int T, int t, int t0, int t1,
-                                           int j0, int dl, bool row_ok) {
+                                           int j0, int dl) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int w = 0; w < 4; ++w) bits[w] = 0;
@@ -167,12 +167,12 @@ __device__ __forceinline__ void draft_bits(uint32_t (&bits)[4], const uint8_t* m
       }
     }
   }
-  if (!row_ok) bits[0] = bits[1] = bits[2] = bits[3] = 0;
 }
 
 // Visible keys among the 128 from drafted token j0 (negative: context) on, from
-// the bits of the first 128 drafted tokens.
-__device__ __forceinline__ void visible_bits(uint32_t (&vis)[4], const uint32_t (&bits)[4], int j0, bool row_ok) {
+// the bits of the first 128 drafted tokens.  (A row without a drafted token
+// sees the context too: its output is made 0 at the end.)
+__device__ __forceinline__ void visible_bits(uint32_t (&vis)[4], const uint32_t (&bits)[4], int j0) {
 #pragma unroll
   for (int w = 0; w < 4; ++w) {
     const int j = j0 + 32 * w;
@@ -187,7 +187,7 @@ __device__ __forceinline__ void visible_bits(uint32_t (&vis)[4], const uint32_t 
       const uint32_t hi = i == 0 ? bits[1] : i == 1 ? bits[2] : i == 2 ? bits[3] : 0;
       x = __funnelshift_r(lo, hi, j & 31);
     }
-    vis[w] = row_ok ? x : 0;
+    vis[w] = x;
   }
 }
 
@@ -569,7 +569,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p) {
     const int u = (warp - 4) >> 2, qw = warp & 3, r = qw * 32 + lane;
     const uint32_t lane_off = (uint32_t)(qw * 32) << 16;
     const uint32_t tS = tmem + 256 * u + lane_off, tO = tmem + 128 + lane_off;  // tO: of unit 0
-    const Score score = {p.scale_log2, p.cap_in, p.cap_log2, 0.f, 0.f};
+    const Score score = {p.scale_log2, p.cap_in, p.cap_log2, p.z_in, 0.f, 0.f};
     uint32_t sc = 0, oc[2] = {0, 0}, seg = 0;  // S tiles / O accumulators waited for
     bool ok = true;
     while (walk.next(p, kRows, sg)) {
@@ -586,7 +586,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p) {
       // still on their way (wider trees read theirs tile by tile)
       uint32_t drafted[4] = {0, 0, 0, 0};
       if (warp_ok && (sg.tile + sg.n) * BK > sg.ctx)
-        draft_bits(drafted, mask, p.T, t, t0, t1, 0, min(sg.dl, 128), row_ok);
+        draft_bits(drafted, mask, p.T, t, t0, t1, 0, min(sg.dl, 128));
       float m_used = -INFINITY, l = 0.f;
       bool first = true;
       const int step = PAIR ? 1 : 2;
@@ -597,17 +597,18 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p) {
         tc::fence_after_sync();
         if (warp_ok) {
           const int kv0 = (sg.tile + j) * BK;
-          const bool masked = kv0 + BK > sg.ctx;
+          // SINGLE takes every tile with a bit per key: pieces that all rows see
+          // whole cost no more, and half the code is half the instruction
+          // fetches, which is what a short call waits for
+          const bool masked = !PAIR || kv0 + BK > sg.ctx;
           uint32_t vis[4];
           if (masked) {
-            if (sg.dl <= 128 || kv0 + BK <= sg.ctx + 128) {
-              visible_bits(vis, drafted, kv0 - sg.ctx, row_ok);
-            } else {
-              draft_bits(vis, mask, p.T, t, t0, t1, kv0 - sg.ctx, sg.dl, row_ok);
-              uint32_t before[4];
-              visible_bits(before, drafted, kv0 - sg.ctx, row_ok);
+            visible_bits(vis, drafted, kv0 - sg.ctx);
+            if (sg.dl > 128 && kv0 + BK > sg.ctx + 128) {
+              uint32_t more[4];
+              draft_bits(more, mask, p.T, t, t0, t1, kv0 - sg.ctx, sg.dl);
 #pragma unroll
-              for (int w = 0; w < 4; ++w) vis[w] |= before[w];
+              for (int w = 0; w < 4; ++w) vis[w] |= more[w];
             }
           }
           const float mx = masked ? score_max<true, CAP, false>(tS, vis, score) : score_max<false, CAP, false>(tS, vis, score);
@@ -1008,6 +1009,7 @@ extern "C" int b2_tree_attn(const void* q, const void* k, const void* v, void* o
     t.scale_log2 = scale * attn::kLog2e;
     t.cap_log2 = softcap * attn::kLog2e;
     t.cap_in = softcap > 0.f ? 2.f * attn::kLog2e * scale / softcap : 0.f;
+    t.z_in = softcap > 0.f ? scale / softcap : 0.f;
     t.err = p.err;
 #define B2_TREE(HD, FMT)                                              \
   do {                                                                \
