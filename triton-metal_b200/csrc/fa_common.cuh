@@ -164,14 +164,46 @@ __device__ __forceinline__ uint64_t exp2_poly_f2(uint64_t x2) {
 struct Score {
   float scale_log2;        // scale * log2 e (> 0)
   float cap_in, cap_log2;  // 2 log2 e scale / cap; cap * log2 e
-  float z_in;              // scale / cap
+  float small;             // scores up to this size take capped_small (0: none)
+  float t[5];              // its coefficients
   float slope, dist;       // slope * log2 e; row - first key of the tile
 };
+
+// What a kernel's parameters hold of the cap.
+struct Cap {
+  float in, log2, small, t[5];
+};
+__device__ __forceinline__ Score make_score(float scale_log2, const Cap& c) {
+  return {scale_log2, c.in, c.log2, c.small, {c.t[0], c.t[1], c.t[2], c.t[3], c.t[4]}, 0.f, 0.f};
+}
+// tanh z = z p(z^2) on [-3/4, 3/4]: this file's own minimax fit (largest error
+// 2.4e-7 in fp32).  The coefficients take scale, cap and log2 e with them, so
+// that a score s gives s q(s^2); where the powers of scale / cap would leave
+// fp32's range (scale / cap below 2e-4), the form is not used.
+inline Cap make_cap(float scale, float softcap) {
+  Cap c = {};
+  if (softcap > 0.f) {
+    const double log2e = 1.4426950408889634, z = (double)scale / softcap;
+    const double p[5] = {0.9999971985816956, -0.33323076367378235, 0.13226091861724854, -0.04928044602274895,
+                         0.012318830005824566};
+    c.in = (float)(2 * log2e * z);
+    c.log2 = (float)(log2e * softcap);
+    c.small = z > 2e-4 ? (float)(0.75 / z) : 0.f;
+    double f = log2e * softcap * z;
+    for (int i = 0; i < 5; ++i, f *= z * z) c.t[i] = (float)(p[i] * f);
+  }
+  return c;
+}
 
 __device__ __forceinline__ float rcp_approx(float x) {
   float y;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+__device__ __forceinline__ uint64_t mul_f2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
 }
 
 // cap tanh(scale s / cap) + add: tanh y = 1 - 2 / (1 + e^2y), good to ~2e-7
@@ -180,24 +212,15 @@ __device__ __forceinline__ float rcp_approx(float x) {
 __device__ __forceinline__ float capped(float s, const Score& c, float add) {
   return fmaf(-2.f * c.cap_log2, rcp_approx(1.f + ex2(s * c.cap_in)), c.cap_log2 + add);
 }
-
-// The same for two scores of at most kSmallCap of the cap, on the FMA pipe: the
-// two MUFU operations a score of the form above would set the pace of the
-// softmax.  tanh z = z p(z^2), this file's own minimax fit on [-3/4, 3/4]
-// (largest error 2.4e-7 in fp32).
-constexpr float kSmallCap = 0.75f;
-__device__ __forceinline__ uint64_t mul_f2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
+// The same for two scores of at most c.small, on the FMA pipe: the two MUFU
+// operations a score of the form above would set the pace of the softmax.
 __device__ __forceinline__ uint64_t capped_small(uint64_t s, const Score& c, uint64_t add) {
-  const uint64_t z = mul_f2(s, f2_pack(c.z_in, c.z_in)), w = mul_f2(z, z);
-  uint64_t q = fma_f2(f2_pack(0.01231883f, 0.01231883f), w, f2_pack(-0.049280446f, -0.049280446f));
-  q = fma_f2(q, w, f2_pack(0.13226092f, 0.13226092f));
-  q = fma_f2(q, w, f2_pack(-0.33323076f, -0.33323076f));
-  q = fma_f2(q, w, f2_pack(0.9999972f, 0.9999972f));
-  return fma_f2(mul_f2(z, f2_pack(c.cap_log2, c.cap_log2)), q, add);
+  const uint64_t w = mul_f2(s, s);
+  uint64_t q = fma_f2(f2_pack(c.t[4], c.t[4]), w, f2_pack(c.t[3], c.t[3]));
+  q = fma_f2(q, w, f2_pack(c.t[2], c.t[2]));
+  q = fma_f2(q, w, f2_pack(c.t[1], c.t[1]));
+  q = fma_f2(q, w, f2_pack(c.t[0], c.t[0]));
+  return fma_f2(s, q, add);
 }
 // Whether all of the warp's N x 32 scores may take capped_small.
 template <int N>
@@ -205,7 +228,7 @@ __device__ __forceinline__ bool all_small(const uint32_t (&sv)[N], const Score& 
   float am = 0.f;
 #pragma unroll
   for (int e = 0; e < N; e += 2) am = max3(am, fabsf(__uint_as_float(sv[e])), fabsf(__uint_as_float(sv[e + 1])));
-  return !__any_sync(0xffffffffu, !(am * c.z_in <= kSmallCap));
+  return !__any_sync(0xffffffffu, !(am <= c.small));
 }
 
 // Score of two neighbouring keys (e and e + 1 from where c.dist counts), plus
@@ -217,7 +240,8 @@ __device__ __forceinline__ uint64_t score_pair(uint32_t s0, uint32_t s1, int e, 
   uint64_t a = f2_pack(add, add);
   if constexpr (BIAS) {
     if constexpr (ABS) {
-      a = f2_pack(fmaf(-c.slope, fabsf(c.dist - (float)e), add), fmaf(-c.slope, fabsf(c.dist - (float)(e + 1)), add));
+      const float sl = -fabsf(c.slope);
+      a = f2_pack(fmaf(sl, fabsf(c.dist - (float)e), add), fmaf(sl, fabsf(c.dist - (float)(e + 1)), add));
     } else {
       const float b = fmaf(-c.slope, c.dist, add);
       a = fma_f2(f2_pack(c.slope, c.slope), f2_pack((float)e, (float)(e + 1)), f2_pack(b, b));
@@ -243,17 +267,17 @@ __device__ __forceinline__ void score_chunk(uint32_t (&sv)[N], const Score& c) {
 
 // Largest score (without a bias: largest raw score) of N columns; BITS: of those
 // with a bit in w (N = 32).
-template <bool BITS, bool ABS, bool CAP, bool BIAS, int N>
+template <bool BITS, bool CAP, bool BIAS, int N>
 __device__ __forceinline__ float max_chunk(uint32_t (&sv)[N], uint32_t w, const Score& c, float mx) {
   if constexpr (CAP && BIAS) {
-    if (all_small(sv, c)) score_chunk<ABS, true>(sv, c);
-    else score_chunk<ABS, false>(sv, c);
+    if (all_small(sv, c)) score_chunk<BITS, true>(sv, c);
+    else score_chunk<BITS, false>(sv, c);
   }
 #pragma unroll
   for (int e = 0; e < N; e += 2) {
     float v0 = __uint_as_float(sv[e]), v1 = __uint_as_float(sv[e + 1]);
     if constexpr (BIAS && !CAP) {
-      const uint64_t x = score_pair<ABS, CAP, BIAS, false>(sv[e], sv[e + 1], e, c, 0.f);
+      const uint64_t x = score_pair<BITS, CAP, BIAS, false>(sv[e], sv[e + 1], e, c, 0.f);
       v0 = f2_lo(x);
       v1 = f2_hi(x);
     }
@@ -266,35 +290,36 @@ __device__ __forceinline__ float max_chunk(uint32_t (&sv)[N], uint32_t w, const 
   return mx;
 }
 
+// A tile that the warp's rows see whole is gone through in halves of 64 keys
+// (two TMEM loads a wait); another one in four pieces of 32.  A piece that each
+// row sees whole or not at all (and, with a bias, whose keys lie on one side of
+// the rows) takes the short way; one that nobody sees is passed over; the rest
+// are masked by bits.  So a document's border costs no more than its one mixed
+// piece, however many tiles the rows above and below it do not share.
+enum Piece { kNone, kRows, kBits };
+__device__ __forceinline__ Piece piece_of(uint32_t w, bool rows_ok) {
+  if (!__any_sync(0xffffffffu, w != 0)) return kNone;
+  return rows_ok && __all_sync(0xffffffffu, w == 0 || w == 0xffffffffu) ? kRows : kBits;
+}
 __device__ __forceinline__ uint32_t word_of(const uint32_t (&vis)[4], int c) {
   return c == 0 ? vis[0] : c == 1 ? vis[1] : c == 2 ? vis[2] : vis[3];
 }
+// the warp's rows see all 128 keys
+__device__ __forceinline__ bool whole_tile(const uint32_t (&vis)[4]) {
+  return __all_sync(0xffffffffu, (vis[0] & vis[1] & vis[2] & vis[3]) == 0xffffffffu);
+}
 
-// Largest score of the row's visible keys, -inf without one.  Scale and cap
-// keep the order, so without a bias the raw maximum is taken and scored once.
-// With cap and bias both, the scores are left in the S columns for score_exp.
-// MASK: visible keys as bits; of the four 32-key pieces those that no row of the
-// warp sees are passed over, and those that all of its rows see whole cost no
-// more than in an unmasked tile (on a diagonal or at a document's border one
-// piece in four is mixed).
-template <bool MASK, bool CAP, bool BIAS>
-__device__ __forceinline__ float score_max(uint32_t tS, const uint32_t (&vis)[4], const Score& sc) {
+// Largest score of the row's visible keys (bits of vis), -inf without one.
+// WIDE: with the way for whole tiles, taken where `whole` says so (all bits set
+// in the warp, and with a bias all keys on one side); one_side: see score_pair.
+// Scale and cap keep the order, so without a bias the raw maximum is taken and
+// scored once.  With cap and bias both, the scores are left in the S columns
+// for score_exp.
+template <bool WIDE, bool CAP, bool BIAS>
+__device__ __forceinline__ float score_max(uint32_t tS, const uint32_t (&vis)[4], bool whole, bool one_side,
+                                           const Score& sc) {
   float mx = -INFINITY;
-  if constexpr (MASK) {
-#pragma unroll 1
-    for (int c = 0; c < 4; ++c) {
-      const uint32_t w = word_of(vis, c);
-      if (!__any_sync(0xffffffffu, w != 0)) continue;
-      uint32_t sv[32];
-      tc::tmem_ld_32x32b_x32(tS + 32 * c, sv);
-      tc::tmem_ld_wait();
-      Score cc = sc;
-      cc.dist -= 32.f * c;
-      if (__all_sync(0xffffffffu, w == 0xffffffffu)) mx = max_chunk<false, true, CAP, BIAS>(sv, w, cc, mx);
-      else mx = max_chunk<true, true, CAP, BIAS>(sv, w, cc, mx);
-      if constexpr (CAP && BIAS) tmem_st_32x32b_x32(tS + 32 * c, sv);
-    }
-  } else {
+  if (WIDE && whole) {
 #pragma unroll 1
     for (int c = 0; c < 4; c += 2) {
       uint32_t sv[64];
@@ -303,11 +328,30 @@ __device__ __forceinline__ float score_max(uint32_t tS, const uint32_t (&vis)[4]
       tc::tmem_ld_wait();
       Score cc = sc;
       cc.dist -= 32.f * c;
-      mx = max_chunk<false, false, CAP, BIAS>(sv, 0, cc, mx);
+      mx = max_chunk<false, CAP, BIAS>(sv, 0, cc, mx);
       if constexpr (CAP && BIAS) {
         tmem_st_32x32b_x32(tS + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(sv));
         tmem_st_32x32b_x32(tS + 32 * c + 32, *reinterpret_cast<uint32_t(*)[32]>(sv + 32));
       }
+    }
+  } else {
+#pragma unroll 1
+    for (int c = 0; c < 4; ++c) {
+      const uint32_t w = word_of(vis, c);
+      const Piece kind = piece_of(w, !BIAS || one_side);
+      if (kind == kNone) continue;
+      uint32_t sv[32];
+      tc::tmem_ld_32x32b_x32(tS + 32 * c, sv);
+      tc::tmem_ld_wait();
+      Score cc = sc;
+      cc.dist -= 32.f * c;
+      if (kind == kRows) {
+        const float m = max_chunk<false, CAP, BIAS>(sv, 0, cc, -INFINITY);
+        mx = fmaxf(mx, w ? m : -INFINITY);
+      } else {
+        mx = max_chunk<true, CAP, BIAS>(sv, w, cc, mx);
+      }
+      if constexpr (CAP && BIAS) tmem_st_32x32b_x32(tS + 32 * c, sv);
     }
   }
   if constexpr (CAP && BIAS) tmem_st_wait();
@@ -319,7 +363,7 @@ __device__ __forceinline__ float score_max(uint32_t tS, const uint32_t (&vis)[4]
 }
 
 // p = exp2(score - m) of N columns as 16-bit pairs; their sum goes to rs.
-template <bool BITS, bool ABS, int FMT, bool CAP, bool BIAS, bool SMALL, int N>
+template <bool BITS, int FMT, bool CAP, bool BIAS, bool SMALL, int N>
 __device__ __forceinline__ void exp_chunk(const uint32_t (&sv)[N], uint32_t (&pk)[N / 2], uint64_t& rs, uint32_t w,
                                           const Score& c, float mref) {
 #pragma unroll
@@ -327,8 +371,10 @@ __device__ __forceinline__ void exp_chunk(const uint32_t (&sv)[N], uint32_t (&pk
     float p0, p1;
     uint64_t x;
     if constexpr (CAP && BIAS) x = add_f2((uint64_t)sv[2 * e] | ((uint64_t)sv[2 * e + 1] << 32), f2_pack(-mref, -mref));
-    else x = score_pair<ABS, CAP, BIAS, SMALL>(sv[2 * e], sv[2 * e + 1], 2 * e, c, -mref);
-    if (e % 3 == 2) {  // a third of the exponentials on the FMA pipe, as in the prefill kernel
+    else x = score_pair<BITS, CAP, BIAS, SMALL>(sv[2 * e], sv[2 * e + 1], 2 * e, c, -mref);
+    // part of the exponentials on the FMA pipe: a third, as in the prefill
+    // kernel, but fewer beside the cap, which has filled it already
+    if (SMALL ? e % 8 == 7 : e % 3 == 2) {
       const uint64_t y = exp2_poly_f2(x);
       p0 = f2_lo(y);
       p1 = f2_hi(y);
@@ -350,44 +396,26 @@ __device__ __forceinline__ void exp_chunk(const uint32_t (&sv)[N], uint32_t (&pk
     }
   }
 }
-template <bool BITS, bool ABS, int FMT, bool CAP, bool BIAS, int N>
+template <bool BITS, int FMT, bool CAP, bool BIAS, int N>
 __device__ __forceinline__ void exp_chunk_any(const uint32_t (&sv)[N], uint32_t (&pk)[N / 2], uint64_t& rs, uint32_t w,
                                               const Score& c, float mref) {
   if constexpr (CAP && !BIAS) {
     if (all_small(sv, c)) {
-      exp_chunk<BITS, ABS, FMT, CAP, BIAS, true>(sv, pk, rs, w, c, mref);
+      exp_chunk<BITS, FMT, CAP, BIAS, true>(sv, pk, rs, w, c, mref);
       return;
     }
   }
-  exp_chunk<BITS, ABS, FMT, CAP, BIAS, false>(sv, pk, rs, w, c, mref);
+  exp_chunk<BITS, FMT, CAP, BIAS, false>(sv, pk, rs, w, c, mref);
 }
 
 // p = exp2(score - m) as 16-bit pairs over the S columns; returns their sum.
 // P rounded to 16 bits (half a step of its own size) is what the MMA takes; the
 // sum is taken before that, in 32 bits.
-template <bool MASK, int FMT, bool CAP, bool BIAS>
-__device__ __forceinline__ float score_exp(uint32_t tS, const uint32_t (&vis)[4], float mref, const Score& sc) {
-  uint64_t rs = 0;
-  if constexpr (MASK) {
-#pragma unroll 1
-    for (int c = 0; c < 4; ++c) {
-      const uint32_t w = word_of(vis, c);
-      uint32_t pk[16];
-      if (!__any_sync(0xffffffffu, w != 0)) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) pk[e] = 0;
-      } else {
-        uint32_t sv[32];
-        tc::tmem_ld_32x32b_x32(tS + 32 * c, sv);
-        tc::tmem_ld_wait();
-        Score cc = sc;
-        cc.dist -= 32.f * c;
-        if (__all_sync(0xffffffffu, w == 0xffffffffu)) exp_chunk_any<false, true, FMT, CAP, BIAS>(sv, pk, rs, w, cc, mref);
-        else exp_chunk_any<true, true, FMT, CAP, BIAS>(sv, pk, rs, w, cc, mref);
-      }
-      tmem_st_32x32b_x16(tS + 16 * c, pk);
-    }
-  } else {
+template <bool WIDE, int FMT, bool CAP, bool BIAS>
+__device__ __forceinline__ float score_exp(uint32_t tS, const uint32_t (&vis)[4], bool whole, bool one_side, float mref,
+                                           const Score& sc) {
+  if (WIDE && whole) {
+    uint64_t rs = 0;
 #pragma unroll 1
     for (int c = 0; c < 4; c += 2) {
       uint32_t sv[64];
@@ -397,11 +425,40 @@ __device__ __forceinline__ float score_exp(uint32_t tS, const uint32_t (&vis)[4]
       Score cc = sc;
       cc.dist -= 32.f * c;
       uint32_t pk[32];
-      exp_chunk_any<false, false, FMT, CAP, BIAS>(sv, pk, rs, 0, cc, mref);
+      exp_chunk_any<false, FMT, CAP, BIAS>(sv, pk, rs, 0, cc, mref);
       tmem_st_32x32b_x32(tS + 16 * c, pk);
     }
+    return f2_lo(rs) + f2_hi(rs);
   }
-  return f2_lo(rs) + f2_hi(rs);
+  float sum = 0.f;
+#pragma unroll 1
+  for (int c = 0; c < 4; ++c) {
+    const uint32_t w = word_of(vis, c);
+    const Piece kind = piece_of(w, !BIAS || one_side);
+    uint32_t pk[16];
+    if (kind == kNone) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) pk[e] = 0;
+    } else {
+      uint32_t sv[32];
+      tc::tmem_ld_32x32b_x32(tS + 32 * c, sv);
+      tc::tmem_ld_wait();
+      Score cc = sc;
+      cc.dist -= 32.f * c;
+      uint64_t rs = 0;
+      if (kind == kRows) {
+        exp_chunk_any<false, FMT, CAP, BIAS>(sv, pk, rs, 0, cc, mref);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) pk[e] &= w;  // all or nothing
+        sum += w ? f2_lo(rs) + f2_hi(rs) : 0.f;
+      } else {
+        exp_chunk_any<true, FMT, CAP, BIAS>(sv, pk, rs, w, cc, mref);
+        sum += f2_lo(rs) + f2_hi(rs);
+      }
+    }
+    tmem_st_32x32b_x16(tS + 16 * c, pk);
+  }
+  return sum;
 }
 
 template <int FMT>

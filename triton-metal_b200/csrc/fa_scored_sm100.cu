@@ -43,7 +43,8 @@ struct Params {
   int B, Hq, Hkv, Sq, Skv, q_tiles;
   int per, n_units;        // Q tiles of a unit (1 where pairs would not fill the SMs); units of a head
   attn::RangeMask range;
-  float scale_log2, cap_in, cap_log2, z_in;
+  float scale_log2;
+  Cap cap;
   const float* slopes;     // [Hq]
   void* o;
   int64_t os_b, os_h, os_s;
@@ -81,6 +82,12 @@ struct Info {
   }
   __device__ __forceinline__ int last() const { return max(nkv[0], nkv[1]); }
 };
+
+__device__ __forceinline__ void prefetch_4d(const CUtensorMap* map, int d, int s, int h, int b) {
+  asm volatile("cp.async.bulk.prefetch.tensor.4d.L2.global.tile [%0, {%1, %2, %3, %4}];" ::"l"(map), "r"(d), "r"(s),
+               "r"(h), "r"(b)
+               : "memory");
+}
 
 // Bits of the keys of [lo, hi) among the 128 from kv0 on.
 __device__ __forceinline__ void range_bits(uint32_t (&vis)[4], int lo, int hi, int kv0) {
@@ -187,6 +194,12 @@ scored_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
         const int jb = f.first(), je = f.last();
         if (je == 0) continue;
         const int hk = un.h / (p.Hq / p.Hkv);
+        // Q has one buffer, free only when the unit before has all its S: have it
+        // in L2 by then
+        for (int u = 0; u < 2; ++u)
+          if (k > 0 && f.nkv[u] > 0)
+#pragma unroll
+            for (int a = 0; a < Cf::NATOM; ++a) prefetch_4d(&tmQ, a * Cf::AE, un.q0 + u * BQ, un.h, un.b);
         ok = wait_abort(q_empty, (qn & 1) ^ 1, p.err, 0xB2600002u, abort_flag);
         if (!ok) break;
         ++qn;
@@ -367,14 +380,21 @@ scored_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
     const int u = (warp - 4) >> 2, qw = warp & 3, r = qw * 32 + lane;
     const uint32_t lane_off = (uint32_t)(qw * 32) << 16;
     const uint32_t tS = tmem + 256 * u + lane_off, tO = tS + 128;
-    Score score = {p.scale_log2, p.cap_in, p.cap_log2, p.z_in, 0.f, 0.f};
+    Score score = make_score(p.scale_log2, p.cap);
     uint32_t sc = 0, oc = 0;  // S tiles / outputs waited for
     bool ok = true;
+    int next_lo = 0, next_hi = 0;
+    auto find_row = [&](int k) {  // keys of this thread's row in turn k
+      Unit n;
+      next_lo = next_hi = 0;
+      if (unit_of(p, k, n) && u < p.per && n.q0 + u * BQ + r < p.Sq)
+        attn::row_range(p.range, n.b, n.q0 + u * BQ + r, p.Skv, next_lo, next_hi);
+    };
+    find_row(0);
     for (int k = 0; ok && unit_of(p, k, un); ++k) {
       const int q0 = un.q0 + u * BQ, qpos = q0 + r;
       const bool exists = u < p.per && qpos < p.Sq;
-      int row_lo = 0, row_hi = 0;
-      if (exists) attn::row_range(p.range, un.b, qpos, p.Skv, row_lo, row_hi);
+      const int row_lo = next_lo, row_hi = next_hi;
       float slope = 0.f;
       if constexpr (BIAS) slope = p.slopes[un.h] * attn::kLog2e;
       ok = __all_sync(0xffffffffu, wait_abort(&info_full[k & 1], (k >> 1) & 1, p.err, 0xB260000Eu, abort_flag));
@@ -390,17 +410,15 @@ scored_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
         ++sc;
         tc::fence_after_sync();
         const int kv0 = j * BKV;
-        bool need_mask = f.masked(u, j);
+        const bool one_side = kv0 + BKV - 1 <= q0 || kv0 >= q0 + BQ - 1;  // where the tile's rows are not in it
         if constexpr (BIAS) {
-          // the bias is linear over the tile unless the tile's rows lie in it
-          const bool before = kv0 + BKV - 1 <= q0, behind = kv0 >= q0 + BQ - 1;
-          need_mask = need_mask || !(before || behind);
           score.dist = (float)(qpos - kv0);
-          score.slope = need_mask || before ? slope : -slope;
+          score.slope = kv0 <= q0 ? slope : -slope;
         }
-        uint32_t vis[4] = {0, 0, 0, 0};
-        if (need_mask) range_bits(vis, row_lo, row_hi, kv0);
-        const float mx = need_mask ? score_max<true, CAP, BIAS>(tS, vis, score) : score_max<false, CAP, BIAS>(tS, vis, score);
+        uint32_t vis[4] = {~0u, ~0u, ~0u, ~0u};
+        if (f.masked(u, j)) range_bits(vis, row_lo, row_hi, kv0);
+        const bool whole = (!BIAS || one_side) && whole_tile(vis);
+        const float mx = score_max<true, CAP, BIAS>(tS, vis, whole, one_side, score);
         // lazy, warp-uniform rescale of O (O_u is quiescent: PV_u(j-1) finished)
         const bool need = mx > m_used + kRescale;
         const float alpha = need ? ((m_used == -INFINITY) ? 0.f : ex2(m_used - mx)) : 1.f;
@@ -420,14 +438,14 @@ scored_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
           }
         }
         const float mref = (m_used == -INFINITY) ? 0.f : m_used;
-        l += need_mask ? score_exp<true, FMT, CAP, BIAS>(tS, vis, mref, score)
-                       : score_exp<false, FMT, CAP, BIAS>(tS, vis, mref, score);
+        l += score_exp<true, FMT, CAP, BIAS>(tS, vis, whole, one_side, mref, score);
         tmem_st_wait();
         tc::fence_before_sync();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_ready[u]);
       }
       if (!ok) break;
+      find_row(k + 1);  // under the last PV
       // O_u / l -> global (rows beyond Sq are not stored)
       uint16_t* orow = reinterpret_cast<uint16_t*>(p.o) + un.b * p.os_b + un.h * p.os_h + (int64_t)qpos * p.os_s;
       if (nkv == kb) {  // no row of the tile sees anything: zeros
@@ -562,9 +580,7 @@ extern "C" int b2_flash_attn_fwd_scored(const void* q, const void* k, const void
       p.err = err;
       p.range = range;
       p.slopes = alibi_slopes;
-      p.cap_log2 = softcap * attn::kLog2e;
-      p.cap_in = softcap > 0.f ? 2.f * attn::kLog2e * scale / softcap : 0.f;
-      p.z_in = softcap > 0.f ? scale / softcap : 0.f;
+      p.cap = fa::make_cap(scale, softcap);
       p.v = (const uint16_t*)v;
       p.vs_b = vs[0];
       p.vs_h = vs[1];

@@ -67,7 +67,7 @@ struct Params {
   uint32_t page_size;           // 0: contiguous
   int max_pages;
   float scale_log2;             // scale * log2 e
-  float cap_log2, cap_in, z_in; // softcap * log2 e; 2 log2 e * scale / softcap; scale / softcap
+  Cap softcap;
   unsigned* err;
 };
 
@@ -569,7 +569,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p) {
     const int u = (warp - 4) >> 2, qw = warp & 3, r = qw * 32 + lane;
     const uint32_t lane_off = (uint32_t)(qw * 32) << 16;
     const uint32_t tS = tmem + 256 * u + lane_off, tO = tmem + 128 + lane_off;  // tO: of unit 0
-    const Score score = {p.scale_log2, p.cap_in, p.cap_log2, p.z_in, 0.f, 0.f};
+    const Score score = make_score(p.scale_log2, p.softcap);
     uint32_t sc = 0, oc[2] = {0, 0}, seg = 0;  // S tiles / O accumulators waited for
     bool ok = true;
     while (walk.next(p, kRows, sg)) {
@@ -597,12 +597,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p) {
         tc::fence_after_sync();
         if (warp_ok) {
           const int kv0 = (sg.tile + j) * BK;
-          // SINGLE takes every tile with a bit per key: pieces that all rows see
-          // whole cost no more, and half the code is half the instruction
-          // fetches, which is what a short call waits for
-          const bool masked = !PAIR || kv0 + BK > sg.ctx;
-          uint32_t vis[4];
-          if (masked) {
+          uint32_t vis[4] = {~0u, ~0u, ~0u, ~0u};
+          if (kv0 + BK > sg.ctx) {
             visible_bits(vis, drafted, kv0 - sg.ctx);
             if (sg.dl > 128 && kv0 + BK > sg.ctx + 128) {
               uint32_t more[4];
@@ -611,7 +607,10 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p) {
               for (int w = 0; w < 4; ++w) vis[w] |= more[w];
             }
           }
-          const float mx = masked ? score_max<true, CAP, false>(tS, vis, score) : score_max<false, CAP, false>(tS, vis, score);
+          // SINGLE has no way of its own for whole tiles: half the code is half the
+          // instruction fetches, which is what a short call waits for
+          const bool whole = PAIR && whole_tile(vis);
+          const float mx = score_max<PAIR, CAP, false>(tS, vis, whole, true, score);
           const bool need = mx > m_used + kRescale;
           const float alpha = need ? (m_used == -INFINITY ? 0.f : ex2(m_used - mx)) : 1.f;
           if (need) {
@@ -631,8 +630,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p) {
             }
           }
           const float mref = m_used == -INFINITY ? 0.f : m_used;
-          l += masked ? score_exp<true, FMT, CAP, false>(tS, vis, mref, score)
-                      : score_exp<false, FMT, CAP, false>(tS, vis, mref, score);
+          l += score_exp<PAIR, FMT, CAP, false>(tS, vis, whole, true, mref, score);
           tmem_st_wait();
         }
         first = false;
@@ -1007,9 +1005,7 @@ extern "C" int b2_tree_attn(const void* q, const void* k, const void* v, void* o
     t.page_size = (uint32_t)page_size;
     t.max_pages = (int)max_pages;
     t.scale_log2 = scale * attn::kLog2e;
-    t.cap_log2 = softcap * attn::kLog2e;
-    t.cap_in = softcap > 0.f ? 2.f * attn::kLog2e * scale / softcap : 0.f;
-    t.z_in = softcap > 0.f ? scale / softcap : 0.f;
+    t.softcap = fa::make_cap(scale, softcap);
     t.err = p.err;
 #define B2_TREE(HD, FMT)                                              \
   do {                                                                \
