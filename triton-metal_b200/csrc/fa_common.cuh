@@ -290,12 +290,12 @@ __device__ __forceinline__ float max_chunk(uint32_t (&sv)[N], uint32_t w, const 
   return mx;
 }
 
-// A tile that the warp's rows see whole is gone through in halves of 64 keys
-// (two TMEM loads a wait); another one in four pieces of 32.  A piece that each
-// row sees whole or not at all (and, with a bias, whose keys lie on one side of
-// the rows) takes the short way; one that nobody sees is passed over; the rest
-// are masked by bits.  So a document's border costs no more than its one mixed
-// piece, however many tiles the rows above and below it do not share.
+// A tile that each of the warp's rows sees whole or not at all is gone through
+// in halves of 64 keys (two TMEM loads a wait), another one in four pieces of
+// 32.  Of those, one that each row sees whole or not at all (and, with a bias,
+// whose keys lie on one side of the rows) takes the short way too, one that
+// nobody sees is passed over, and the rest are masked by bits.  So a document's
+// border costs little in the many tiles that lie to one side of it.
 enum Piece { kNone, kRows, kBits };
 __device__ __forceinline__ Piece piece_of(uint32_t w, bool rows_ok) {
   if (!__any_sync(0xffffffffu, w != 0)) return kNone;
@@ -304,14 +304,15 @@ __device__ __forceinline__ Piece piece_of(uint32_t w, bool rows_ok) {
 __device__ __forceinline__ uint32_t word_of(const uint32_t (&vis)[4], int c) {
   return c == 0 ? vis[0] : c == 1 ? vis[1] : c == 2 ? vis[2] : vis[3];
 }
-// the warp's rows see all 128 keys
+// each of the warp's rows sees all 128 keys or none (vis[0] says which)
 __device__ __forceinline__ bool whole_tile(const uint32_t (&vis)[4]) {
-  return __all_sync(0xffffffffu, (vis[0] & vis[1] & vis[2] & vis[3]) == 0xffffffffu);
+  return __all_sync(0xffffffffu, (vis[0] & vis[1] & vis[2] & vis[3]) == 0xffffffffu ||
+                                     (vis[0] | vis[1] | vis[2] | vis[3]) == 0);
 }
 
 // Largest score of the row's visible keys (bits of vis), -inf without one.
-// WIDE: with the way for whole tiles, taken where `whole` says so (all bits set
-// in the warp, and with a bias all keys on one side); one_side: see score_pair.
+// WIDE: with the way for whole tiles, taken where `whole` says so (whole_tile,
+// and with a bias all keys on one side); one_side: see score_pair.
 // Scale and cap keep the order, so without a bias the raw maximum is taken and
 // scored once.  With cap and bias both, the scores are left in the S columns
 // for score_exp.
@@ -320,6 +321,7 @@ __device__ __forceinline__ float score_max(uint32_t tS, const uint32_t (&vis)[4]
                                            const Score& sc) {
   float mx = -INFINITY;
   if (WIDE && whole) {
+    if (!__any_sync(0xffffffffu, vis[0] != 0)) return -INFINITY;
 #pragma unroll 1
     for (int c = 0; c < 4; c += 2) {
       uint32_t sv[64];
@@ -334,6 +336,7 @@ __device__ __forceinline__ float score_max(uint32_t tS, const uint32_t (&vis)[4]
         tmem_st_32x32b_x32(tS + 32 * c + 32, *reinterpret_cast<uint32_t(*)[32]>(sv + 32));
       }
     }
+    if (!vis[0]) mx = -INFINITY;
   } else {
 #pragma unroll 1
     for (int c = 0; c < 4; ++c) {
@@ -426,9 +429,11 @@ __device__ __forceinline__ float score_exp(uint32_t tS, const uint32_t (&vis)[4]
       cc.dist -= 32.f * c;
       uint32_t pk[32];
       exp_chunk_any<false, FMT, CAP, BIAS>(sv, pk, rs, 0, cc, mref);
+#pragma unroll
+      for (int e = 0; e < 32; ++e) pk[e] &= vis[0];  // all or nothing
       tmem_st_32x32b_x32(tS + 16 * c, pk);
     }
-    return f2_lo(rs) + f2_hi(rs);
+    return vis[0] ? f2_lo(rs) + f2_hi(rs) : 0.f;
   }
   float sum = 0.f;
 #pragma unroll 1

@@ -24,9 +24,10 @@ using namespace fa;
 // The pipeline of the plain prefill kernel (fa_fwd_sm100.cu: two Q tiles in
 // ping-pong, P in TMEM), made persistent: with short documents a unit (a pair
 // of Q tiles of one head) has a handful of KV tiles, and what counts is how
-// soon the next one starts.  One CTA per SM walks units; the next unit's Q, K
-// and V are loaded and its first S is computed while this one's last softmax
-// and output are under way.
+// soon the next one starts.  One CTA per SM walks units; the next unit's first
+// Q, K and V tiles are loaded and its first S is computed while this one's last
+// softmax and output are under way (three Q tiles of room and two K tiles,
+// where the plain kernel has two and three).
 //   warp 0      TMA
 //   warp 1      TMEM owner, MMA issuer
 //   warps 2-3   key ranges of the next unit (which KV tiles its Q tiles visit,
@@ -37,6 +38,7 @@ using namespace fa;
 //   warps 4-11  two softmax warpgroups, one per Q tile, one row per thread
 // ---------------------------------------------------------------------------
 constexpr int kThreads = 384;
+constexpr int kQ = 3, kK = 2, kV = 2;  // tiles of each ring
 constexpr float kRescale = 8.f;  // log2 units
 
 struct Params {
@@ -83,12 +85,6 @@ struct Info {
   __device__ __forceinline__ int last() const { return max(nkv[0], nkv[1]); }
 };
 
-__device__ __forceinline__ void prefetch_4d(const CUtensorMap* map, int d, int s, int h, int b) {
-  asm volatile("cp.async.bulk.prefetch.tensor.4d.L2.global.tile [%0, {%1, %2, %3, %4}];" ::"l"(map), "r"(d), "r"(s),
-               "r"(h), "r"(b)
-               : "memory");
-}
-
 // Bits of the keys of [lo, hi) among the 128 from kv0 on.
 __device__ __forceinline__ void range_bits(uint32_t (&vis)[4], int lo, int hi, int kv0) {
 #pragma unroll
@@ -107,17 +103,17 @@ scored_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
   constexpr int kTile = Cf::kTile, kAtom = Cf::kAtom;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
-  uint8_t* sQ = smem;  // 2 tiles
-  uint8_t* sK = sQ + 2 * kTile;
-  uint8_t* sV = sK + kKStages * kTile;
-  uint64_t* q_full = reinterpret_cast<uint64_t*>(sV + kVStages * kTile);
-  uint64_t* q_empty = q_full + 1;
-  uint64_t* k_full = q_empty + 1;
-  uint64_t* k_empty = k_full + kKStages;
-  uint64_t* v_full = k_empty + kKStages;
-  uint64_t* v_clean = v_full + kVStages;
-  uint64_t* v_empty = v_clean + kVStages;
-  uint64_t* s_full = v_empty + kVStages;      // [2] per Q tile
+  uint8_t* sQ = smem;  // a unit's two Q tiles and the next one's first
+  uint8_t* sK = sQ + kQ * kTile;
+  uint8_t* sV = sK + kK * kTile;
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(sV + kV * kTile);
+  uint64_t* q_empty = q_full + kQ;
+  uint64_t* k_full = q_empty + kQ;
+  uint64_t* k_empty = k_full + kK;
+  uint64_t* v_full = k_empty + kK;
+  uint64_t* v_clean = v_full + kV;
+  uint64_t* v_empty = v_clean + kV;
+  uint64_t* s_full = v_empty + kV;            // [2] per Q tile
   uint64_t* p_ready = s_full + 2;             // [2]
   uint64_t* o_done = p_ready + 2;             // [2]
   uint64_t* info_full = o_done + 2;           // [2] by unit parity
@@ -127,17 +123,19 @@ scored_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
   volatile int* s_bad = reinterpret_cast<volatile int*>(tmem_holder + 2);      // [4]: unit with a bad V value
   int4* s_info = reinterpret_cast<int4*>(q_full + 32);                         // [2 parities][2 warps][2 tiles]
-  static_assert(2 + 2 * kKStages + 3 * kVStages + 11 + 3 <= 32, "barriers");
+  static_assert(2 * kQ + 2 * kK + 3 * kV + 11 + 3 <= 32, "barriers");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    mbar_init(q_full, 1);
-    mbar_init(q_empty, 1);
-    for (int i = 0; i < kKStages; ++i) {
+    for (int i = 0; i < kQ; ++i) {
+      mbar_init(&q_full[i], 1);
+      mbar_init(&q_empty[i], 1);
+    }
+    for (int i = 0; i < kK; ++i) {
       mbar_init(&k_full[i], 1);
       mbar_init(&k_empty[i], 1);
     }
-    for (int i = 0; i < kVStages; ++i) {
+    for (int i = 0; i < kV; ++i) {
       mbar_init(&v_full[i], 1);
       mbar_init(&v_clean[i], 64);
       mbar_init(&v_empty[i], 1);
@@ -184,8 +182,19 @@ scored_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
     // ---------------------------------- TMA ----------------------------------
     if (lane == 0) {
       int kst = 0, vst = 0;
-      uint32_t kph = 0, vph = 0, qn = 0;  // qn: units with anything to load
+      uint32_t kph = 0, vph = 0, qn = 0;  // qn: Q tiles loaded
       bool ok = true;
+      auto load = [&](const CUtensorMap* map, uint8_t* tile, uint64_t* bar, int row, int h, int b) {
+        mbar_arrive_expect_tx(bar, kTile);
+#pragma unroll
+        for (int a = 0; a < Cf::NATOM; ++a) tma_load_4d(tile + a * kAtom, map, a * Cf::AE, row, h, b, bar);
+      };
+      auto load_q = [&](int u) {
+        const uint32_t at = qn % kQ;
+        ok = ok && wait_abort(&q_empty[at], ((qn / kQ) & 1) ^ 1, p.err, 0xB2600002u, abort_flag);
+        if (ok) load(&tmQ, sQ + at * kTile, &q_full[at], un.q0 + u * BQ, un.h, un.b);
+        ++qn;
+      };
       for (int k = 0; ok && unit_of(p, k, un); ++k) {
         ok = wait_abort(&info_full[k & 1], (k >> 1) & 1, p.err, 0xB2600001u, abort_flag);
         if (!ok) break;
@@ -194,36 +203,20 @@ scored_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
         const int jb = f.first(), je = f.last();
         if (je == 0) continue;
         const int hk = un.h / (p.Hq / p.Hkv);
-        // Q has one buffer, free only when the unit before has all its S: have it
-        // in L2 by then
-        for (int u = 0; u < 2; ++u)
-          if (k > 0 && f.nkv[u] > 0)
-#pragma unroll
-            for (int a = 0; a < Cf::NATOM; ++a) prefetch_4d(&tmQ, a * Cf::AE, un.q0 + u * BQ, un.h, un.b);
-        ok = wait_abort(q_empty, (qn & 1) ^ 1, p.err, 0xB2600002u, abort_flag);
-        if (!ok) break;
-        ++qn;
-        mbar_arrive_expect_tx(q_full, ((f.nkv[0] > 0) + (f.nkv[1] > 0)) * kTile);
-        for (int u = 0; u < 2; ++u)
-          if (f.nkv[u] > 0)
-#pragma unroll
-            for (int a = 0; a < Cf::NATOM; ++a)
-              tma_load_4d(sQ + u * kTile + a * kAtom, &tmQ, a * Cf::AE, un.q0 + u * BQ, un.h, un.b, q_full);
-        for (int j = jb; j < je; ++j) {
+        // the unit's first Q tile has room while the unit before is still at
+        // work; its second one takes the place of that unit's first
+        const int u0 = f.nkv[0] > 0 ? 0 : 1;
+        load_q(u0);
+        for (int j = jb; j < je && ok; ++j) {
           ok = wait_abort(&k_empty[kst], kph ^ 1, p.err, 0xB2600003u, abort_flag);
           if (!ok) break;
-          mbar_arrive_expect_tx(&k_full[kst], kTile);
-#pragma unroll
-          for (int a = 0; a < Cf::NATOM; ++a)
-            tma_load_4d(sK + kst * kTile + a * kAtom, &tmK, a * Cf::AE, j * BKV, hk, un.b, &k_full[kst]);
-          ok = wait_abort(&v_empty[vst], vph ^ 1, p.err, 0xB2600004u, abort_flag);
+          load(&tmK, sK + kst * kTile, &k_full[kst], j * BKV, hk, un.b);
+          if (j == jb && u0 == 0 && f.nkv[1] > 0) load_q(1);
+          ok = ok && wait_abort(&v_empty[vst], vph ^ 1, p.err, 0xB2600004u, abort_flag);
           if (!ok) break;
-          mbar_arrive_expect_tx(&v_full[vst], kTile);
-#pragma unroll
-          for (int a = 0; a < Cf::NATOM; ++a)
-            tma_load_4d(sV + vst * kTile + a * kAtom, &tmV, a * Cf::AE, j * BKV, hk, un.b, &v_full[vst]);
-          if (++kst == kKStages) { kst = 0; kph ^= 1; }
-          if (++vst == kVStages) { vst = 0; vph ^= 1; }
+          load(&tmV, sV + vst * kTile, &v_full[vst], j * BKV, hk, un.b);
+          if (++kst == kK) { kst = 0; kph ^= 1; }
+          if (++vst == kV) { vst = 0; vph ^= 1; }
         }
       }
     }
@@ -235,14 +228,23 @@ scored_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
       int kst = 0, vst = 0;
       uint32_t kph = 0, vph = 0, qn = 0, pc[2] = {0, 0};
       bool ok = true;
-      auto issue_s = [&](int u) {
+      uint32_t q_at[2] = {0, 0};
+      auto issue_s = [&](int u, int j) {
+        if (j == f.kb[u]) {  // the unit's first S of this tile: is its Q there?
+          q_at[u] = qn % kQ;
+          ok = wait_abort(&q_full[q_at[u]], (qn / kQ) & 1, p.err, 0xB2600007u, abort_flag);
+          if (!ok) return;
+          ++qn;
+          tc::fence_after_sync();
+        }
 #pragma unroll
         for (int kk = 0; kk < HD / Cf::KSTEP; ++kk) {
-          const uint64_t da = tc::desc_kmajor_sw128(sQ + u * kTile + (kk >> 2) * kAtom + (kk & 3) * 32);
+          const uint64_t da = tc::desc_kmajor_sw128(sQ + q_at[u] * kTile + (kk >> 2) * kAtom + (kk & 3) * 32);
           const uint64_t db = tc::desc_kmajor_sw128(sK + kst * kTile + (kk >> 2) * kAtom + (kk & 3) * 32);
           mma_ss<FMT>(tmem + 256 * u, da, db, idS, kk != 0);
         }
         tc::commit(&s_full[u]);
+        if (j == f.nkv[u] - 1) tc::commit(&q_empty[q_at[u]]);
       };
       auto wait_k = [&]() {
         ok = ok && wait_abort(&k_full[kst], kph, p.err, 0xB2600005u, abort_flag);
@@ -251,7 +253,7 @@ scored_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
       };
       auto free_k = [&]() {
         tc::commit(&k_empty[kst]);
-        if (++kst == kKStages) { kst = 0; kph ^= 1; }
+        if (++kst == kK) { kst = 0; kph ^= 1; }
       };
       for (int k = 0; ok && unit_of(p, k, un); ++k) {
         ok = wait_abort(&info_full[k & 1], (k >> 1) & 1, p.err, 0xB2600006u, abort_flag);
@@ -260,17 +262,14 @@ scored_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
         mbar_arrive(&info_empty[k & 1]);
         const int jb = f.first(), je = f.last();
         if (je == 0) continue;
-        ok = wait_abort(q_full, qn & 1, p.err, 0xB2600007u, abort_flag);
-        if (!ok) break;
-        ++qn;
         // S of the first KV tile.  Its columns hold the last P of the unit before,
         // whose PV was issued earlier: MMAs of one thread run in order.
         if (!wait_k()) break;
-        for (int u = 0; u < 2; ++u)
-          if (f.active(u, jb)) issue_s(u);
+        for (int u = 0; u < 2 && ok; ++u)
+          if (f.active(u, jb)) issue_s(u, jb);
+        if (!ok) break;
         free_k();
         for (int j = jb; j < je && ok; ++j) {
-          if (j == je - 1) tc::commit(q_empty);  // every S of the unit is issued
           ok = wait_abort(&v_clean[vst], vph, p.err, 0xB2600008u, abort_flag);
           if (!ok) break;
           bool have_k = false;
@@ -290,12 +289,12 @@ scored_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
             if (f.active(u, j + 1)) {
               if (!have_k && !wait_k()) break;
               have_k = true;
-              issue_s(u);
+              issue_s(u, j + 1);
             }
           }
           if (!ok) break;
           tc::commit(&v_empty[vst]);
-          if (++vst == kVStages) { vst = 0; vph ^= 1; }
+          if (++vst == kV) { vst = 0; vph ^= 1; }
           if (have_k) free_k();
         }
       }
@@ -372,7 +371,7 @@ scored_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
           tc::fence_proxy_async_smem();
         }
         mbar_arrive(&v_clean[vst]);
-        if (++vst == kVStages) { vst = 0; vph ^= 1; }
+        if (++vst == kV) { vst = 0; vph ^= 1; }
       }
     }
   } else {
@@ -505,7 +504,7 @@ scored_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
 template <int HD, int FMT, bool CAP, bool BIAS>
 static void launch(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const Params& p,
                    cudaStream_t st) {
-  constexpr int smem = 7 * FaCfg<HD, FMT>::kTile + 1024 + 512;
+  constexpr int smem = (kQ + kK + kV) * FaCfg<HD, FMT>::kTile + 1024 + 512;
   const int64_t units = (int64_t)p.n_units * p.Hq * p.B;
   const int grid = (int)(units < num_sms() ? units : num_sms());
   set_max_smem((const void*)scored_kernel<HD, FMT, CAP, BIAS>, smem);
