@@ -229,8 +229,8 @@ scored_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
       uint32_t kph = 0, vph = 0, qn = 0, pc[2] = {0, 0};
       bool ok = true;
       uint32_t q_at[2] = {0, 0};
-      auto issue_s = [&](int u, int j) {
-        if (j == f.kb[u]) {  // the unit's first S of this tile: is its Q there?
+      auto issue_s = [&](int u, int j, const Info& g) {
+        if (j == g.kb[u]) {  // the unit's first S of this tile: is its Q there?
           q_at[u] = qn % kQ;
           ok = wait_abort(&q_full[q_at[u]], (qn / kQ) & 1, p.err, 0xB2600007u, abort_flag);
           if (!ok) return;
@@ -244,7 +244,7 @@ scored_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
           mma_ss<FMT>(tmem + 256 * u, da, db, idS, kk != 0);
         }
         tc::commit(&s_full[u]);
-        if (j == f.nkv[u] - 1) tc::commit(&q_empty[q_at[u]]);
+        if (j == g.nkv[u] - 1) tc::commit(&q_empty[q_at[u]]);
       };
       auto wait_k = [&]() {
         ok = ok && wait_abort(&k_full[kst], kph, p.err, 0xB2600005u, abort_flag);
@@ -255,22 +255,41 @@ scored_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
         tc::commit(&k_empty[kst]);
         if (++kst == kK) { kst = 0; kph ^= 1; }
       };
-      for (int k = 0; ok && unit_of(p, k, un); ++k) {
-        ok = wait_abort(&info_full[k & 1], (k >> 1) & 1, p.err, 0xB2600006u, abort_flag);
-        if (!ok) break;
-        read_info(k, f);
-        mbar_arrive(&info_empty[k & 1]);
-        const int jb = f.first(), je = f.last();
-        if (je == 0) continue;
-        // S of the first KV tile.  Its columns hold the last P of the unit before,
-        // whose PV was issued earlier: MMAs of one thread run in order.
-        if (!wait_k()) break;
+      int k = 0;
+      auto next_unit = [&](Info& g) {  // the next unit with anything to do
+        while (ok && unit_of(p, k, un)) {
+          ok = wait_abort(&info_full[k & 1], (k >> 1) & 1, p.err, 0xB2600006u, abort_flag);
+          if (!ok) break;
+          read_info(k, g);
+          mbar_arrive(&info_empty[k & 1]);
+          ++k;
+          if (g.last() > 0) return true;
+        }
+        return false;
+      };
+      // Order: PV_0(j) S_0(j + 1) PV_1(j) S_1(j + 1), where the tile after a
+      // unit's last is the next unit's first: one Q tile's softmax warps start on
+      // it while the other's are still at the diagonal.  S overwrites P of the
+      // tile before, whose PV was issued earlier: MMAs of one thread run in order.
+      bool have = next_unit(f);
+      if (have && wait_k()) {
         for (int u = 0; u < 2 && ok; ++u)
-          if (f.active(u, jb)) issue_s(u, jb);
-        if (!ok) break;
-        free_k();
-        for (int j = jb; j < je && ok; ++j) {
-          ok = wait_abort(&v_clean[vst], vph, p.err, 0xB2600008u, abort_flag);
+          if (f.active(u, f.first())) issue_s(u, f.first(), f);
+        if (ok) free_k();
+      }
+      while (ok && have) {
+        const int je = f.last();
+        Info nx;
+        bool more = true;
+        for (int j = f.first(); j < je && ok; ++j) {
+          int jn = j + 1;
+          Info g = f;
+          if (jn == je) {
+            more = next_unit(nx);
+            g = nx;
+            jn = more ? nx.first() : 0;
+          }
+          ok = ok && wait_abort(&v_clean[vst], vph, p.err, 0xB2600008u, abort_flag);
           if (!ok) break;
           bool have_k = false;
           for (int u = 0; u < 2 && ok; ++u) {
@@ -286,10 +305,10 @@ scored_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
                             (j != f.kb[u]) || kk != 0);
               if (j == f.nkv[u] - 1) tc::commit(&o_done[u]);
             }
-            if (f.active(u, j + 1)) {
+            if (more && g.active(u, jn)) {
               if (!have_k && !wait_k()) break;
               have_k = true;
-              issue_s(u, j + 1);
+              issue_s(u, jn, g);
             }
           }
           if (!ok) break;
@@ -297,6 +316,8 @@ scored_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
           if (++vst == kV) { vst = 0; vph ^= 1; }
           if (have_k) free_k();
         }
+        f = nx;
+        have = more;
       }
       if (!ok) {
         tc::commit(drain);
