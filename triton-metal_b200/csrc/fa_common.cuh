@@ -254,33 +254,25 @@ __device__ __forceinline__ uint64_t score_pair(uint32_t s0, uint32_t s1, int e, 
   return fma_f2(s, f2_pack(c.scale_log2, c.scale_log2), a);
 }
 
-// Scores of the N columns in sv, left in sv (cap and bias both: computed once).
-template <bool ABS, bool SMALL, int N>
+// Scores of the N columns in sv, left in sv (with a bias, which the maximum
+// needs too).
+template <bool ABS, bool CAP, bool SMALL, int N>
 __device__ __forceinline__ void score_chunk(uint32_t (&sv)[N], const Score& c) {
 #pragma unroll
   for (int e = 0; e < N; e += 2) {
-    const uint64_t x = score_pair<ABS, true, true, SMALL>(sv[e], sv[e + 1], e, c, 0.f);
+    const uint64_t x = score_pair<ABS, CAP, true, SMALL>(sv[e], sv[e + 1], e, c, 0.f);
     sv[e] = (uint32_t)x;
     sv[e + 1] = (uint32_t)(x >> 32);
   }
 }
 
-// Largest score (without a bias: largest raw score) of N columns; BITS: of those
-// with a bit in w (N = 32).
-template <bool BITS, bool CAP, bool BIAS, int N>
-__device__ __forceinline__ float max_chunk(uint32_t (&sv)[N], uint32_t w, const Score& c, float mx) {
-  if constexpr (CAP && BIAS) {
-    if (all_small(sv, c)) score_chunk<BITS, true>(sv, c);
-    else score_chunk<BITS, false>(sv, c);
-  }
+// Largest of N columns; BITS: of those with a bit in w (N = 32).
+template <bool BITS, int N>
+__device__ __forceinline__ float max_chunk(const uint32_t (&sv)[N], uint32_t w) {
+  float mx = -INFINITY;
 #pragma unroll
   for (int e = 0; e < N; e += 2) {
     float v0 = __uint_as_float(sv[e]), v1 = __uint_as_float(sv[e + 1]);
-    if constexpr (BIAS && !CAP) {
-      const uint64_t x = score_pair<BITS, CAP, BIAS, false>(sv[e], sv[e + 1], e, c, 0.f);
-      v0 = f2_lo(x);
-      v1 = f2_hi(x);
-    }
     if constexpr (BITS) {
       if (!(w >> e & 1)) v0 = -INFINITY;
       if (!(w >> (e + 1) & 1)) v1 = -INFINITY;
@@ -310,74 +302,20 @@ __device__ __forceinline__ bool whole_tile(const uint32_t (&vis)[4]) {
                                      (vis[0] | vis[1] | vis[2] | vis[3]) == 0);
 }
 
-// Largest score of the row's visible keys (bits of vis), -inf without one.
-// WIDE: with the way for whole tiles, taken where `whole` says so (whole_tile,
-// and with a bias all keys on one side); one_side: see score_pair.
-// Scale and cap keep the order, so without a bias the raw maximum is taken and
-// scored once.  With cap and bias both, the scores are left in the S columns
-// for score_exp.
-template <bool WIDE, bool CAP, bool BIAS>
-__device__ __forceinline__ float score_max(uint32_t tS, const uint32_t (&vis)[4], bool whole, bool one_side,
-                                           const Score& sc) {
-  float mx = -INFINITY;
-  if (WIDE && whole) {
-    if (!__any_sync(0xffffffffu, vis[0] != 0)) return -INFINITY;
-#pragma unroll 1
-    for (int c = 0; c < 4; c += 2) {
-      uint32_t sv[64];
-      tc::tmem_ld_32x32b_x32(tS + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(sv));
-      tc::tmem_ld_32x32b_x32(tS + 32 * c + 32, *reinterpret_cast<uint32_t(*)[32]>(sv + 32));
-      tc::tmem_ld_wait();
-      Score cc = sc;
-      cc.dist -= 32.f * c;
-      mx = max_chunk<false, CAP, BIAS>(sv, 0, cc, mx);
-      if constexpr (CAP && BIAS) {
-        tmem_st_32x32b_x32(tS + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(sv));
-        tmem_st_32x32b_x32(tS + 32 * c + 32, *reinterpret_cast<uint32_t(*)[32]>(sv + 32));
-      }
-    }
-    if (!vis[0]) mx = -INFINITY;
-  } else {
-#pragma unroll 1
-    for (int c = 0; c < 4; ++c) {
-      const uint32_t w = word_of(vis, c);
-      const Piece kind = piece_of(w, !BIAS || one_side);
-      if (kind == kNone) continue;
-      uint32_t sv[32];
-      tc::tmem_ld_32x32b_x32(tS + 32 * c, sv);
-      tc::tmem_ld_wait();
-      Score cc = sc;
-      cc.dist -= 32.f * c;
-      if (kind == kRows) {
-        const float m = max_chunk<false, CAP, BIAS>(sv, 0, cc, -INFINITY);
-        mx = fmaxf(mx, w ? m : -INFINITY);
-      } else {
-        mx = max_chunk<true, CAP, BIAS>(sv, w, cc, mx);
-      }
-      if constexpr (CAP && BIAS) tmem_st_32x32b_x32(tS + 32 * c, sv);
-    }
-  }
-  if constexpr (CAP && BIAS) tmem_st_wait();
-  if constexpr (!BIAS) {
-    if constexpr (CAP) mx = mx == -INFINITY ? mx : capped(mx, sc, 0.f);
-    else mx *= sc.scale_log2;
-  }
-  return mx;
-}
-
-// p = exp2(score - m) of N columns as 16-bit pairs; their sum goes to rs.
+// p = exp2(score - m) of N columns as 16-bit pairs; returns their sum.
 template <bool BITS, int FMT, bool CAP, bool BIAS, bool SMALL, int N>
-__device__ __forceinline__ void exp_chunk(const uint32_t (&sv)[N], uint32_t (&pk)[N / 2], uint64_t& rs, uint32_t w,
-                                          const Score& c, float mref) {
+__device__ __forceinline__ float exp_chunk(const uint32_t (&sv)[N], uint32_t (&pk)[N / 2], uint32_t w, const Score& c,
+                                           float mref) {
+  uint64_t rs = 0;
 #pragma unroll
   for (int e = 0; e < N / 2; ++e) {
     float p0, p1;
     uint64_t x;
-    if constexpr (CAP && BIAS) x = add_f2((uint64_t)sv[2 * e] | ((uint64_t)sv[2 * e + 1] << 32), f2_pack(-mref, -mref));
+    if constexpr (BIAS) x = add_f2((uint64_t)sv[2 * e] | ((uint64_t)sv[2 * e + 1] << 32), f2_pack(-mref, -mref));
     else x = score_pair<BITS, CAP, BIAS, SMALL>(sv[2 * e], sv[2 * e + 1], 2 * e, c, -mref);
     // part of the exponentials on the FMA pipe: a third, as in the prefill
     // kernel, but fewer beside the cap, which has filled it already
-    if (SMALL ? e % 8 == 7 : e % 3 == 2) {
+    if (CAP ? e % 8 == 7 : e % 3 == 2) {
       const uint64_t y = exp2_poly_f2(x);
       p0 = f2_lo(y);
       p1 = f2_hi(y);
@@ -398,72 +336,158 @@ __device__ __forceinline__ void exp_chunk(const uint32_t (&sv)[N], uint32_t (&pk
       pk[e] = *reinterpret_cast<uint32_t*>(&hv);
     }
   }
-}
-template <bool BITS, int FMT, bool CAP, bool BIAS, int N>
-__device__ __forceinline__ void exp_chunk_any(const uint32_t (&sv)[N], uint32_t (&pk)[N / 2], uint64_t& rs, uint32_t w,
-                                              const Score& c, float mref) {
-  if constexpr (CAP && !BIAS) {
-    if (all_small(sv, c)) {
-      exp_chunk<BITS, FMT, CAP, BIAS, true>(sv, pk, rs, w, c, mref);
-      return;
-    }
-  }
-  exp_chunk<BITS, FMT, CAP, BIAS, false>(sv, pk, rs, w, c, mref);
+  return f2_lo(rs) + f2_hi(rs);
 }
 
-// p = exp2(score - m) as 16-bit pairs over the S columns; returns their sum.
-// P rounded to 16 bits (half a step of its own size) is what the MMA takes; the
-// sum is taken before that, in 32 bits.
-template <bool WIDE, int FMT, bool CAP, bool BIAS>
-__device__ __forceinline__ float score_exp(uint32_t tS, const uint32_t (&vis)[4], bool whole, bool one_side, float mref,
-                                           const Score& sc) {
+__device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+
+template <int FMT>
+__device__ __forceinline__ float widen16(uint16_t h) {
+  if constexpr (FMT == kF16) return __half2float(__ushort_as_half(h));
+  else return __uint_as_float((uint32_t)h << 16);
+}
+template <int FMT>
+__device__ __forceinline__ uint32_t narrow2(float a, float b) {
+  if constexpr (FMT == kF16) {
+    __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<uint32_t*>(&h);
+  } else {
+    __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<uint32_t*>(&h);
+  }
+}
+
+// The running maximum has grown: O (HD columns, if there is one yet) and the P
+// that this tile has stored so far (`stored` keys) are brought to the new one.
+template <int HD, int FMT>
+__device__ __noinline__ void rescale(uint32_t tO, uint32_t tS, bool has_o, int stored, float alpha) {
+  if (has_o) {
+#pragma unroll 1
+    for (int c = 0; c < HD / 32; ++c) {
+      uint32_t o[32];
+      tc::tmem_ld_32x32b_x32(tO + 32 * c, o);
+      tc::tmem_ld_wait();
+#pragma unroll
+      for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+      tmem_st_32x32b_x32(tO + 32 * c, o);
+    }
+  }
+  if (stored) {
+    tmem_st_wait();
+#pragma unroll 1
+    for (int c = 0; c < stored / 32; ++c) {
+      uint32_t x[16];
+      tmem_ld_32x32b_x16(tS + 16 * c, x);
+      tc::tmem_ld_wait();
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        x[e] = narrow2<FMT>(widen16<FMT>((uint16_t)x[e]) * alpha, widen16<FMT>((uint16_t)(x[e] >> 16)) * alpha);
+      tmem_st_32x32b_x16(tS + 16 * c, x);
+    }
+  }
+}
+
+constexpr float kRescale = 8.f;  // log2 units: P holds up to 2^8
+
+// 2^d for a whole d <= 0 (-inf: 0)
+__device__ __forceinline__ float pow2_down(float d) {
+  return d < -126.f ? 0.f : __int_as_float((int)(d + 127.f) << 23);
+}
+
+// One chunk of a tile (N = 64 or 32 keys from key `at` on): its maximum, the
+// rescaling if that has grown by more than kRescale, and its P over the S
+// columns.  w: BITS, a bit per key; else all ones or zero, the row sees the
+// chunk or not.
+template <bool BITS, int HD, int FMT, bool CAP, bool BIAS, int N>
+__device__ __forceinline__ void softmax_chunk(uint32_t (&sv)[N], uint32_t tS, uint32_t tO, int at, uint32_t w,
+                                              const Score& sc, bool has_o, float& m, float& l) {
+  Score cc = sc;
+  cc.dist -= (float)at;
+  bool small = false;
+  if constexpr (CAP) small = all_small(sv, sc);
+  if constexpr (BIAS) {
+    if (CAP && small) score_chunk<BITS, CAP, CAP>(sv, cc);
+    else score_chunk<BITS, CAP, false>(sv, cc);
+  }
+  float mx = max_chunk<BITS>(sv, w);
+  if constexpr (!BIAS) {  // scale and cap keep the order
+    if constexpr (CAP) mx = mx == -INFINITY ? mx : capped(mx, sc, 0.f);
+    else mx *= sc.scale_log2;
+  }
+  if (!BITS && !w) mx = -INFINITY;
+  const bool need = mx > m + kRescale;
+  if (__any_sync(0xffffffffu, need)) {
+    // the first maximum as it is (a row's only key has weight 1), then whole steps
+    // up from it: what is stored as P already is rescaled exactly, and no weight
+    // is rounded twice
+    const float up = ceilf(mx - m);
+    const float alpha = need ? pow2_down(-up) : 1.f;
+    if (need) {
+      l *= alpha;
+      m = m == -INFINITY ? mx : m + up;
+    }
+    if (has_o || at) rescale<HD, FMT>(tO, tS, has_o, at, alpha);
+  }
+  const float mref = m == -INFINITY ? 0.f : m;
+  uint32_t pk[N / 2];
+  float rs;
+  if (CAP && !BIAS && small) rs = exp_chunk<BITS, FMT, CAP, BIAS, CAP && !BIAS>(sv, pk, w, cc, mref);
+  else rs = exp_chunk<BITS, FMT, CAP, BIAS, false>(sv, pk, w, cc, mref);
+  if constexpr (!BITS) {
+#pragma unroll
+    for (int e = 0; e < N / 2; ++e) pk[e] &= w;
+    if (!w) rs = 0.f;
+  }
+  l += rs;
+  if constexpr (N == 64) tmem_st_32x32b_x32(tS + at / 2, pk);
+  else tmem_st_32x32b_x16(tS + at / 2, pk);
+}
+
+// The softmax of one tile in a single pass over S: P = exp2(score - m) as 16-bit
+// pairs over the S columns, m and l brought up to date, O (has_o: there is one)
+// rescaled where the maximum has grown by more than kRescale.  P rounded to 16
+// bits (half a step of its own size) is what the MMA takes; the sum l is taken
+// before that, in 32 bits.
+// vis: a bit per key.  WIDE: with the way for whole tiles, taken where `whole`
+// says so (whole_tile, and with a bias all keys on one side); one_side: see
+// score_pair.
+template <bool WIDE, int HD, int FMT, bool CAP, bool BIAS>
+__device__ __forceinline__ void softmax_tile(uint32_t tS, uint32_t tO, const uint32_t (&vis)[4], bool whole,
+                                             bool one_side, const Score& sc, bool has_o, float& m, float& l) {
   if (WIDE && whole) {
-    uint64_t rs = 0;
 #pragma unroll 1
     for (int c = 0; c < 4; c += 2) {
       uint32_t sv[64];
       tc::tmem_ld_32x32b_x32(tS + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(sv));
       tc::tmem_ld_32x32b_x32(tS + 32 * c + 32, *reinterpret_cast<uint32_t(*)[32]>(sv + 32));
       tc::tmem_ld_wait();
-      Score cc = sc;
-      cc.dist -= 32.f * c;
-      uint32_t pk[32];
-      exp_chunk_any<false, FMT, CAP, BIAS>(sv, pk, rs, 0, cc, mref);
-#pragma unroll
-      for (int e = 0; e < 32; ++e) pk[e] &= vis[0];  // all or nothing
-      tmem_st_32x32b_x32(tS + 16 * c, pk);
+      softmax_chunk<false, HD, FMT, CAP, BIAS>(sv, tS, tO, 32 * c, vis[0], sc, has_o, m, l);
     }
-    return vis[0] ? f2_lo(rs) + f2_hi(rs) : 0.f;
+    return;
   }
-  float sum = 0.f;
 #pragma unroll 1
   for (int c = 0; c < 4; ++c) {
     const uint32_t w = word_of(vis, c);
     const Piece kind = piece_of(w, !BIAS || one_side);
-    uint32_t pk[16];
     if (kind == kNone) {
+      uint32_t zero[16];
 #pragma unroll
-      for (int e = 0; e < 16; ++e) pk[e] = 0;
-    } else {
-      uint32_t sv[32];
-      tc::tmem_ld_32x32b_x32(tS + 32 * c, sv);
-      tc::tmem_ld_wait();
-      Score cc = sc;
-      cc.dist -= 32.f * c;
-      uint64_t rs = 0;
-      if (kind == kRows) {
-        exp_chunk_any<false, FMT, CAP, BIAS>(sv, pk, rs, 0, cc, mref);
-#pragma unroll
-        for (int e = 0; e < 16; ++e) pk[e] &= w;  // all or nothing
-        sum += w ? f2_lo(rs) + f2_hi(rs) : 0.f;
-      } else {
-        exp_chunk_any<true, FMT, CAP, BIAS>(sv, pk, rs, w, cc, mref);
-        sum += f2_lo(rs) + f2_hi(rs);
-      }
+      for (int e = 0; e < 16; ++e) zero[e] = 0;
+      tmem_st_32x32b_x16(tS + 16 * c, zero);
+      continue;
     }
-    tmem_st_32x32b_x16(tS + 16 * c, pk);
+    uint32_t sv[32];
+    tc::tmem_ld_32x32b_x32(tS + 32 * c, sv);
+    tc::tmem_ld_wait();
+    if (kind == kRows) softmax_chunk<false, HD, FMT, CAP, BIAS>(sv, tS, tO, 32 * c, w, sc, has_o, m, l);
+    else softmax_chunk<true, HD, FMT, CAP, BIAS>(sv, tS, tO, 32 * c, w, sc, has_o, m, l);
   }
-  return sum;
 }
 
 template <int FMT>
@@ -483,22 +507,6 @@ __device__ __forceinline__ bool zero_not_finite(uint4& x) {
   }
   return hit;
 }
-template <int FMT>
-__device__ __forceinline__ float widen16(uint16_t h) {
-  if constexpr (FMT == kF16) return __half2float(__ushort_as_half(h));
-  else return __uint_as_float((uint32_t)h << 16);
-}
-template <int FMT>
-__device__ __forceinline__ uint32_t narrow2(float a, float b) {
-  if constexpr (FMT == kF16) {
-    __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<uint32_t*>(&h);
-  } else {
-    __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<uint32_t*>(&h);
-  }
-}
-
 // 4-D tensor map coordinates: (d, s, h, b)
 __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, int d, int s, int h, int b,
                                             uint64_t* bar) {

@@ -30,16 +30,12 @@ using namespace fa;
 // where the plain kernel has two and three).
 //   warp 0      TMA
 //   warp 1      TMEM owner, MMA issuer
-//   warps 2-3   key ranges of the next unit (which KV tiles its Q tiles visit,
-//               which of them are masked), and V: a tile in which some row must
-//               not see some key has its infinities and NaN zeroed, since a
-//               weight of 0 would make NaN of them; rows that do see such a
-//               value get it added at the end
+//   warps 2-3   key ranges of the next unit: which KV tiles its Q tiles visit,
+//               which of them are masked
 //   warps 4-11  two softmax warpgroups, one per Q tile, one row per thread
 // ---------------------------------------------------------------------------
 constexpr int kThreads = 384;
 constexpr int kQ = 3, kK = 2, kV = 2;  // tiles of each ring
-constexpr float kRescale = 8.f;  // log2 units
 
 struct Params {
   int B, Hq, Hkv, Sq, Skv, q_tiles;
@@ -50,8 +46,8 @@ struct Params {
   const float* slopes;     // [Hq]
   void* o;
   int64_t os_b, os_h, os_s;
-  const uint16_t* v;       // V again, for values that are not finite
-  int64_t vs_b, vs_h, vs_s;
+  const uint16_t *q, *k, *v;  // for rows that are done again
+  int64_t qs[3], ks[3], vs[3];
   unsigned* err;
 };
 
@@ -95,6 +91,37 @@ __device__ __forceinline__ void range_bits(uint32_t (&vis)[4], int lo, int hi, i
   }
 }
 
+// 32 columns (from `col` on) of a row, key by key, for an output that is not finite: the
+// tiles' PV takes every key of a tile, and a hidden one's infinity or NaN times
+// its weight of 0 is NaN.  Slow (no tile, no tensor core) and rarely needed.
+struct Row {
+  const uint16_t *q, *k, *v;
+  int64_t ks, vs;
+  int lo, hi, pos;
+};
+template <int HD, int FMT, bool CAP, bool BIAS>
+__device__ __noinline__ void again(float (&o)[32], const Row& r, int col, float m, const Score& sc) {
+#pragma unroll
+  for (int e = 0; e < 32; ++e) o[e] = 0.f;
+  for (int key = r.lo; key < r.hi; ++key) {
+    const uint16_t *k = r.k + key * r.ks, *v = r.v + key * r.vs + col;
+    float s = 0.f;
+    for (int d = 0; d < HD; d += 8) {
+      const uint4 a = *reinterpret_cast<const uint4*>(r.q + d), b = *reinterpret_cast<const uint4*>(k + d);
+      const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s = fmaf(widen16<FMT>((uint16_t)x[e]), widen16<FMT>((uint16_t)y[e]), s);
+        s = fmaf(widen16<FMT>((uint16_t)(x[e] >> 16)), widen16<FMT>((uint16_t)(y[e] >> 16)), s);
+      }
+    }
+    float t = -m;
+    if constexpr (BIAS) t = fmaf(-sc.slope, fabsf((float)(r.pos - key)), t);
+    const float w = ex2(CAP ? capped(s, sc, t) : fmaf(s, sc.scale_log2, t));
+    for (int e = 0; e < 32; ++e) o[e] = fmaf(w, widen16<FMT>(v[e]), o[e]);
+  }
+}
+
 template <int HD, int FMT, bool CAP, bool BIAS>
 __global__ void __launch_bounds__(kThreads, 1)
 scored_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
@@ -111,8 +138,7 @@ scored_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
   uint64_t* k_full = q_empty + kQ;
   uint64_t* k_empty = k_full + kK;
   uint64_t* v_full = k_empty + kK;
-  uint64_t* v_clean = v_full + kV;
-  uint64_t* v_empty = v_clean + kV;
+  uint64_t* v_empty = v_full + kV;
   uint64_t* s_full = v_empty + kV;            // [2] per Q tile
   uint64_t* p_ready = s_full + 2;             // [2]
   uint64_t* o_done = p_ready + 2;             // [2]
@@ -121,9 +147,8 @@ scored_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
   uint64_t* drain = info_empty + 2;
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
-  volatile int* s_bad = reinterpret_cast<volatile int*>(tmem_holder + 2);      // [4]: unit with a bad V value
   int4* s_info = reinterpret_cast<int4*>(q_full + 32);                         // [2 parities][2 warps][2 tiles]
-  static_assert(2 * kQ + 2 * kK + 3 * kV + 11 + 3 <= 32, "barriers");
+  static_assert(2 * kQ + 2 * kK + 2 * kV + 11 + 1 <= 32, "barriers");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -137,7 +162,6 @@ scored_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
     }
     for (int i = 0; i < kV; ++i) {
       mbar_init(&v_full[i], 1);
-      mbar_init(&v_clean[i], 64);
       mbar_init(&v_empty[i], 1);
     }
     for (int u = 0; u < 2; ++u) {
@@ -147,7 +171,6 @@ scored_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
       mbar_init(&info_full[u], 64);
       mbar_init(&info_empty[u], 10);  // TMA, MMA, 8 softmax warps
     }
-    for (int i = 0; i < 4; ++i) s_bad[i] = -1;
     mbar_init(drain, 1);
     *abort_flag = 0;
     fence_mbar_init();
@@ -289,7 +312,7 @@ scored_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
             g = nx;
             jn = more ? nx.first() : 0;
           }
-          ok = ok && wait_abort(&v_clean[vst], vph, p.err, 0xB2600008u, abort_flag);
+          ok = ok && wait_abort(&v_full[vst], vph, p.err, 0xB2600008u, abort_flag);
           if (!ok) break;
           bool have_k = false;
           for (int u = 0; u < 2 && ok; ++u) {
@@ -325,11 +348,9 @@ scored_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
       }
     }
   } else if (warp < 4) {
-    // ------------------------- key ranges, V of masked tiles -------------------------
+    // ------------------------------- key ranges -------------------------------
     const int t = threadIdx.x - 64;
-    auto find = [&](int k) {  // info of turn k; true when there is such a turn
-      Unit n;
-      if (!unit_of(p, k, n)) return true;
+    auto find = [&](int k) {  // info of turn k
       if (k >= 2 && !__all_sync(0xffffffffu, wait_abort(&info_empty[k & 1], ((k >> 1) - 1) & 1, p.err, 0xB260000Bu, abort_flag)))
         return false;
 #pragma unroll
@@ -339,10 +360,10 @@ scored_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
         int4 x = make_int4(INT_MAX, 0, 0, INT_MAX);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const int row = n.q0 + u * BQ + i * 64 + t;
+          const int row = un.q0 + u * BQ + i * 64 + t;
           if (u < p.per && row < p.Sq) {
             int lo, hi;
-            attn::row_range(p.range, n.b, row, p.Skv, lo, hi);
+            attn::row_range(p.range, un.b, row, p.Skv, lo, hi);
             const bool sees = hi > lo;
             if (sees) x.x = min(x.x, lo);
             x.y = sees ? max(x.y, lo) : INT_MAX;
@@ -360,40 +381,7 @@ scored_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
       mbar_arrive(&info_full[k & 1]);
       return true;
     };
-    int vst = 0;
-    uint32_t vph = 0;
-    bool ok = find(0);
-    for (int k = 0; ok && unit_of(p, k, un); ++k) {
-      // before the next info may replace this one's neighbour: the other warp's half
-      ok = __all_sync(0xffffffffu, wait_abort(&info_full[k & 1], (k >> 1) & 1, p.err, 0xB260000Cu, abort_flag));
-      if (!ok) break;
-      read_info(k, f);
-      ok = find(k + 1);
-      const int jb = f.first(), je = f.last();
-      for (int j = jb; j < je && ok; ++j) {
-        // every tile passes through here, so that these warps are never a ring
-        // turn behind a stage (a parity wait cannot tell that)
-        ok = __all_sync(0xffffffffu, wait_abort(&v_full[vst], vph, p.err, 0xB260000Du, abort_flag));
-        if (!ok) break;
-        if ((f.active(0, j) && f.masked(0, j)) || (f.active(1, j) && f.masked(1, j))) {
-          uint4* tile = reinterpret_cast<uint4*>(sV + vst * kTile);
-          bool bad = false;
-#pragma unroll 8
-          for (int i = t; i < kTile / 16; i += 64) {
-            uint4 x = tile[i];
-            if (zero_not_finite<FMT>(x)) {
-              tile[i] = x;
-              bad = true;
-            }
-          }
-          // four turns of flags: warps 4-11 have left turn k - 4 when info k + 1
-          // could be made
-          if (bad) s_bad[k & 3] = k;
-          tc::fence_proxy_async_smem();
-        }
-        mbar_arrive(&v_clean[vst]);
-        if (++vst == kV) { vst = 0; vph ^= 1; }
-      }
+    for (int k = 0; unit_of(p, k, un) && find(k); ++k) {
     }
   } else {
     // -------------------------------- softmax --------------------------------
@@ -423,6 +411,7 @@ scored_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
       __syncwarp();
       if (lane == 0) mbar_arrive(&info_empty[k & 1]);
       const int kb = f.kb[u], nkv = f.nkv[u];
+      const bool any_masked = nkv > kb && (f.masked(u, kb) || f.masked(u, nkv - 1));  // ranges end in a tile's span
       float m_used = -INFINITY, l = 0.f;
       for (int j = kb; j < nkv; ++j) {
         ok = __all_sync(0xffffffffu, wait_abort(&s_full[u], sc & 1, p.err, 0xB260000Fu, abort_flag));
@@ -438,27 +427,8 @@ scored_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
         uint32_t vis[4] = {~0u, ~0u, ~0u, ~0u};
         if (f.masked(u, j)) range_bits(vis, row_lo, row_hi, kv0);
         const bool whole = (!BIAS || one_side) && whole_tile(vis);
-        const float mx = score_max<true, CAP, BIAS>(tS, vis, whole, one_side, score);
-        // lazy, warp-uniform rescale of O (O_u is quiescent: PV_u(j-1) finished)
-        const bool need = mx > m_used + kRescale;
-        const float alpha = need ? ((m_used == -INFINITY) ? 0.f : ex2(m_used - mx)) : 1.f;
-        if (need) {
-          l *= alpha;
-          m_used = mx;
-        }
-        if (__any_sync(0xffffffffu, need) && j > kb) {
-#pragma unroll 1
-          for (int c = 0; c < HD / 32; ++c) {
-            uint32_t o[32];
-            tc::tmem_ld_32x32b_x32(tO + 32 * c, o);
-            tc::tmem_ld_wait();
-#pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-            tmem_st_32x32b_x32(tO + 32 * c, o);
-          }
-        }
-        const float mref = (m_used == -INFINITY) ? 0.f : m_used;
-        l += score_exp<true, FMT, CAP, BIAS>(tS, vis, whole, one_side, mref, score);
+        // O_u is quiescent: PV_u(j-1) finished before S_u(j)
+        softmax_tile<true, HD, FMT, CAP, BIAS>(tS, tO, vis, whole, one_side, score, j > kb, m_used, l);
         tmem_st_wait();
         tc::fence_before_sync();
         __syncwarp();
@@ -478,21 +448,26 @@ scored_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
       ++oc;
       tc::fence_after_sync();
       const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-      const bool bad = s_bad[k & 3] == k;
       const int hk = un.h / (p.Hq / p.Hkv);
 #pragma unroll 1
       for (int c = 0; c < HD / 32; ++c) {
         float o[32];
         tc::tmem_ld_32x32b_x32(tO + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(o));
         tc::tmem_ld_wait();
-        if (bad) {
-          for (int key = row_lo; key < row_hi; ++key) {
-            const uint16_t* v = p.v + un.b * p.vs_b + hk * p.vs_h + (int64_t)key * p.vs_s + 32 * c;
+        if (any_masked) {
+          // 0 x infinity: V of a hidden key may have made NaN of the row
+          float sum = 0.f;
 #pragma unroll
-            for (int e = 0; e < 32; ++e) {
-              const uint16_t x = v[e];
-              if (not_finite16<FMT>(x)) o[e] += widen16<FMT>(x);
-            }
+          for (int e = 0; e < 32; ++e) sum = fmaf(o[e], 0.f, sum);
+          if (sum != 0.f && l != 0.f && exists) {
+            const Row rw = {p.q + un.b * p.qs[0] + un.h * p.qs[1] + (int64_t)qpos * p.qs[2],
+                            p.k + un.b * p.ks[0] + hk * p.ks[1], p.v + un.b * p.vs[0] + hk * p.vs[1], p.ks[2], p.vs[2],
+                            row_lo, row_hi, qpos};
+            score.slope = slope;
+            float t[32];  // not o itself: that would have to live in local memory
+            again<HD, FMT, CAP, BIAS>(t, rw, 32 * c, m_used, score);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = t[e];
           }
         }
         if (l == 0.f) {
@@ -575,10 +550,11 @@ extern "C" int b2_flash_attn_fwd_scored(const void* q, const void* k, const void
   bool wide = aligned(q, 16) && aligned(k, 16) && aligned(v, 16) && aligned(o, 16);
   for (int i = 0; i < 3; ++i) wide = wide && qs[i] % 8 == 0 && ks[i] % 8 == 0 && vs[i] % 8 == 0 && os[i] % 8 == 0;
   // scale > 0: the row maximum is taken before the scale.  fp32 stays fp32 here
-  // (the plain kernel reads it as tf32 at head dim 64).
+  // (the plain kernel reads it as tf32 at head dim 64).  Up to 2^20 keys a row
+  // that is done again takes about a second, well inside the others' waits.
   unsigned* err = device_error_word();
   if (wide && (D == 64 || D == 128) && dtype != B2_F32 && scale > 0.f && Skv > 0 && err &&
-      B * Hq * ((Sq + fa::BQ - 1) / fa::BQ) <= (1 << 30)) {
+      B * Hq * ((Sq + fa::BQ - 1) / fa::BQ) <= (1 << 30) && Skv <= (1 << 20)) {
     CUtensorMap tq, tk, tv;
     if (make_tmap_4d(&tq, q, dtype, D, Sq, Hq, B, qs) && make_tmap_4d(&tk, k, dtype, D, Skv, Hkv, B, ks) &&
         make_tmap_4d(&tv, v, dtype, D, Skv, Hkv, B, vs)) {
@@ -601,10 +577,14 @@ extern "C" int b2_flash_attn_fwd_scored(const void* q, const void* k, const void
       p.range = range;
       p.slopes = alibi_slopes;
       p.cap = fa::make_cap(scale, softcap);
+      p.q = (const uint16_t*)q;
+      p.k = (const uint16_t*)k;
       p.v = (const uint16_t*)v;
-      p.vs_b = vs[0];
-      p.vs_h = vs[1];
-      p.vs_s = vs[2];
+      for (int i = 0; i < 3; ++i) {
+        p.qs[i] = qs[i];
+        p.ks[i] = ks[i];
+        p.vs[i] = vs[i];
+      }
 #define B2_SCORED(HD, FMT)                                                                             \
   do {                                                                                                 \
     if (softcap > 0.f && alibi_slopes) scored::launch<HD, FMT, true, true>(tq, tk, tv, p, st);         \

@@ -38,7 +38,6 @@ using namespace fa;
 
 constexpr int kThreads = 416;
 constexpr int BR = 128, BK = 128;          // rows and keys of a tile
-constexpr float kRescale = 8.f;            // log2 units: P holds up to 2^8
 constexpr int kItemCost = 2;               // what starting and ending an item costs, in tiles
 
 template <int HD>
@@ -610,27 +609,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const Params p) {
           // SINGLE has no way of its own for whole tiles: half the code is half the
           // instruction fetches, which is what a short call waits for
           const bool whole = PAIR && whole_tile(vis);
-          const float mx = score_max<PAIR, CAP, false>(tS, vis, whole, true, score);
-          const bool need = mx > m_used + kRescale;
-          const float alpha = need ? (m_used == -INFINITY ? 0.f : ex2(m_used - mx)) : 1.f;
-          if (need) {
-            l *= alpha;
-            m_used = mx;
-          }
-          if (__any_sync(0xffffffffu, need) && !first) {
-            const uint32_t mine = tO + 256 * u;
-#pragma unroll 1
-            for (int c = 0; c < HD / 32; ++c) {
-              uint32_t o[32];
-              tc::tmem_ld_32x32b_x32(mine + 32 * c, o);
-              tc::tmem_ld_wait();
-#pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-              tmem_st_32x32b_x32(mine + 32 * c, o);
-            }
-          }
-          const float mref = m_used == -INFINITY ? 0.f : m_used;
-          l += score_exp<PAIR, FMT, CAP, false>(tS, vis, whole, true, mref, score);
+          softmax_tile<PAIR, HD, FMT, CAP, false>(tS, tO + 256 * u, vis, whole, true, score, !first, m_used, l);
           tmem_st_wait();
         }
         first = false;
