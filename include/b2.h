@@ -234,7 +234,11 @@ B2_API int b2_decode_attn(const void* q, const void* k, const void* v, void* o,
  * tanh(s / softcap); alibi_slopes fp32 [Hq] or NULL: s -= slope[h] |q_pos -
  * key|.  n_pages: pages of a paged cache; a page number outside [0, n_pages)
  * reads as zeros and is recorded in the device error word.
+ *   workspace: b2_decode_attn_scored_workspace_size(...) bytes, 16-byte aligned,
+ *   when softcap or alibi_slopes is given (else b2_decode_attn_workspace_size).
  */
+B2_API size_t b2_decode_attn_scored_workspace_size(int64_t B, int64_t Hq, int64_t Hkv,
+                                                   int64_t D, int64_t max_seq_len);
 B2_API int b2_decode_attn_scored(const void* q, const void* k, const void* v, void* o,
                                  const int32_t* page_table, const int32_t* seq_lens,
                                  void* workspace, int64_t B, int64_t Hq, int64_t Hkv,

@@ -37,6 +37,7 @@ SIGNATURES = {
                                         _pi64, _f32, _i64, _i32, _vp]),
     "b2_flash_attn_fwd_scored": (_i32, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _pi64, _pi64, _pi64,
                                         _pi64, _f32, _i32, _i64, _f32, _vp, _vp, _i64, _vp, _i32, _vp]),
+    "b2_decode_attn_scored_workspace_size": (ctypes.c_size_t, [_i64, _i64, _i64, _i64, _i64]),
     "b2_decode_attn_scored": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
                                      _i64, _pi64, _pi64, _vp, _i64, _vp, _f32, _f32, _vp, _i32, _i32, _vp]),
     "b2_decode_attn_workspace_size": (ctypes.c_size_t, [_i64, _i64, _i64, _i64, _i64]),

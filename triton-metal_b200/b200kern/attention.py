@@ -218,8 +218,9 @@ def decode_attention(q, k_cache, v_cache, seq_lens, scale=None, page_table=None,
     q = q.contiguous()
     o = (_lib.check_out(out, (B, Hq, D), q.dtype, "decode_attention") if out is not None
          else torch.empty(B, Hq, D, dtype=q.dtype, device=q.device))
-    lib = _lib.load()
-    need = int(lib.b2_decode_attn_workspace_size(B, Hq, Hkv, D, S))
+    scored = softcap or alibi_slopes is not None
+    need = int(_lib.fn("b2_decode_attn_scored_workspace_size" if scored else "b2_decode_attn_workspace_size")(
+        B, Hq, Hkv, D, S))
     ws = torch.empty(max(need, 1), dtype=torch.uint8, device=q.device)
     qp = None if q_pos is None else _seq_lens(q_pos, B, q.device)
     fr = None

@@ -31,6 +31,14 @@
 #include <type_traits>
 
 namespace b2 {
+namespace tree {  // decode_scored_sm100.cu, tree_attn_sm100.cu
+int launch_decode(const void* q, const void* k, const void* v, void* o, const int32_t* page_table,
+                  const int32_t* seq_lens, void* workspace, int64_t B, int64_t Hq, int64_t Hkv, int64_t D,
+                  int64_t max_keys, int64_t page_size, int64_t max_pages, int64_t n_pages, const int64_t* k_strides,
+                  const int64_t* v_strides, float scale, float softcap, const float* slopes, int dtype,
+                  cudaStream_t st);
+size_t workspace(int64_t T, int64_t rep, int64_t D);
+}  // namespace tree
 namespace dec {
 
 constexpr int kThreads = 128;
@@ -755,6 +763,15 @@ extern "C" int b2_decode_attn(const void* q, const void* k, const void* v, void*
                      stream);
 }
 
+// The plain kernel's partials, or the two partials a CTA of the tree kernel.
+extern "C" size_t b2_decode_attn_scored_workspace_size(int64_t B, int64_t Hq, int64_t Hkv, int64_t D,
+                                                       int64_t max_seq_len) {
+  const size_t plain = b2_decode_attn_workspace_size(B, Hq, Hkv, D, max_seq_len);
+  if (B <= 0 || Hq <= 0 || Hkv <= 0 || (D != 64 && D != 128)) return plain;
+  const size_t tc = tree::workspace(1, Hq / Hkv, D);
+  return tc > plain ? tc : plain;
+}
+
 extern "C" int b2_decode_attn_scored(const void* q, const void* k, const void* v, void* o, const int32_t* page_table,
                                      const int32_t* seq_lens, void* workspace, int64_t B, int64_t Hq, int64_t Hkv,
                                      int64_t D, int64_t max_seq_len, int64_t page_size, int64_t max_pages,
@@ -765,6 +782,14 @@ extern "C" int b2_decode_attn_scored(const void* q, const void* k, const void* v
   B2_CHECK_ARG(softcap >= 0.f && isfinite(softcap), B2_ERR_INVALID,
                "decode_attn_scored: softcap must be finite and >= 0");
   B2_CHECK_ARG(n_pages >= 0, B2_ERR_INVALID, "decode_attn_scored: bad shape");
+  if ((softcap > 0.f || alibi_slopes) && q_dtype == kv_dtype && !q_pos && window <= 0 && !rope_freqs && q && k && v && o &&
+      seq_lens && k_strides && v_strides && B > 0 && Hq > 0 && Hkv > 0 && Hq % Hkv == 0 &&
+      (page_size == 0 || (page_table && page_size > 0 && max_pages > 0 && max_seq_len <= page_size * max_pages))) {
+    const int st = tree::launch_decode(q, k, v, o, page_size ? page_table : nullptr, seq_lens, workspace, B, Hq, Hkv, D,
+                                       max_seq_len, page_size, max_pages, n_pages, k_strides, v_strides, scale, softcap,
+                                       alibi_slopes, q_dtype, (cudaStream_t)stream);
+    if (st != B2_ERR_UNSUPPORTED) return st;
+  }
   return decode_impl(q, k, v, o, page_table, seq_lens, workspace, B, Hq, Hkv, D, max_seq_len, page_size, max_pages,
                      n_pages, k_strides, v_strides, q_pos, window, rope_freqs, scale, softcap, alibi_slopes, q_dtype,
                      kv_dtype, stream);

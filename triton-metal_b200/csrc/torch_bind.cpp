@@ -215,7 +215,9 @@ py::object decode_attention(const at::Tensor& q, const at::Tensor& k, const at::
     return py::none();
   at::Tensor o;
   if (!output(out, q, q.sizes(), o)) return py::none();
-  const size_t need = b2_decode_attn_workspace_size(B, Hq, c.Hkv, D, c.keys);
+  const size_t need = softcap > 0 || slopes.has_value()
+                          ? b2_decode_attn_scored_workspace_size(B, Hq, c.Hkv, D, c.keys)
+                          : b2_decode_attn_workspace_size(B, Hq, c.Hkv, D, c.keys);
   at::Tensor ws = at::empty({(int64_t)(need ? need : 1)}, q.options().dtype(at::kByte));
   const int rc = b2_decode_attn_scored(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
                                        (const int32_t*)ptr(table), lens.data_ptr<int>(), ws.data_ptr(), B, Hq, c.Hkv, D,

@@ -1,0 +1,26 @@
+// Attention of a tree of drafted tokens: the cp.async form, for page sizes that
+// are no multiple of 8.
+#include "tree_attn_kernel.cuh"
+
+namespace b2 {
+namespace tree {
+
+void launch_tree_cp(const Params& p, int D, bool f16, bool pair, cudaStream_t st) {
+  const Maps none = {};
+  const bool cap = p.softcap.log2 > 0.f;
+#define B2_TREE(HD, FMT)                                                                       \
+  do {                                                                                         \
+    if (pair && cap) launch<HD, FMT, true, true, false, false>(none, p, st);                   \
+    else if (pair) launch<HD, FMT, true, false, false, false>(none, p, st);                    \
+    else if (cap) launch<HD, FMT, false, true, false, false>(none, p, st);                     \
+    else launch<HD, FMT, false, false, false, false>(none, p, st);                             \
+  } while (0)
+  if (D == 128 && f16) B2_TREE(128, fa::kF16);
+  else if (D == 128) B2_TREE(128, fa::kBF16);
+  else if (f16) B2_TREE(64, fa::kF16);
+  else B2_TREE(64, fa::kBF16);
+#undef B2_TREE
+}
+
+}  // namespace tree
+}  // namespace b2
