@@ -52,7 +52,11 @@ int launch_decode(const void* q, const void* k, const void* v, void* o, const in
   t.box = box_of(page_size, n_pages);
   const bool f16 = dtype == B2_F16, cap = softcap > 0.f;
   Maps m;
-  if (!t.err || !t.box || !make_maps(m, t, D, Hq, f16)) return B2_ERR_UNSUPPORTED;
+  if (!t.err) return B2_ERR_UNSUPPORTED;
+  if (!t.box || !make_maps(m, t, D, Hq, f16)) {
+    launch_tree_cp(t, (int)D, f16, false, st);
+    return launch_status("decode_attn_scored");
+  }
 #define B2_DECODE(HD, FMT)                                                                   \
   do {                                                                                       \
     if (cap && slopes) launch<HD, FMT, false, true, true, true>(m, t, st);                   \

@@ -364,9 +364,10 @@ __device__ __forceinline__ uint32_t narrow2(float a, float b) {
 }
 
 // The running maximum has grown: O (HD columns, if there is one yet) and the P
-// that this tile has stored so far (`stored` keys) are brought to the new one.
+// of the keys [from, to), which this tile has stored already, are brought to the
+// new one.
 template <int HD, int FMT>
-__device__ __noinline__ void rescale(uint32_t tO, uint32_t tS, bool has_o, int stored, float alpha) {
+__device__ __forceinline__ void rescale(uint32_t tO, uint32_t tP, bool has_o, int from, int to, float alpha) {
   if (has_o) {
 #pragma unroll 1
     for (int c = 0; c < HD / 32; ++c) {
@@ -378,20 +379,26 @@ __device__ __noinline__ void rescale(uint32_t tO, uint32_t tS, bool has_o, int s
       tmem_st_32x32b_x32(tO + 32 * c, o);
     }
   }
-  if (stored) {
+  if (from < to) {
     tmem_st_wait();
 #pragma unroll 1
-    for (int c = 0; c < stored / 32; ++c) {
+    for (int c = from / 32; c < to / 32; ++c) {
       uint32_t x[16];
-      tmem_ld_32x32b_x16(tS + 16 * c, x);
+      tmem_ld_32x32b_x16(tP + 16 * c, x);
       tc::tmem_ld_wait();
 #pragma unroll
       for (int e = 0; e < 16; ++e)
         x[e] = narrow2<FMT>(widen16<FMT>((uint16_t)x[e]) * alpha, widen16<FMT>((uint16_t)(x[e] >> 16)) * alpha);
-      tmem_st_32x32b_x16(tS + 16 * c, x);
+      tmem_st_32x32b_x16(tP + 16 * c, x);
     }
   }
 }
+
+// First column of P (64 columns) among the 128 of S: P of a piece must only
+// cover columns of S that are read already, from the left when the keys are
+// taken from first to last, from the right when they are taken from last to
+// first.
+__host__ __device__ constexpr int p_column(bool last_first) { return last_first ? 64 : 0; }
 
 constexpr float kRescale = 8.f;  // log2 units: P holds up to 2^8
 
@@ -432,7 +439,7 @@ __device__ __forceinline__ void softmax_chunk(uint32_t (&sv)[N], uint32_t tS, ui
       l *= alpha;
       m = m == -INFINITY ? mx : m + up;
     }
-    if (has_o || at) rescale<HD, FMT>(tO, tS, has_o, at, alpha);
+    rescale<HD, FMT>(tO, tS + p_column(BIAS), has_o, BIAS ? at + N : 0, BIAS ? 128 : at, alpha);
   }
   const float mref = m == -INFINITY ? 0.f : m;
   uint32_t pk[N / 2];
@@ -445,8 +452,8 @@ __device__ __forceinline__ void softmax_chunk(uint32_t (&sv)[N], uint32_t tS, ui
     if (!w) rs = 0.f;
   }
   l += rs;
-  if constexpr (N == 64) tmem_st_32x32b_x32(tS + at / 2, pk);
-  else tmem_st_32x32b_x16(tS + at / 2, pk);
+  if constexpr (N == 64) tmem_st_32x32b_x32(tS + p_column(BIAS) + at / 2, pk);
+  else tmem_st_32x32b_x16(tS + p_column(BIAS) + at / 2, pk);
 }
 
 // The softmax of one tile in a single pass over S: P = exp2(score - m) as 16-bit
@@ -454,6 +461,9 @@ __device__ __forceinline__ void softmax_chunk(uint32_t (&sv)[N], uint32_t tS, ui
 // rescaled where the maximum has grown by more than kRescale.  P rounded to 16
 // bits (half a step of its own size) is what the MMA takes; the sum l is taken
 // before that, in 32 bits.
+// With a bias the keys are taken from the last to the first (and the tiles, by
+// the callers): the nearer a key, the larger its score, so that the maximum is
+// found at once instead of growing with every piece.
 // vis: a bit per key.  WIDE: with the way for whole tiles, taken where `whole`
 // says so (whole_tile, and with a bias all keys on one side); one_side: see
 // score_pair.
@@ -462,7 +472,8 @@ __device__ __forceinline__ void softmax_tile(uint32_t tS, uint32_t tO, const uin
                                              bool one_side, const Score& sc, bool has_o, float& m, float& l) {
   if (WIDE && whole) {
 #pragma unroll 1
-    for (int c = 0; c < 4; c += 2) {
+    for (int i = 0; i < 4; i += 2) {
+      const int c = BIAS ? 2 - i : i;
       uint32_t sv[64];
       tc::tmem_ld_32x32b_x32(tS + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(sv));
       tc::tmem_ld_32x32b_x32(tS + 32 * c + 32, *reinterpret_cast<uint32_t(*)[32]>(sv + 32));
@@ -472,14 +483,15 @@ __device__ __forceinline__ void softmax_tile(uint32_t tS, uint32_t tO, const uin
     return;
   }
 #pragma unroll 1
-  for (int c = 0; c < 4; ++c) {
+  for (int i = 0; i < 4; ++i) {
+    const int c = BIAS ? 3 - i : i;
     const uint32_t w = word_of(vis, c);
     const Piece kind = piece_of(w, !BIAS || one_side);
     if (kind == kNone) {
       uint32_t zero[16];
 #pragma unroll
       for (int e = 0; e < 16; ++e) zero[e] = 0;
-      tmem_st_32x32b_x16(tS + 16 * c, zero);
+      tmem_st_32x32b_x16(tS + p_column(BIAS) + 16 * c, zero);
       continue;
     }
     uint32_t sv[32];

@@ -69,16 +69,22 @@ __device__ __forceinline__ bool unit_of(const Params& p, int turn, Unit& u) {
   return true;
 }
 
-// What warps 2-3 find out about a unit's two Q tiles.
+// What warps 2-3 find out about a unit's two Q tiles.  KV tiles are counted in
+// the order in which they are taken: from the first key on, or with a bias from
+// the last one back (tile number -j, so that all the loops count up).
 struct Info {
-  int kb[2], nkv[2];            // KV tiles visited: kb .. nkv - 1
+  bool has[2];                  // a row of the tile sees anything
+  int kb[2], nkv[2];            // turns kb .. nkv - 1
   int lo_most[2], hi_least[2];  // keys that every row of the tile sees
   __device__ __forceinline__ bool active(int u, int j) const { return j >= kb[u] && j < nkv[u]; }
-  __device__ __forceinline__ bool masked(int u, int j) const { return j * BKV < lo_most[u] || j * BKV + BKV > hi_least[u]; }
-  __device__ __forceinline__ int first() const {
-    return nkv[0] == 0 ? kb[1] : nkv[1] == 0 ? kb[0] : min(kb[0], kb[1]);
+  __device__ __forceinline__ bool masked(int u, int tile) const {
+    return tile * BKV < lo_most[u] || tile * BKV + BKV > hi_least[u];
   }
-  __device__ __forceinline__ int last() const { return max(nkv[0], nkv[1]); }
+  __device__ __forceinline__ bool any() const { return has[0] || has[1]; }
+  __device__ __forceinline__ int first() const { return !has[0] ? kb[1] : !has[1] ? kb[0] : min(kb[0], kb[1]); }
+  __device__ __forceinline__ int last() const { return !has[0] ? nkv[1] : !has[1] ? nkv[0] : max(nkv[0], nkv[1]); }
+  // the Q tile whose turn comes first
+  __device__ __forceinline__ int lead() const { return !has[0] || (has[1] && kb[1] < kb[0]) ? 1 : 0; }
 };
 
 // Bits of the keys of [lo, hi) among the 128 from kv0 on.
@@ -184,6 +190,7 @@ scored_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
   tc::fence_after_sync();
   const uint32_t tmem = *tmem_holder;
 
+  auto tile_of = [](int j) { return BIAS ? -j : j; };  // KV tile of a turn
   // The info of turn k, once it is there; every reader says that it has it.
   auto read_info = [&](int k, Info& f) {
 #pragma unroll
@@ -194,8 +201,10 @@ scored_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
       f.hi_least[u] = min(a.w, b.w);
       // A row that sees anything sees itself or everything, so the two tiles'
       // spans touch and the pair's union has no gap.
-      f.kb[u] = hi > 0 ? lo / BKV : 0;
-      f.nkv[u] = (hi + BKV - 1) / BKV;
+      f.has[u] = hi > 0;
+      const int t0 = hi > 0 ? lo / BKV : 0, t1 = (hi + BKV - 1) / BKV;  // KV tiles t0 .. t1 - 1
+      f.kb[u] = BIAS ? 1 - t1 : t0;
+      f.nkv[u] = hi > 0 ? (BIAS ? 1 - t0 : t1) : f.kb[u];
     }
   };
 
@@ -224,20 +233,20 @@ scored_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
         read_info(k, f);
         mbar_arrive(&info_empty[k & 1]);
         const int jb = f.first(), je = f.last();
-        if (je == 0) continue;
+        if (!f.any()) continue;
         const int hk = un.h / (p.Hq / p.Hkv);
         // the unit's first Q tile has room while the unit before is still at
         // work; its second one takes the place of that unit's first
-        const int u0 = f.nkv[0] > 0 ? 0 : 1;
+        const int u0 = f.lead();
         load_q(u0);
         for (int j = jb; j < je && ok; ++j) {
           ok = wait_abort(&k_empty[kst], kph ^ 1, p.err, 0xB2600003u, abort_flag);
           if (!ok) break;
-          load(&tmK, sK + kst * kTile, &k_full[kst], j * BKV, hk, un.b);
-          if (j == jb && u0 == 0 && f.nkv[1] > 0) load_q(1);
+          load(&tmK, sK + kst * kTile, &k_full[kst], tile_of(j) * BKV, hk, un.b);
+          if (j == jb && f.has[u0 ^ 1]) load_q(u0 ^ 1);
           ok = ok && wait_abort(&v_empty[vst], vph ^ 1, p.err, 0xB2600004u, abort_flag);
           if (!ok) break;
-          load(&tmV, sV + vst * kTile, &v_full[vst], j * BKV, hk, un.b);
+          load(&tmV, sV + vst * kTile, &v_full[vst], tile_of(j) * BKV, hk, un.b);
           if (++kst == kK) { kst = 0; kph ^= 1; }
           if (++vst == kV) { vst = 0; vph ^= 1; }
         }
@@ -286,7 +295,7 @@ scored_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
           read_info(k, g);
           mbar_arrive(&info_empty[k & 1]);
           ++k;
-          if (g.last() > 0) return true;
+          if (g.any()) return true;
         }
         return false;
       };
@@ -323,7 +332,7 @@ scored_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
               tc::fence_after_sync();
 #pragma unroll
               for (int kk = 0; kk < BKV / Cf::KSTEP; ++kk)
-                mma_ts<FMT>(tmem + 256 * u + 128, tmem + 256 * u + kk * 8,
+                mma_ts<FMT>(tmem + 256 * u + 128, tmem + 256 * u + p_column(BIAS) + kk * 8,
                             tc::smem_desc(sV + vst * kTile + kk * Cf::KSTEP * 128, kAtom, 1024, tc::kSwizzle128B), idPV,
                             (j != f.kb[u]) || kk != 0);
               if (j == f.nkv[u] - 1) tc::commit(&o_done[u]);
@@ -411,21 +420,22 @@ scored_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
       __syncwarp();
       if (lane == 0) mbar_arrive(&info_empty[k & 1]);
       const int kb = f.kb[u], nkv = f.nkv[u];
-      const bool any_masked = nkv > kb && (f.masked(u, kb) || f.masked(u, nkv - 1));  // ranges end in a tile's span
+      // some tile is masked if the first or the last is
+      const bool any_masked = nkv > kb && (f.masked(u, tile_of(kb)) || f.masked(u, tile_of(nkv - 1)));
       float m_used = -INFINITY, l = 0.f;
       for (int j = kb; j < nkv; ++j) {
         ok = __all_sync(0xffffffffu, wait_abort(&s_full[u], sc & 1, p.err, 0xB260000Fu, abort_flag));
         if (!ok) break;
         ++sc;
         tc::fence_after_sync();
-        const int kv0 = j * BKV;
+        const int kv0 = tile_of(j) * BKV;
         const bool one_side = kv0 + BKV - 1 <= q0 || kv0 >= q0 + BQ - 1;  // where the tile's rows are not in it
         if constexpr (BIAS) {
           score.dist = (float)(qpos - kv0);
           score.slope = kv0 <= q0 ? slope : -slope;
         }
         uint32_t vis[4] = {~0u, ~0u, ~0u, ~0u};
-        if (f.masked(u, j)) range_bits(vis, row_lo, row_hi, kv0);
+        if (f.masked(u, tile_of(j))) range_bits(vis, row_lo, row_hi, kv0);
         const bool whole = (!BIAS || one_side) && whole_tile(vis);
         // O_u is quiescent: PV_u(j-1) finished before S_u(j)
         softmax_tile<true, HD, FMT, CAP, BIAS>(tS, tO, vis, whole, one_side, score, j > kb, m_used, l);

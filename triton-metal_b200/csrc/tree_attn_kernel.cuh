@@ -16,16 +16,16 @@
 // A run is a few segments, each inside one item; a segment that is not a whole
 // item leaves (m, l, unnormalised o) in the workspace, and a second kernel
 // joins those.
-// TMA form (contiguous caches and page sizes that are multiples of 8: a box holds
-// gcd(page size, 128) keys of one page):
+// TMA form (contiguous caches, and pages of which a box can hold 64 keys or more:
+// with 16 keys a box, 2 KB, the copy engine gave 2.5 TB/s over the 148 SMs):
 //   warp 0      TMA for Q, K and V into a ring of kRing tiles, in the order
 //               K0 K1 V0 K2 V1 ...
 //   warp 1      TMEM owner and MMA issuer
 //   warps 2-3   pass the tiles on; in V tiles with drafted tokens they zero the
 //               rows behind the last key and what is infinite or NaN
 //   warps 4-11  two softmax warpgroups, one row per thread (TMEM lane = row)
-// cp.async form (any other page size): warps 0-3 copy with 16-byte cp.async and do
-// the zeroing, warp 12 issues the MMAs.
+// cp.async form (smaller boxes): warps 0-2 copy with 16-byte cp.async and do the
+// zeroing, warp 3 issues the MMAs.
 // TMEM as in the prefill kernel: unit u has S_u / P_u at column 256u and O_u at
 // 256u + 128.  With one row tile per item (SINGLE) the two units take the even
 // and the odd key tiles of the same rows, so that one unit's softmax runs under
@@ -42,8 +42,8 @@ namespace tree {
 
 using namespace fa;
 
-template <bool TMA>
-constexpr int kThreads = TMA ? 384 : 416;
+constexpr int kThreads = 384;
+constexpr int kCopyRows = 44;              // cp.async form: rows of a copying warp (the third: 40)
 constexpr int BR = 128, BK = 128;          // rows and keys of a tile
 constexpr int kItemCost = 2;               // what starting and ending an item costs, in tiles
 
@@ -250,11 +250,11 @@ __device__ __forceinline__ int k_at(int i) { return i == 0 ? 0 : 2 * i - 1; }
 __device__ __forceinline__ int v_at(int i, int n) { return i == n - 1 ? 2 * n - 1 : 2 * i + 2; }
 
 template <int HD, int FMT, bool PAIR, bool CAP, bool BIAS, bool TMA>
-__global__ void __launch_bounds__(kThreads<TMA>, 1)
+__global__ void __launch_bounds__(kThreads, 1)
 tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
             const __grid_constant__ CUtensorMap tmV, const Params p) {
   using C = Cfg<HD>;
-  constexpr int NS = C::kRing, LAG = C::kLag, NT = kThreads<TMA>, kMmaWarp = TMA ? 1 : 12;
+  constexpr int NS = C::kRing, LAG = C::kLag, NT = kThreads, kMmaWarp = TMA ? 1 : 3;
   constexpr int kRows = PAIR ? 2 * BR : BR;  // rows of an item
   const int tokens = p.tpt * (PAIR ? 2 : 1), br = p.tpt * p.rep;  // of an item; rows of a tile
   extern __shared__ uint8_t smem_raw[];
@@ -284,7 +284,7 @@ tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (tid == 0) {
     for (int i = 0; i < NS; ++i) {
-      mbar_init(&full[i], TMA ? 1 : 128);
+      mbar_init(&full[i], TMA ? 1 : 96);
       mbar_init(&ready[i], 2);
       mbar_init(&empty[i], 1);
     }
@@ -366,9 +366,11 @@ tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
   }
 
   Segment sg;
+  // key tile that the segment's i-th turn takes: with a bias from the last one on
+  auto key_tile = [&](int i) { return sg.tile + (BIAS ? sg.n - 1 - i : i); };
   if (TMA && some && warp == 0) {
     // ----------------------------------- TMA -----------------------------------
-    // Lane i issues box i / NA, columns 64 (i % NA): at most 16 boxes of 8 keys.
+    // Lane i issues box i / NA, columns 64 (i % NA).
     constexpr int NA = HD / 64;
     const int boxes = BK / p.box, mine_box = lane / NA, atom = lane % NA;
     const bool has_box = mine_box < boxes;
@@ -384,7 +386,7 @@ tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
       ok = __all_sync(0xffffffffu, wait_abort(&empty[slot], ((seq / NS) & 1) ^ 1, p.err, 0xB2400002u, abort_flag));
       if (!ok) return;
       uint8_t* dst = sRing + slot * C::kTile + atom * C::kAtom + mine_box * p.box * 128;
-      const int pos = (sg.tile + tile) * BK + mine_box * p.box;
+      const int pos = key_tile(tile) * BK + mine_box * p.box;
       bool valid = has_box && pos < sg.keys;
       if (valid && p.page_size && (pg < 0 || pg >= p.n_pages)) {
         valid = false;  // none of the cache's pages: zeros
@@ -407,7 +409,7 @@ tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
     };
     while (ok && walk.next(p, tokens, sg)) {
       auto page = [&](int tile) {
-        const int pos = (sg.tile + tile) * BK + mine_box * p.box;
+        const int pos = key_tile(tile) * BK + mine_box * p.box;
         return has_box && tile < sg.n && pos < sg.keys ? key_page(p, sg.b, pos) : 0;
       };
       int pg = page(0), pg1 = page(1);  // one tile ahead
@@ -443,7 +445,7 @@ tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
         ok = __all_sync(0xffffffffu, wait_abort(&full[slot], (seq / NS) & 1, p.err, 0xB240000Bu, abort_flag));
         if (!ok) break;
         const int i = e == 2 * sg.n - 1 ? sg.n - 1 : e > 0 && e % 2 == 0 ? e / 2 - 1 : -1;  // V_i, or -1: a K tile
-        const int kv0 = (sg.tile + i) * BK;
+        const int kv0 = key_tile(i) * BK;
         if (i >= 0 && kv0 + BK > sg.ctx) {
           uint4* tile = reinterpret_cast<uint4*>(sRing + slot * C::kTile);
           const int first = max(sg.ctx - kv0, 0), last = sg.keys - kv0;  // drafted rows, then rows behind the end
@@ -469,14 +471,11 @@ tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
       ++seg;
     }
   }
-  // Registers of the cp.async form: 13 warps are launched with 128 a thread
-  // (53,248); the copying warpgroup gives some up to the two softmax warpgroups,
-  // which would spill: 128 x 88 + 256 x 144 + 32 x 128 = 52,224.
-  if (!TMA && some && warp < 4) {
+  if (!TMA && some && warp < 3) {
     // --------------------------------- copies ---------------------------------
-    if constexpr (!TMA) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     constexpr int CH = HD / 8, RPP = 32 / CH;  // 16-byte chunks of a row, rows a warp copies at once
     const int cc = lane % CH, rsub = lane / CH;
+    const int row0 = kCopyRows * warp, its = (warp == 2 ? 128 - 2 * kCopyRows : kCopyRows) / RPP;
     uint32_t seq = 0, handed = 0;  // tiles issued / handed over
     uint32_t end0 = 0, end1 = 0;   // seq at the end of the last segment and of the one before
     uint64_t meta = 0;             // 12 bits a tile in flight: first drafted row of a V tile (255: none), parity
@@ -494,8 +493,8 @@ tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
       if (first < 128) {
         bool bad = false;
         const uint32_t tile = smem_u32(sRing) + slot * C::kTile;
-        for (int i = 0; i < 32 / RPP; ++i) {
-          const int r = 32 * warp + RPP * i + rsub;
+        for (int i = 0; i < its; ++i) {
+          const int r = row0 + RPP * i + rsub;
           if (r < first) continue;
           uint4* at = reinterpret_cast<uint4*>(sRing + (chunk_at(tile, r) - smem_u32(sRing)));
           uint4 x = *at;
@@ -528,11 +527,16 @@ tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
       cp_async_wait<0>();
       while (handed != seq) hand_over((uint32_t)(meta >> (12 * (seq - handed - 1))) & 0xfff);
     };
-    auto copy_tile = [&](uint32_t tile, const uint16_t* base, int64_t off) {  // off < 0: zeros
+    // element offsets of this warp's rows: lane i has rows i and 32 + i; < 0: zeros
+    struct Rows {
+      int64_t a, b;
+    };
+    auto copy_tile = [&](uint32_t tile, const uint16_t* base, const Rows& off) {
 #pragma unroll
-      for (int i = 0; i < 32 / RPP; ++i) {
-        const int64_t o = __shfl_sync(0xffffffffu, off, RPP * i + rsub);
-        const int r = 32 * warp + RPP * i + rsub;
+      for (int i = 0; i < kCopyRows / RPP; ++i) {
+        if (i >= its) break;
+        const int64_t o = __shfl_sync(0xffffffffu, RPP * i < 32 ? off.a : off.b, (RPP * i + rsub) & 31);
+        const int r = row0 + RPP * i + rsub;
         cp_async16(chunk_at(tile, r), base + (o < 0 ? 0 : o) + cc * 8, o >= 0);
       }
     };
@@ -547,29 +551,40 @@ tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
                         wait_abort(&epi_done[prev & 1], (prev >> 1) & 1, p.err, 0xB2400003u, abort_flag));
         if (!ok) break;
       }
-      // this lane's key of each tile, one tile ahead, and its page, two ahead
-      int64_t ko, vo, ko1 = -1, vo1 = -1;
-      auto key = [&](int tile) { return (sg.tile + tile) * BK + 32 * warp + lane; };
-      auto page = [&](int tile) { return tile < sg.n && key(tile) < sg.keys ? key_page(p, sg.b, key(tile)) : 0; };
-      auto locate = [&](int tile, int pg, int64_t& a, int64_t& c) {
-        a = c = -1;
-        if (key(tile) < sg.keys && !key_offset(p, sg.b, sg.hk, key(tile), pg, a, c)) {
-          atomicCAS(p.err, 0u, attn::kErrPage);
-          a = c = -1;
-        }
+      // this lane's keys of each tile, one tile ahead, and their pages, two ahead
+      Rows ko, vo, ko1 = {-1, -1}, vo1 = {-1, -1};
+      auto key = [&](int tile, int half) {  // -1: none
+        const int at = 32 * half + lane, pos = key_tile(tile) * BK + row0 + at;
+        return tile < sg.n && at < kCopyRows && row0 + at < BK && pos < sg.keys ? pos : -1;
       };
-      const int pg0 = page(0);
-      int pg1 = page(1);
+      auto page = [&](int tile) {
+        const int a = key(tile, 0), b = key(tile, 1);
+        return make_int2(a < 0 ? 0 : key_page(p, sg.b, a), b < 0 ? 0 : key_page(p, sg.b, b));
+      };
+      auto locate = [&](int tile, int2 pg, Rows& k, Rows& v) {
+        const int a = key(tile, 0), b = key(tile, 1);
+        k = {-1, -1};
+        v = {-1, -1};
+        bool fine = true;
+        if (a >= 0 && !key_offset(p, sg.b, sg.hk, a, pg.x, k.a, v.a)) k.a = v.a = -1, fine = false;
+        if (b >= 0 && !key_offset(p, sg.b, sg.hk, b, pg.y, k.b, v.b)) k.b = v.b = -1, fine = false;
+        if (!fine) atomicCAS(p.err, 0u, attn::kErrPage);
+      };
+      const int2 pg0 = page(0);
+      int2 pg1 = page(1);
       locate(0, pg0, ko, vo);
       uint32_t tile = begin();
       if (!ok) break;
 #pragma unroll 1
       for (int u = 0; u < (PAIR ? 2 : 1); ++u) {
         const int rt = PAIR ? 2 * sg.rt + u : sg.rt;
-        const int row = 32 * warp + lane, t = rt * p.tpt + row / p.rep;
-        int64_t off = -1;
-        if (row < br && t < p.T)
-          off = sg.b * p.qs[0] + (int64_t)t * p.qs[1] + (int64_t)(sg.hk * p.rep + row % p.rep) * p.qs[2];
+        auto q_row = [&](int at) {
+          const int row = row0 + at, t = rt * p.tpt + row / p.rep;
+          return at < kCopyRows && row < br && t < p.T
+                     ? sg.b * p.qs[0] + (int64_t)t * p.qs[1] + (int64_t)(sg.hk * p.rep + row % p.rep) * p.qs[2]
+                     : (int64_t)-1;
+        };
+        const Rows off = {q_row(lane), q_row(32 + lane)};
         copy_tile(smem_u32(sQ) + (PAIR ? u : seg & 1) * C::kTile, p.q, off);
       }
       copy_tile(tile, p.k, ko);
@@ -586,7 +601,7 @@ tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
         tile = begin();
         if (!ok) break;
         copy_tile(tile, p.v, vo);
-        const int first = max(sg.ctx - (sg.tile + i) * BK, 0);
+        const int first = max(sg.ctx - key_tile(i) * BK, 0);
         end((first < 128 && sg.dl > 0 ? first : 255) | (seg & 1) << 8);
         vo = vo1;
       }
@@ -621,7 +636,7 @@ tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
       auto issue_pv = [&](int u, const uint8_t* v, bool first) {
 #pragma unroll
         for (int kk = 0; kk < BK / 16; ++kk)
-          mma_ts<FMT>(tmem + 256 * u + 128, tmem + 256 * u + kk * 8,
+          mma_ts<FMT>(tmem + 256 * u + 128, tmem + 256 * u + p_column(BIAS) + kk * 8,
                       tc::smem_desc(v + kk * 16 * 128, C::kAtom, 1024, tc::kSwizzle128B), idPV, !first || kk != 0);
       };
       auto wait_p = [&](int u) {
@@ -686,7 +701,6 @@ tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
     }
   } else if (some && warp >= 4) {
     // --------------------------------- softmax ---------------------------------
-    if constexpr (!TMA) asm volatile("setmaxnreg.inc.sync.aligned.u32 144;");
     const int u = (warp - 4) >> 2, qw = warp & 3, r = qw * 32 + lane;
     const uint32_t lane_off = (uint32_t)(qw * 32) << 16;
     const uint32_t tS = tmem + 256 * u + lane_off, tO = tmem + 128 + lane_off;  // tO: of unit 0
@@ -718,7 +732,7 @@ tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
         if (!ok) break;
         tc::fence_after_sync();
         if (warp_ok) {
-          const int kv0 = (sg.tile + j) * BK;
+          const int kv0 = key_tile(j) * BK;
           uint32_t vis[4] = {~0u, ~0u, ~0u, ~0u};
           if (kv0 + BK > sg.ctx) {
             visible_bits(vis, drafted, kv0 - sg.ctx);
@@ -729,12 +743,10 @@ tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
               for (int w = 0; w < 4; ++w) vis[w] |= more[w];
             }
           }
-          // SINGLE has no way of its own for whole tiles: half the code is half the
-          // instruction fetches, which is what a short call waits for
-          const bool whole = PAIR && whole_tile(vis);
+          const bool whole = whole_tile(vis);
           // single tokens only: every visible key is at or before the row's own
           if constexpr (BIAS) score.dist = (float)(sg.ctx - kv0);
-          softmax_tile<PAIR, HD, FMT, CAP, BIAS>(tS, tO + 256 * u, vis, whole, true, score, !first, m_used, l);
+          softmax_tile<true, HD, FMT, CAP, BIAS>(tS, tO + 256 * u, vis, whole, true, score, !first, m_used, l);
           tmem_st_wait();
         }
         first = false;
@@ -979,7 +991,7 @@ template <int HD, int FMT, bool PAIR, bool CAP, bool BIAS, bool TMA>
 static void launch(const Maps& m, const Params& p, cudaStream_t st) {
   const int G = num_sms();
   set_max_smem((const void*)tree_kernel<HD, FMT, PAIR, CAP, BIAS, TMA>, Cfg<HD>::kSmem);
-  tree_kernel<HD, FMT, PAIR, CAP, BIAS, TMA><<<G, kThreads<TMA>, Cfg<HD>::kSmem, st>>>(m.q, m.k, m.v, p);
+  tree_kernel<HD, FMT, PAIR, CAP, BIAS, TMA><<<G, kThreads, Cfg<HD>::kSmem, st>>>(m.q, m.k, m.v, p);
   const int rows = PAIR ? 2 * BR : (p.T < p.tpt ? p.T : p.tpt) * p.rep;
   const dim3 grid((unsigned)(p.n_rt * p.Hkv * ((rows + kJoin - 1) / kJoin)), p.B);
   cudaLaunchConfig_t cfg = {};
@@ -1008,7 +1020,7 @@ int launch_decode(const void* q, const void* k, const void* v, void* o, const in
 // d, key, head, request; paged: d, head, token, page), boxes of one 128-byte
 // swizzle row by the rows that the kernel's copies ask for.
 bool make_maps(Maps& m, const Params& p, int64_t D, int64_t Hq, bool f16);
-// Keys of a K / V box, 0 where the TMA form does not take the cache.
+// Keys of a K / V box where the TMA form takes the cache, else 0.
 int box_of(int64_t page_size, int64_t n_pages);
 // Bytes of the workspace: two partials a CTA.
 size_t workspace(int64_t T, int64_t rep, int64_t D);

@@ -51,7 +51,7 @@ int box_of(int64_t page_size, int64_t n_pages) {
   if (n_pages <= 0) return 0;
   int box = BK;
   while (box && page_size % box) box /= 2;
-  return box >= 8 ? box : 0;  // a swizzle atom has 8 rows
+  return box >= 8 ? box : 0;
 }
 
 size_t workspace(int64_t T, int64_t rep, int64_t D) {
