@@ -41,7 +41,8 @@ int launch_decode(const void* q, const void* k, const void* v, void* o, const in
   t.Hkv = (int)Hkv;
   t.rep = (int)rep;
   t.cap = (int)max_keys;
-  t.tpt = (int)(BR / rep);
+  t.copies = copies_of(rep);
+  t.tpt = (int)(BR / t.copies / rep);
   t.n_rt = 1;
   t.page_size = (uint32_t)page_size;
   t.max_pages = (int)max_pages;

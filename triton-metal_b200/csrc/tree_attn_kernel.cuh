@@ -32,6 +32,11 @@
 // the other's MMAs, and their (m, l, O) are joined from TMEM at the segment's
 // end; with more row tiles (PAIR) the units are two row tiles that share every
 // K/V tile.
+// Few rows (at most 64 or 32) would leave most softmax warps idle, since a warp
+// reaches only its own 32 TMEM lanes: such rows stand in the tile 2 or 4 times,
+// and each copy takes every 2nd or 4th part of a tile's keys (its P is 0 for the
+// others), so that all warps share the exponentials.  The copies are joined like
+// the units, through shared memory.
 #pragma once
 #include "attn_common.cuh"
 #include "fa_common.cuh"
@@ -69,7 +74,8 @@ struct Params {
   int64_t mask_stride, n_pages;
   int64_t qs[3], os[3], ks[3], vs[3];
   int B, T, Hkv, rep, cap;      // rep: query heads of a kv head; cap: keys a cache row holds
-  int tpt;                      // drafted tokens of a row tile: 128 / rep, rows t * rep + head
+  int tpt;                      // drafted tokens of a row tile, rows t * rep + head
+  int copies;                   // how often the rows stand in the tile (SINGLE: 1, 2 or 4)
   int n_rt;                     // items of a kv head: row tiles (PAIR: pairs of them)
   uint32_t page_size;           // 0: contiguous
   int max_pages;
@@ -224,6 +230,7 @@ __device__ __forceinline__ bool any_of_softmax(bool x) {
       : "memory");
   return r != 0;
 }
+__device__ __forceinline__ void warpgroup_sync(int u) { asm volatile("barrier.cta.sync %0, 128;" ::"r"(3 + u) : "memory"); }
 __device__ __forceinline__ void softmax_sync() { asm volatile("barrier.cta.sync 2, 256;" ::: "memory"); }
 
 // Page table entry of key `pos` of request b (contiguous: 0).
@@ -257,6 +264,7 @@ tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
   constexpr int NS = C::kRing, LAG = C::kLag, NT = kThreads, kMmaWarp = TMA ? 1 : 3;
   constexpr int kRows = PAIR ? 2 * BR : BR;  // rows of an item
   const int tokens = p.tpt * (PAIR ? 2 : 1), br = p.tpt * p.rep;  // of an item; rows of a tile
+  const int copies = PAIR ? 1 : p.copies, rw = BR / copies;       // rows a copy takes up
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem_raw);
@@ -395,15 +403,16 @@ tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
         tc::fence_proxy_async_smem();
       }
       const int n = __popc(__ballot_sync(0xffffffffu, valid));
-      if (lane == 0) mbar_arrive_expect_tx(&full[slot], n * p.box * 128 + q_tiles * NA * br * 128);
+      if (lane == 0) mbar_arrive_expect_tx(&full[slot], n * p.box * 128 + q_tiles * copies * NA * br * 128);
       __syncwarp();
       if (valid) {
         if (p.page_size) load4(dst, m, sg.hk, (uint32_t)pos % p.page_size, pg, &full[slot]);
         else load4(dst, m, pos, sg.hk, sg.b, &full[slot]);
       }
-      if (lane < q_tiles * NA) {
-        const int u = lane / NA, rt = PAIR ? 2 * sg.rt + u : sg.rt;
-        load4(sQ + (PAIR ? u : seg & 1) * C::kTile + atom * C::kAtom, &tmQ, sg.hk * p.rep, rt * p.tpt, sg.b, &full[slot]);
+      if (lane < q_tiles * copies * NA) {
+        const int i = lane / NA, rt = PAIR ? 2 * sg.rt + i : sg.rt;  // PAIR: row tile, else copy
+        load4(sQ + (PAIR ? i : seg & 1) * C::kTile + atom * C::kAtom + (PAIR ? 0 : i * rw * 128), &tmQ, sg.hk * p.rep,
+              rt * p.tpt, sg.b, &full[slot]);
       }
       ++seq;
     };
@@ -579,7 +588,7 @@ tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
       for (int u = 0; u < (PAIR ? 2 : 1); ++u) {
         const int rt = PAIR ? 2 * sg.rt + u : sg.rt;
         auto q_row = [&](int at) {
-          const int row = row0 + at, t = rt * p.tpt + row / p.rep;
+          const int row = (row0 + at) & (rw - 1), t = rt * p.tpt + row / p.rep;
           return at < kCopyRows && row < br && t < p.T
                      ? sg.b * p.qs[0] + (int64_t)t * p.qs[1] + (int64_t)(sg.hk * p.rep + row % p.rep) * p.qs[2]
                      : (int64_t)-1;
@@ -710,12 +719,14 @@ tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
     while (walk.next(p, tokens, sg)) {
       const int rt = PAIR ? 2 * sg.rt + u : sg.rt;
       const int units = PAIR ? ((2 * sg.rt + 1) * p.tpt < p.T ? 2 : 1) : min(sg.n, 2);
-      const int tt = r / p.rep, t = rt * p.tpt + tt, head = sg.hk * p.rep + r - tt * p.rep;
-      const bool row_in = r < br && t < p.T, row_ok = row_in && t < sg.dl;
+      const int copy = r / rw, row = r - copy * rw;
+      const int tt = row / p.rep, t = rt * p.tpt + tt, head = sg.hk * p.rep + row - tt * p.rep;
+      const bool row_in = row < br && t < p.T, row_ok = row_in && t < sg.dl;
       // tokens of this warp; a warp without one leaves its P rows as they are
       // (their O is never read)
-      const int t0 = rt * p.tpt + qw * 32 / p.rep, t1 = min(rt * p.tpt + min((qw * 32 + 31) / p.rep, p.tpt - 1), sg.dl - 1);
-      const bool warp_ok = t0 < sg.dl && qw * 32 < br, warp_in = t0 < p.T && qw * 32 < br;
+      const int w0 = qw * 32 & (rw - 1);
+      const int t0 = rt * p.tpt + w0 / p.rep, t1 = min(rt * p.tpt + min((w0 + 31) / p.rep, p.tpt - 1), sg.dl - 1);
+      const bool warp_ok = t0 < sg.dl && w0 < br, warp_in = t0 < p.T && w0 < br;
       const uint8_t* mask = p.mask ? p.mask + sg.b * p.mask_stride : nullptr;
       if constexpr (BIAS) score.slope = row_in ? p.slopes[head] * attn::kLog2e : 0.f;
       // mask bits of the first 128 drafted tokens, read while the first keys are
@@ -743,10 +754,18 @@ tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
               for (int w = 0; w < 4; ++w) vis[w] |= more[w];
             }
           }
-          const bool whole = whole_tile(vis);
+          if (!PAIR && copies > 1) {
+#pragma unroll
+            for (int w = 0; w < 4; ++w)
+              if (w * copies / 4 != copy) vis[w] = 0;
+          }
+          // SINGLE has no way of its own for whole tiles: it doubles the code of the
+          // inner loop, whose instruction fetches then set its pace (single tokens
+          // with cap and bias over 1 GB of cache: 360 us with it, 284 us without)
+          const bool whole = PAIR && whole_tile(vis);
           // single tokens only: every visible key is at or before the row's own
           if constexpr (BIAS) score.dist = (float)(sg.ctx - kv0);
-          softmax_tile<true, HD, FMT, CAP, BIAS>(tS, tO + 256 * u, vis, whole, true, score, !first, m_used, l);
+          softmax_tile<PAIR, HD, FMT, CAP, BIAS>(tS, tO + 256 * u, vis, whole, true, score, !first, m_used, l);
           tmem_st_wait();
         }
         first = false;
@@ -761,14 +780,15 @@ tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
       if constexpr (!PAIR) {
         s_ml[u * 128 + r] = make_float2(m_used, l);
         softmax_sync();
-        const float2 ot = s_ml[(u ^ 1) * 128 + r];
-        M = fmaxf(m_used, ot.x);
+        for (int i = 0; i < 2 * copies; ++i) M = fmaxf(M, s_ml[(i & 1) * 128 + (i >> 1) * rw + row].x);
         const float ref = M == -INFINITY ? 0.f : M;
-        const float fa = m_used == -INFINITY ? 0.f : ex2(m_used - ref);
-        const float fb = ot.x == -INFINITY ? 0.f : ex2(ot.x - ref);
-        L = l * fa + ot.y * fb;
-        f0 = u ? fb : fa;
-        f1 = u ? fa : fb;
+        L = f0 = 0.f;
+        for (int i = 0; i < 2 * copies; ++i) {
+          const float2 ml = s_ml[(i & 1) * 128 + (i >> 1) * rw + row];
+          const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - ref);
+          L = fmaf(ml.y, f, L);
+          if (i >> 1 == copy) (i & 1 ? f1 : f0) = f;
+        }
       }
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
@@ -776,11 +796,85 @@ tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
         ok = ok && __all_sync(0xffffffffu, wait_abort(&o_done[x], oc[x] & 1, p.err, 0xB240000Au, abort_flag));
         ++oc[x];
       }
-      if (ok && (!PAIR || u < units) && warp_in) {
+      const bool whole = sg.n == sg.of;  // else a partial: before the run's first item border, or behind its last
+      const bool bad = s_bad[seg & 1] == seg;
+      const float inv = L > 0.f || L != L ? 1.f / L : 0.f;
+      float* part = p.ws + (2 * (int64_t)blockIdx.x + (sg.tile == 0 ? 1 : 0)) * (kRows * (HD + 2));
+      // A drafted token's V that is infinite or NaN, for the rows that see it
+      // (columns c .. c + N - 1)
+      auto add_bad = [&](float* o, int c, int N) {
+        const int j0 = max(sg.tile * BK - sg.ctx, 0), j1 = min((sg.tile + sg.n) * BK - sg.ctx, sg.dl);
+        for (int j = j0; j < j1; ++j) {
+          int64_t ko, vo;
+          if (mask && !mask[(int64_t)t * p.T + j]) continue;
+          if (!key_offset(p, sg.b, sg.hk, sg.ctx + j, key_page(p, sg.b, sg.ctx + j), ko, vo)) continue;
+#pragma unroll
+          for (int e = 0; e < N; ++e) {
+            const uint16_t h = p.v[vo + c + e];
+            if (not_finite16<FMT>(h)) o[e] += widen16<FMT>(h);
+          }
+        }
+      };
+      if (!PAIR && copies > 1) {
+        // Copies: each warp stages its rows' sums over the units, CW columns at a
+        // time, and the warpgroup adds the copies up on the way out.
+        if (!any_of_softmax(!ok)) {
+          tc::fence_after_sync();
+          constexpr int CW = HD == 128 ? 32 : 16, CPR = CW / 4;
+          uint8_t* area = sQ + (seg & 1) * C::kTile + u * 128 * CW * 4;
+          auto staged = [&](int rr, int ch) { return reinterpret_cast<float4*>(area + rr * CW * 4 + ((ch ^ (rr / (8 / CPR) & (CPR - 1))) << 4)); };
+          if (!whole && u == 0 && copy == 0) {
+            part[kRows * HD + row] = row_ok ? M : -INFINITY;
+            part[kRows * HD + kRows + row] = row_ok ? L : 0.f;
+          }
+#pragma unroll 1
+          for (int c = u * (HD / 2); c < (u + 1) * (HD / 2); c += CW) {
+            float o[CW];
+            float o1[CW];
+            if constexpr (CW == 32) {
+              tc::tmem_ld_32x32b_x32(tO + c, *reinterpret_cast<uint32_t(*)[32]>(o));
+              if (units == 2) tc::tmem_ld_32x32b_x32(tO + 256 + c, *reinterpret_cast<uint32_t(*)[32]>(o1));
+            } else {
+              tmem_ld_32x32b_x16(tO + c, *reinterpret_cast<uint32_t(*)[16]>(o));
+              if (units == 2) tmem_ld_32x32b_x16(tO + 256 + c, *reinterpret_cast<uint32_t(*)[16]>(o1));
+            }
+            tc::tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < CW; ++e) {
+              float x = f0 == 0.f ? 0.f : o[e] * f0;
+              if (units == 2 && f1 != 0.f) x = fmaf(o1[e], f1, x);
+              o[e] = x;
+            }
+            if (bad && row_ok && copy == 0) add_bad(o, c, CW);
+            const float scale = whole ? inv : 1.f;
+#pragma unroll
+            for (int e = 0; e < CW; ++e) o[e] = row_ok && L != 0.f ? o[e] * scale : 0.f;
+#pragma unroll
+            for (int e = 0; e < CPR; ++e) *staged(r, e) = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+            warpgroup_sync(u);
+            for (int i = tid & 127; i < rw * CPR; i += 128) {
+              const int rr = i / CPR, ch = i % CPR, t2 = rt * p.tpt + rr / p.rep;
+              if (rr >= br || t2 >= p.T) continue;
+              float4 a = *staged(rr, ch);
+              for (int k = 1; k < copies; ++k) {
+                const float4 b = *staged(rr + k * rw, ch);
+                a.x += b.x;
+                a.y += b.y;
+                a.z += b.z;
+                a.w += b.w;
+              }
+              if (whole) {
+                uint16_t* to = p.o + sg.b * p.os[0] + (int64_t)t2 * p.os[1] + (int64_t)(sg.hk * p.rep + rr % p.rep) * p.os[2] + c + 4 * ch;
+                *reinterpret_cast<uint2*>(to) = make_uint2(narrow2<FMT>(a.x, a.y), narrow2<FMT>(a.z, a.w));
+              } else {
+                *reinterpret_cast<float4*>(part + rr * HD + c + 4 * ch) = a;
+              }
+            }
+            warpgroup_sync(u);
+          }
+        }
+      } else if (ok && (!PAIR || u < units) && warp_in) {
         tc::fence_after_sync();
-        const bool whole = sg.n == sg.of;  // else a partial: before the run's first item border, or behind its last
-        const bool bad = s_bad[seg & 1] == seg;
-        const float inv = L > 0.f || L != L ? 1.f / L : 0.f;
         constexpr int kCols = PAIR ? HD : HD / 2;
         const int c0 = PAIR ? 0 : u * kCols;
         // Rows leave through shared memory (Q's tile, which the segment no longer
@@ -794,8 +888,7 @@ tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
           if (row_in)
             dst = reinterpret_cast<uint8_t*>(p.o + sg.b * p.os[0] + (int64_t)t * p.os[1] + (int64_t)head * p.os[2]);
         } else {
-          const int64_t slot = 2 * (int64_t)blockIdx.x + (sg.tile == 0 ? 1 : 0);
-          float* w = p.ws + slot * (kRows * (HD + 2));
+          float* w = part;
           const int prow = PAIR ? u * BR + r : r;
           if (PAIR || u == 0) {
             w[kRows * HD + prow] = row_ok ? M : -INFINITY;
@@ -832,19 +925,7 @@ tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
               o[e] = x;
             }
           }
-          if (bad && row_ok) {
-            const int j0 = max(sg.tile * BK - sg.ctx, 0), j1 = min((sg.tile + sg.n) * BK - sg.ctx, sg.dl);
-            for (int j = j0; j < j1; ++j) {
-              int64_t ko, vo;
-              if (mask && !mask[(int64_t)t * p.T + j]) continue;
-              if (!key_offset(p, sg.b, sg.hk, sg.ctx + j, key_page(p, sg.b, sg.ctx + j), ko, vo)) continue;
-#pragma unroll
-              for (int e = 0; e < 32; ++e) {
-                const uint16_t h = p.v[vo + c + e];
-                if (not_finite16<FMT>(h)) o[e] += widen16<FMT>(h);
-              }
-            }
-          }
+          if (bad && row_ok) add_bad(o, c, 32);
           if (!row_ok || L == 0.f) {
 #pragma unroll
             for (int e = 0; e < 32; ++e) o[e] = 0.f;
@@ -1005,6 +1086,9 @@ static void launch(const Maps& m, const Params& p, cudaStream_t st) {
   cfg.numAttrs = 1;
   cudaLaunchKernelEx(&cfg, tree_join_kernel<HD, FMT, PAIR>, p, (int64_t)G);
 }
+
+// Copies of the rows in a tile: as many as fit.
+inline int copies_of(int64_t rows) { return rows <= 32 ? 4 : rows <= 64 ? 2 : 1; }
 
 // The forms: TMA of drafted trees (tree_attn_sm100.cu), cp.async of drafted
 // trees (tree_attn_cp_sm100.cu), TMA of single tokens with capped or biased

@@ -145,7 +145,8 @@ extern "C" int b2_tree_attn(const void* q, const void* k, const void* v, void* o
   bool wide = aligned(q, 16) && aligned(k, 16) && aligned(v, 16) && aligned(o, 16) && aligned(workspace, 16);
   for (int i = 0; i < 3; ++i)
     wide = wide && q_strides[i] % 8 == 0 && k_strides[i] % 8 == 0 && v_strides[i] % 8 == 0 && o_strides[i] % 8 == 0;
-  const int64_t tpt = rep <= tree::BR ? tree::BR / rep : 0;
+  const int copies = tree::copies_of(T * rep);
+  const int64_t tpt = rep <= tree::BR ? tree::BR / copies / rep : 0;
   const bool pair = T > tpt;
   const int64_t n_rt = tpt ? (T + tpt * (pair ? 2 : 1) - 1) / (tpt * (pair ? 2 : 1)) : 0;
   // scale > 0: the row maximum is taken before the scale
@@ -175,6 +176,7 @@ extern "C" int b2_tree_attn(const void* q, const void* k, const void* v, void* o
     t.rep = (int)rep;
     t.cap = (int)max_keys;
     t.tpt = (int)tpt;
+    t.copies = copies;
     t.n_rt = (int)n_rt;
     t.page_size = (uint32_t)page_size;
     t.max_pages = (int)max_pages;
