@@ -89,6 +89,7 @@ struct SimtParams {
   const int32_t *ctx, *draft;                // tree: context / draft lengths (draft null: T)
   float* ws;                                 // split partials, rows of (m, l, D values)
   int nsplit, split_len;
+  int wide;                                  // set by launch_simt: 16-byte loads of K / V rows
   unsigned* err;
 };
 

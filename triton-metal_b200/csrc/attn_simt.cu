@@ -124,7 +124,38 @@ __global__ void __launch_bounds__(kThreads) simt_kernel(const SimtParams p) {
     }
     __syncthreads();
     int odd = 0;  // a V value that is not finite
-    for (int e = tid; e < BN * DP; e += kThreads) {
+    // the tile: 16-byte loads, eight of K and of V in flight a thread, where rows
+    // start on 16 bytes and are whole vectors long, else one value at a time
+    constexpr int VE = 16 / (int)sizeof(TKV), VR = DP / VE;  // values of a vector, vectors of a row
+    if (p.wide) {
+#pragma unroll 1
+      for (int e0 = tid; e0 < BN * VR; e0 += 8 * kThreads) {
+        uint4 a[8], c[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          const int e = e0 + u * kThreads, j = e / VR, d = e % VR * VE;
+          const bool there = e < BN * VR && d < p.D && sOff[j] >= 0;
+          a[u] = there ? *reinterpret_cast<const uint4*>((const TKV*)p.k + sOff[j] + d) : make_uint4(0, 0, 0, 0);
+          c[u] = there ? *reinterpret_cast<const uint4*>((const TKV*)p.v + sOff[BN + j] + d) : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          const int e = e0 + u * kThreads, j = e / VR, d = e % VR * VE;
+          if (e >= BN * VR) break;
+          const TKV* ka = reinterpret_cast<const TKV*>(&a[u]);
+          const TKV* va = reinterpret_cast<const TKV*>(&c[u]);
+#pragma unroll
+          for (int x = 0; x < VE; x += 4) {
+            const float4 kf = make_float4(ldf(ka + x), ldf(ka + x + 1), ldf(ka + x + 2), ldf(ka + x + 3));
+            const float4 vf = make_float4(ldf(va + x), ldf(va + x + 1), ldf(va + x + 2), ldf(va + x + 3));
+            odd |= !(fabsf(vf.x) < INFINITY) | !(fabsf(vf.y) < INFINITY) | !(fabsf(vf.z) < INFINITY) | !(fabsf(vf.w) < INFINITY);
+            *reinterpret_cast<float4*>(sK + j * C::LD + d + x) = kf;
+            *reinterpret_cast<float4*>(sV + j * C::LD + d + x) = vf;
+          }
+        }
+      }
+    }
+    for (int e = tid; e < (p.wide ? 0 : BN * DP); e += kThreads) {
       const int j = e / DP, d = e % DP;
       float kv = 0.f, vv = 0.f;
       if (d < p.D && sOff[j] >= 0) {
@@ -315,6 +346,9 @@ int launch_simt(SimtParams p, int q_dtype, int kv_dtype, cudaStream_t st, const 
   p.nsplit = p.ws ? simt_splits(tiles * p.B * p.Hkv, p.Skv) : 1;
   p.split_len = (int)(((int64_t)p.Skv + p.nsplit - 1) / p.nsplit);
   p.split_len = (p.split_len + BN - 1) / BN * BN;
+  const int es = kv_dtype == B2_F32 ? 4 : 2;
+  p.wide = p.D * es % 16 == 0 && aligned(p.k, 16) && aligned(p.v, 16);
+  for (int i = 0; i < 3; ++i) p.wide = p.wide && p.ks[i] * es % 16 == 0 && p.vs[i] * es % 16 == 0;
   const dim3 grid((unsigned)(tiles * p.nsplit), p.Hkv, p.B);
 #define B2_SIMT_KV(TQ)                                             \
   do {                                                             \

@@ -115,22 +115,39 @@ __global__ void __launch_bounds__(kThreads) build_table_kernel(const TableParams
         if (sTok[mid] <= ta) lo = mid;
         else hi = mid;
       }
-      for (int64_t t = ta; t < tb; ++t) {
+      // where each token's page number stands, then all the loads together, then
+      // the stores: one trip to memory for the kPer of them
+      const int32_t* from[kPer];
+      int32_t* entry[kPer];
+      uint32_t off[kPer];
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) {
+        const int64_t t = t_lo + e;
+        from[e] = nullptr;
+        entry[e] = nullptr;
+        if (t < ta || t >= tb) continue;
         while (sTok[lo + 1] <= t) ++lo;
         const uint32_t c = sCtx[lo], pos = c + (uint32_t)(t - sTok[lo]), pi = pos / p.page_size;
-        const uint32_t have = pages_for(c, p.page_size), at = pos - pi * p.page_size;
-        int64_t page = -1;
-        if (pi < (uint32_t)p.max_pages) {
-          int32_t* entry = p.table + (int64_t)(r0 + lo) * p.table_stride + pi;
-          if (pi < have) {
-            page = *entry;
-          } else {
-            const int64_t f = sPage[lo] + (pi - have);
-            if (f < p.n_free) page = p.free_pages[f];
-            if (at == 0) *entry = (int32_t)page;
-          }
+        const uint32_t have = pages_for(c, p.page_size);
+        off[e] = pos - pi * p.page_size;
+        if (pi >= (uint32_t)p.max_pages) continue;
+        int32_t* at = p.table + (int64_t)(r0 + lo) * p.table_stride + pi;
+        if (pi < have) {
+          from[e] = at;
+        } else {
+          const int64_t f = sPage[lo] + (pi - have);
+          if (f < p.n_free) from[e] = p.free_pages + f;
+          if (off[e] == 0) entry[e] = at;
         }
-        p.slots[t] = page >= 0 ? page * p.page_size + at : -1;
+      }
+      int64_t page[kPer];
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) page[e] = from[e] ? *from[e] : -1;
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) {
+        if (t_lo + e < ta || t_lo + e >= tb) continue;
+        if (entry[e]) *entry[e] = (int32_t)page[e];
+        p.slots[t_lo + e] = page[e] >= 0 ? page[e] * p.page_size + off[e] : -1;
       }
     }
     tok0 = nt;
