@@ -295,6 +295,40 @@ def test_decode(cuda, qd, kd, paged, B, Hq, Hkv, S, D, cap, alibi, window):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dt,D", [(BF16, 128), (F16, 64)])
+@pytest.mark.parametrize("ps", [1, 4, 8, 12, 16, 32, 64, 128])
+@pytest.mark.parametrize("Hq,Hkv,cap,alibi", [(8, 8, 30.0, False), (6, 2, 0.0, True), (40, 1, 20.0, True)])
+def test_decode_page_sizes(cuda, dt, D, ps, Hq, Hkv, cap, alibi):
+    """Every way to load the cache, with infinities behind the last key."""
+    g = torch.Generator().manual_seed(ps + D)
+    lens = [0, 1, 129, 777]
+    B, S = len(lens), max(lens)
+    q = (torch.randn(B, Hq, D, generator=g) * 3).to(dt)
+    k, v = (torch.randn(B, Hkv, S, D, generator=g).to(dt) for _ in range(2))
+    width = -(-S // ps)
+    table = torch.randperm(B * width + 1, generator=g)[:B * width].reshape(B, width)
+    pages = []
+    for x in (k, v):
+        pg = torch.full((B * width + 1, ps, Hkv, D), math.inf, dtype=dt)
+        for b, n in enumerate(lens):
+            at = torch.arange(n)
+            pg[table[b, at // ps], at % ps] = x[b, :, :n].transpose(0, 1)
+        pages.append(pg.to(cuda))
+    slopes = _slopes(Hq) if alibi else None
+    out = bk.decode_attention(q.to(cuda), *pages, torch.tensor(lens, device=cuda), softcap=cap,
+                              page_table=table.to(torch.int32).to(cuda),
+                              alibi_slopes=None if slopes is None else slopes.to(cuda)).double().cpu()
+    for b, n in enumerate(lens):
+        far = (n - 1 - torch.arange(n).double())[None]
+        for h in range(Hq):
+            o, av, mag = scored.rows(q[b, h:h + 1], k[b, h // (Hq // Hkv), :n], v[b, h // (Hq // Hkv), :n],
+                                     torch.ones(1, n, dtype=torch.bool), 1 / math.sqrt(D), cap,
+                                     None if slopes is None else -slopes[h].double() * far)
+            lim = scored.bound(o, av, mag, dt, n, D, cap, 0.0 if slopes is None else min(float(slopes[h]) * S, 60.0))
+            assert bool(((out[b, h:h + 1] - o).abs() <= lim).all()), (b, h)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dt", [BF16, F32])
 def test_decode_rope_and_score_forms(cuda, dt):
     """RoPE and a query position together with cap and bias (distances count from q_pos)."""

@@ -159,6 +159,23 @@ def test_tree_context_lengths(cuda, dt, ctx):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dt,D", [(BF16, 128), (F16, 64)])
+@pytest.mark.parametrize("ps", [1, 3, 4, 8, 12, 32, 64, 100, 128])
+@pytest.mark.parametrize("T,Hq,Hkv,cap", [(4, 8, 2, 0.0), (12, 8, 2, 20.0), (25, 4, 1, 0.0), (80, 4, 2, 0.0)])
+def test_tree_page_sizes(cuda, dt, D, ps, T, Hq, Hkv, cap):
+    """Every way to load the cache; 16 to 160 rows a group: rows in the tile four times, twice, once, two tiles."""
+    _run(cuda, 3, T, Hq, Hkv, D, [0, 130, 517], [T, T - 1, T], dt, dt, ps, cap)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [BF16, F32])
+@pytest.mark.parametrize("T,Hq,Hkv", [(6, 3, 1), (4, 10, 2), (9, 7, 1), (3, 24, 1), (2, 40, 2), (2, 130, 1), (11, 48, 4)])
+def test_tree_head_groups(cuda, dt, T, Hq, Hkv):
+    """Groups that no power of two divides, and one of more heads than a tile has rows."""
+    _run(cuda, 2, T, Hq, Hkv, 64, [77, 300], [T, T], dt, dt, 16)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dt", [BF16, F16, F32])
 @pytest.mark.parametrize("cap,big", [(50.0, 8.0), (1.0, 4.0), (30.0, 40.0)])
 def test_tree_caps(cuda, dt, cap, big):

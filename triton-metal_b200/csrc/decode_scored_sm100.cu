@@ -51,24 +51,9 @@ int launch_decode(const void* q, const void* k, const void* v, void* o, const in
   t.slopes = slopes;
   t.err = device_error_word();
   t.box = box_of(page_size, n_pages);
-  const bool f16 = dtype == B2_F16, cap = softcap > 0.f;
-  Maps m;
+  const bool f16 = dtype == B2_F16;
   if (!t.err) return B2_ERR_UNSUPPORTED;
-  if (!t.box || !make_maps(m, t, D, Hq, f16)) {
-    launch_tree_cp(t, (int)D, f16, false, st);
-    return launch_status("decode_attn_scored");
-  }
-#define B2_DECODE(HD, FMT)                                                                   \
-  do {                                                                                       \
-    if (cap && slopes) launch<HD, FMT, false, true, true, true>(m, t, st);                   \
-    else if (cap) launch<HD, FMT, false, true, false, true>(m, t, st);                       \
-    else launch<HD, FMT, false, false, true, true>(m, t, st);                                \
-  } while (0)
-  if (D == 128 && f16) B2_DECODE(128, fa::kF16);
-  else if (D == 128) B2_DECODE(128, fa::kBF16);
-  else if (f16) B2_DECODE(64, fa::kF16);
-  else B2_DECODE(64, fa::kBF16);
-#undef B2_DECODE
+  launch_any(t, D, Hq, f16, false, st);
   return launch_status("decode_attn_scored");
 }
 

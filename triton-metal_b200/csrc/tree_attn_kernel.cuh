@@ -16,16 +16,19 @@
 // A run is a few segments, each inside one item; a segment that is not a whole
 // item leaves (m, l, unnormalised o) in the workspace, and a second kernel
 // joins those.
-// TMA form (contiguous caches, and pages of which a box can hold 64 keys or more:
-// with 16 keys a box, 2 KB, the copy engine gave 2.5 TB/s over the 148 SMs):
+// TMA form (contiguous caches, and page sizes that are a multiple of 8 keys):
 //   warp 0      TMA for Q, K and V into a ring of kRing tiles, in the order
-//               K0 K1 V0 K2 V1 ...
+//               K0 K1 V0 K2 V1 ...; a box is as many keys as divide a page and a
+//               tile.  Pages of 16 keys need eight boxes of 2 KB for 16 KB; with
+//               V copied by two warps instead, so that the copy engine had half
+//               the boxes, 48 requests of 16 heads over 4 to 8 thousand keys took
+//               365 us, not 282.
 //   warp 1      TMEM owner and MMA issuer
 //   warps 2-3   pass the tiles on; in V tiles with drafted tokens they zero the
 //               rows behind the last key and what is infinite or NaN
 //   warps 4-11  two softmax warpgroups, one row per thread (TMEM lane = row)
-// cp.async form (smaller boxes): warps 0-2 copy with 16-byte cp.async and do the
-// zeroing, warp 3 issues the MMAs.
+// cp.async form (other page sizes, and tensors that no tensor map describes):
+// warps 0-2 copy with 16-byte cp.async and do the zeroing, warp 3 issues the MMAs.
 // TMEM as in the prefill kernel: unit u has S_u / P_u at column 256u and O_u at
 // 256u + 128.  With one row tile per item (SINGLE) the two units take the even
 // and the odd key tiles of the same rows, so that one unit's softmax runs under
@@ -1090,10 +1093,29 @@ static void launch(const Maps& m, const Params& p, cudaStream_t st) {
 // Copies of the rows in a tile: as many as fit.
 inline int copies_of(int64_t rows) { return rows <= 32 ? 4 : rows <= 64 ? 2 : 1; }
 
-// The forms: TMA of drafted trees (tree_attn_sm100.cu), cp.async of drafted
-// trees (tree_attn_cp_sm100.cu), TMA of single tokens with capped or biased
-// scores (decode_scored_sm100.cu).
-void launch_tree_cp(const Params& p, int D, bool f16, bool pair, cudaStream_t st);
+// Launches by what the call has (BIAS: p.slopes, CAP: p.softcap).
+void launch_tma(const Maps& m, const Params& p, int D, bool f16, bool pair, cudaStream_t st);
+void launch_cp(const Maps& m, const Params& p, int D, bool f16, bool pair, cudaStream_t st);
+template <bool TMA>
+static void launch_form(const Maps& m, const Params& p, int D, bool f16, bool pair, cudaStream_t st) {
+  const bool cap = p.softcap.log2 > 0.f, bias = p.slopes != nullptr;  // bias: single tokens, never pair
+#define B2_TREE(HD, FMT)                                                                    \
+  do {                                                                                      \
+    if (pair && cap) launch<HD, FMT, true, true, false, TMA>(m, p, st);                     \
+    else if (pair) launch<HD, FMT, true, false, false, TMA>(m, p, st);                      \
+    else if (cap && bias) launch<HD, FMT, false, true, true, TMA>(m, p, st);                \
+    else if (bias) launch<HD, FMT, false, false, true, TMA>(m, p, st);                      \
+    else if (cap) launch<HD, FMT, false, true, false, TMA>(m, p, st);                       \
+    else launch<HD, FMT, false, false, false, TMA>(m, p, st);                               \
+  } while (0)
+  if (D == 128 && f16) B2_TREE(128, fa::kF16);
+  else if (D == 128) B2_TREE(128, fa::kBF16);
+  else if (f16) B2_TREE(64, fa::kF16);
+  else B2_TREE(64, fa::kBF16);
+#undef B2_TREE
+}
+// launch_tma where tensor maps can describe the tensors, else launch_cp.
+void launch_any(const Params& p, int64_t D, int64_t Hq, bool f16, bool pair, cudaStream_t st);
 int launch_decode(const void* q, const void* k, const void* v, void* o, const int32_t* page_table,
                   const int32_t* seq_lens, void* workspace, int64_t B, int64_t Hq, int64_t Hkv, int64_t D,
                   int64_t max_keys, int64_t page_size, int64_t max_pages, int64_t n_pages, const int64_t* k_strides,

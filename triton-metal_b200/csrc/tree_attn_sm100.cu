@@ -51,7 +51,17 @@ int box_of(int64_t page_size, int64_t n_pages) {
   if (n_pages <= 0) return 0;
   int box = BK;
   while (box && page_size % box) box /= 2;
-  return box >= 8 ? box : 0;
+  return box >= 8 ? box : 0;  // a swizzle atom has 8 rows
+}
+
+void launch_any(const Params& p, int64_t D, int64_t Hq, bool f16, bool pair, cudaStream_t st) {
+  Maps m = {};
+  if (!p.box || !make_maps(m, p, D, Hq, f16)) launch_cp(m, p, (int)D, f16, pair, st);
+  else launch_tma(m, p, (int)D, f16, pair, st);
+}
+
+void launch_tma(const Maps& m, const Params& p, int D, bool f16, bool pair, cudaStream_t st) {
+  launch_form<true>(m, p, D, f16, pair, st);
 }
 
 size_t workspace(int64_t T, int64_t rep, int64_t D) {
@@ -185,23 +195,7 @@ extern "C" int b2_tree_attn(const void* q, const void* k, const void* v, void* o
     t.err = p.err;
     t.box = tree::box_of(page_size, n_pages);
     const bool f16 = q_dtype == B2_F16;
-    tree::Maps m;
-    if (!t.box || !tree::make_maps(m, t, D, Hq, f16)) {
-      tree::launch_tree_cp(t, (int)D, f16, pair, st);
-      return launch_status("tree_attn");
-    }
-#define B2_TREE(HD, FMT)                                                                          \
-  do {                                                                                            \
-    if (pair && softcap > 0.f) tree::launch<HD, FMT, true, true, false, true>(m, t, st);          \
-    else if (pair) tree::launch<HD, FMT, true, false, false, true>(m, t, st);                     \
-    else if (softcap > 0.f) tree::launch<HD, FMT, false, true, false, true>(m, t, st);            \
-    else tree::launch<HD, FMT, false, false, false, true>(m, t, st);                              \
-  } while (0)
-    if (D == 128 && f16) B2_TREE(128, fa::kF16);
-    else if (D == 128) B2_TREE(128, fa::kBF16);
-    else if (f16) B2_TREE(64, fa::kF16);
-    else B2_TREE(64, fa::kBF16);
-#undef B2_TREE
+    tree::launch_any(t, D, Hq, f16, pair, st);
     return launch_status("tree_attn");
   }
   p.ws = need ? (float*)workspace : nullptr;
