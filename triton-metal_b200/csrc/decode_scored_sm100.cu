@@ -46,7 +46,6 @@ int launch_decode(const void* q, const void* k, const void* v, void* o, const in
   t.n_rt = 1;
   t.page_size = (uint32_t)page_size;
   t.max_pages = (int)max_pages;
-  t.scale_log2 = scale * attn::kLog2e;
   t.softcap = fa::make_cap(scale, softcap);
   t.slopes = slopes;
   t.err = device_error_word();

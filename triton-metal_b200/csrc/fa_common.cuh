@@ -4,6 +4,7 @@
 // between the MUFU unit and the FMA pipe).
 #pragma once
 #include "tc_common.cuh"
+#include <string.h>
 
 namespace b2 {
 namespace fa {
@@ -165,23 +166,38 @@ struct Score {
   float scale_log2;        // scale * log2 e (> 0)
   float cap_in, cap_log2;  // 2 log2 e scale / cap; cap * log2 e
   float small;             // scores up to this size take capped_small (0: none)
-  float t[5];              // its coefficients
+  uint64_t t[5], scale2;   // its coefficients and scale_log2, each twice
   float slope, dist;       // slope * log2 e; row - first key of the tile
 };
 
-// What a kernel's parameters hold of the cap.
+// What a kernel's parameters hold of it.  The operands of the paired instructions
+// lie there as pairs, so that they are read from constant memory; pairs made in
+// registers cost a move or two at every use.
 struct Cap {
-  float in, log2, small, t[5];
+  float scale_log2, in, log2, small;
+  uint64_t t[5], scale2;
 };
-__device__ __forceinline__ Score make_score(float scale_log2, const Cap& c) {
-  return {scale_log2, c.in, c.log2, c.small, {c.t[0], c.t[1], c.t[2], c.t[3], c.t[4]}, 0.f, 0.f};
+__device__ __forceinline__ Score make_score(const Cap& c) {
+  return {c.scale_log2, c.in, c.log2, c.small, {c.t[0], c.t[1], c.t[2], c.t[3], c.t[4]}, c.scale2, 0.f, 0.f};
 }
+// key numbers of a piece, for the distance bias
+__device__ __constant__ const float2 kKeys[32] = {
+    {0, 1},   {2, 3},   {4, 5},   {6, 7},   {8, 9},   {10, 11}, {12, 13}, {14, 15}, {16, 17}, {18, 19}, {20, 21},
+    {22, 23}, {24, 25}, {26, 27}, {28, 29}, {30, 31}, {32, 33}, {34, 35}, {36, 37}, {38, 39}, {40, 41}, {42, 43},
+    {44, 45}, {46, 47}, {48, 49}, {50, 51}, {52, 53}, {54, 55}, {56, 57}, {58, 59}, {60, 61}, {62, 63}};
 // tanh z = z p(z^2) on [-3/4, 3/4]: this file's own minimax fit (largest error
 // 2.4e-7 in fp32).  The coefficients take scale, cap and log2 e with them, so
 // that a score s gives s q(s^2); where the powers of scale / cap would leave
 // fp32's range (scale / cap below 2e-4), the form is not used.
 inline Cap make_cap(float scale, float softcap) {
   Cap c = {};
+  auto twice = [](float x) {
+    uint32_t u;
+    memcpy(&u, &x, 4);
+    return (uint64_t)u << 32 | u;
+  };
+  c.scale_log2 = scale * 1.4426950408889634f;
+  c.scale2 = twice(c.scale_log2);
   if (softcap > 0.f) {
     const double log2e = 1.4426950408889634, z = (double)scale / softcap;
     const double p[5] = {0.9999971985816956, -0.33323076367378235, 0.13226091861724854, -0.04928044602274895,
@@ -190,7 +206,7 @@ inline Cap make_cap(float scale, float softcap) {
     c.log2 = (float)(log2e * softcap);
     c.small = z > 2e-4 ? (float)(0.75 / z) : 0.f;
     double f = log2e * softcap * z;
-    for (int i = 0; i < 5; ++i, f *= z * z) c.t[i] = (float)(p[i] * f);
+    for (int i = 0; i < 5; ++i, f *= z * z) c.t[i] = twice((float)(p[i] * f));
   }
   return c;
 }
@@ -216,19 +232,20 @@ __device__ __forceinline__ float capped(float s, const Score& c, float add) {
 // operations a score of the form above would set the pace of the softmax.
 __device__ __forceinline__ uint64_t capped_small(uint64_t s, const Score& c, uint64_t add) {
   const uint64_t w = mul_f2(s, s);
-  uint64_t q = fma_f2(f2_pack(c.t[4], c.t[4]), w, f2_pack(c.t[3], c.t[3]));
-  q = fma_f2(q, w, f2_pack(c.t[2], c.t[2]));
-  q = fma_f2(q, w, f2_pack(c.t[1], c.t[1]));
-  q = fma_f2(q, w, f2_pack(c.t[0], c.t[0]));
+  uint64_t q = fma_f2(c.t[4], w, c.t[3]);
+  q = fma_f2(q, w, c.t[2]);
+  q = fma_f2(q, w, c.t[1]);
+  q = fma_f2(q, w, c.t[0]);
   return fma_f2(s, q, add);
 }
-// Whether all of the warp's N x 32 scores may take capped_small.
+// Whether all of the warp's N x 32 scores may take capped_small (w: 0 where the
+// row sees none of them).
 template <int N>
-__device__ __forceinline__ bool all_small(const uint32_t (&sv)[N], const Score& c) {
+__device__ __forceinline__ bool all_small(const uint32_t (&sv)[N], uint32_t w, const Score& c) {
   float am = 0.f;
 #pragma unroll
   for (int e = 0; e < N; e += 2) am = max3(am, fabsf(__uint_as_float(sv[e])), fabsf(__uint_as_float(sv[e + 1])));
-  return !__any_sync(0xffffffffu, !(am <= c.small));
+  return !__any_sync(0xffffffffu, w && !(am <= c.small));
 }
 
 // Score of two neighbouring keys (e and e + 1 from where c.dist counts), plus
@@ -244,14 +261,14 @@ __device__ __forceinline__ uint64_t score_pair(uint32_t s0, uint32_t s1, int e, 
       a = f2_pack(fmaf(sl, fabsf(c.dist - (float)e), add), fmaf(sl, fabsf(c.dist - (float)(e + 1)), add));
     } else {
       const float b = fmaf(-c.slope, c.dist, add);
-      a = fma_f2(f2_pack(c.slope, c.slope), f2_pack((float)e, (float)(e + 1)), f2_pack(b, b));
+      a = fma_f2(f2_pack(c.slope, c.slope), f2_pack(kKeys[e / 2].x, kKeys[e / 2].y), f2_pack(b, b));
     }
   }
   const uint64_t s = (uint64_t)s0 | ((uint64_t)s1 << 32);
   if constexpr (CAP && SMALL) return capped_small(s, c, a);
   if constexpr (CAP)
     return f2_pack(capped(__uint_as_float(s0), c, f2_lo(a)), capped(__uint_as_float(s1), c, f2_hi(a)));
-  return fma_f2(s, f2_pack(c.scale_log2, c.scale_log2), a);
+  return fma_f2(s, c.scale2, a);
 }
 
 // Scores of the N columns in sv, left in sv (with a bias, which the maximum
@@ -417,7 +434,7 @@ __device__ __forceinline__ void softmax_chunk(uint32_t (&sv)[N], uint32_t tS, ui
   Score cc = sc;
   cc.dist -= (float)at;
   bool small = false;
-  if constexpr (CAP) small = all_small(sv, sc);
+  if constexpr (CAP) small = all_small(sv, w, sc);
   if constexpr (BIAS) {
     if (CAP && small) score_chunk<BITS, CAP, CAP>(sv, cc);
     else score_chunk<BITS, CAP, false>(sv, cc);

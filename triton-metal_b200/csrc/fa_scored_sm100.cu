@@ -41,7 +41,6 @@ struct Params {
   int B, Hq, Hkv, Sq, Skv, q_tiles;
   int per, n_units;        // Q tiles of a unit (1 where pairs would not fill the SMs); units of a head
   attn::RangeMask range;
-  float scale_log2;
   Cap cap;
   const float* slopes;     // [Hq]
   void* o;
@@ -397,7 +396,7 @@ scored_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
     const int u = (warp - 4) >> 2, qw = warp & 3, r = qw * 32 + lane;
     const uint32_t lane_off = (uint32_t)(qw * 32) << 16;
     const uint32_t tS = tmem + 256 * u + lane_off, tO = tS + 128;
-    Score score = make_score(p.scale_log2, p.cap);
+    Score score = make_score(p.cap);
     uint32_t sc = 0, oc = 0;  // S tiles / outputs waited for
     bool ok = true;
     int next_lo = 0, next_hi = 0;
@@ -578,7 +577,6 @@ extern "C" int b2_flash_attn_fwd_scored(const void* q, const void* k, const void
       // Q-tile pairs, or single Q tiles when the pairs would not fill the SMs
       p.per = (int64_t)((p.q_tiles + 1) / 2) * Hq * B < num_sms() ? 1 : 2;
       p.n_units = (p.q_tiles + p.per - 1) / p.per;
-      p.scale_log2 = scale * attn::kLog2e;
       p.o = o;
       p.os_b = os[0];
       p.os_h = os[1];

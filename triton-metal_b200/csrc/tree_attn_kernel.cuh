@@ -83,7 +83,6 @@ struct Params {
   uint32_t page_size;           // 0: contiguous
   int max_pages;
   int box;                      // TMA: keys of a K / V box
-  float scale_log2;             // scale * log2 e
   Cap softcap;
   const float* slopes;          // BIAS: [Hq]
   unsigned* err;
@@ -194,8 +193,7 @@ __device__ __forceinline__ void draft_bits(uint32_t (&bits)[4], const uint8_t* m
 }
 
 // Visible keys among the 128 from drafted token j0 (negative: context) on, from
-// the bits of the first 128 drafted tokens.  (A row without a drafted token
-// sees the context too: its output is made 0 at the end.)
+// the bits of the first 128 drafted tokens.  
 __device__ __forceinline__ void visible_bits(uint32_t (&vis)[4], const uint32_t (&bits)[4], int j0) {
 #pragma unroll
   for (int w = 0; w < 4; ++w) {
@@ -716,7 +714,7 @@ tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
     const int u = (warp - 4) >> 2, qw = warp & 3, r = qw * 32 + lane;
     const uint32_t lane_off = (uint32_t)(qw * 32) << 16;
     const uint32_t tS = tmem + 256 * u + lane_off, tO = tmem + 128 + lane_off;  // tO: of unit 0
-    Score score = make_score(p.scale_log2, p.softcap);
+    Score score = make_score(p.softcap);
     uint32_t sc = 0, oc[2] = {0, 0}, seg = 0;  // S tiles / O accumulators waited for
     bool ok = true;
     while (walk.next(p, tokens, sg)) {
@@ -757,11 +755,12 @@ tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
               for (int w = 0; w < 4; ++w) vis[w] |= more[w];
             }
           }
-          if (!PAIR && copies > 1) {
+          // rows that are none see nothing: what stands in their place in Q's tile
+          // must neither raise a maximum nor keep the warp from the short form of
+          // the cap
 #pragma unroll
-            for (int w = 0; w < 4; ++w)
-              if (w * copies / 4 != copy) vis[w] = 0;
-          }
+          for (int w = 0; w < 4; ++w)
+            if (!row_ok || (!PAIR && w * copies / 4 != copy)) vis[w] = 0;
           // SINGLE has no way of its own for whole tiles: it doubles the code of the
           // inner loop, whose instruction fetches then set its pace (single tokens
           // with cap and bias over 1 GB of cache: 360 us with it, 284 us without)

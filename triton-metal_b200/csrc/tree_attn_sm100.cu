@@ -190,7 +190,6 @@ extern "C" int b2_tree_attn(const void* q, const void* k, const void* v, void* o
     t.n_rt = (int)n_rt;
     t.page_size = (uint32_t)page_size;
     t.max_pages = (int)max_pages;
-    t.scale_log2 = scale * attn::kLog2e;
     t.softcap = fa::make_cap(scale, softcap);
     t.err = p.err;
     t.box = tree::box_of(page_size, n_pages);
