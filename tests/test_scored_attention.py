@@ -295,6 +295,25 @@ def test_decode(cuda, qd, kd, paged, B, Hq, Hkv, S, D, cap, alibi, window):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dt,D,window", [(BF16, 64, 0), (F16, 128, 0), (F32, 64, 0), (BF16, 128, 150), (F16, 256, 0)])
+@pytest.mark.parametrize("cap", [1e-40, 1e-6, 2e3, 1e9, 3e38])
+def test_extreme_caps(cuda, dt, D, window, cap):
+    """Caps that leave nothing of the scores, and caps that none of them feels: no larger errors than without."""
+    g = torch.Generator().manual_seed(D)
+    q, k, v = (torch.randn(1, 2, 200, D, generator=g).to(dt) for _ in range(3))
+    q[:, :, 199] = 0
+    vis = scored.ranges(200, 200, True, window)
+    out = bk.flash_attention(q.to(cuda), k.to(cuda), v.to(cuda), causal=True, window=window, softcap=cap).double().cpu()
+    one = bk.decode_attention(q[:, :, 150].to(cuda), k.to(cuda), v.to(cuda), torch.tensor([200], device=cuda),
+                              softcap=cap, window=window).double().cpu()
+    for h in range(2):
+        for got, qq, vv in ((out[0, h], q[0, h], vis), (one[:, h], q[0, h, 150:151], vis[199:])):
+            o, av, mag = scored.rows(qq, k[0, h], v[0, h], vv, 1 / math.sqrt(D), cap)
+            lim = scored.bound(o, av, mag, dt, 200, D, min(cap, float(mag.max())))  # the tanh is off by 3e-7 of the score
+            assert bool(((got - o).abs() <= lim).all()), (h, ((got - o).abs() / lim).max())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dt,D", [(BF16, 128), (F16, 64)])
 @pytest.mark.parametrize("ps", [1, 4, 8, 12, 16, 32, 64, 128])
 @pytest.mark.parametrize("Hq,Hkv,cap,alibi", [(8, 8, 30.0, False), (6, 2, 0.0, True), (40, 1, 20.0, True)])

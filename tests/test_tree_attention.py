@@ -184,6 +184,23 @@ def test_tree_caps(cuda, dt, cap, big):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dt", [BF16, F32])
+@pytest.mark.parametrize("cap", [1e-40, 1e-6, 2e3, 1e9, 3e38])
+def test_tree_extreme_caps(cuda, dt, cap):
+    """Caps that leave nothing of the scores, and caps that none of them feels: no larger errors than without."""
+    gen = torch.Generator().manual_seed(11)
+    q, k, v = torch.randn(1, 6, 4, 64, generator=gen).to(dt), *(torch.randn(1, 2, 206, 64, generator=gen).to(dt) for _ in range(2))
+    q[0, 2] = 0
+    mask = _masks(1, 6, gen)[0]
+    out = bk.tree_attention(q.to(cuda), k.to(cuda), v.to(cuda), torch.tensor([200], dtype=torch.int32, device=cuda),
+                            mask.to(cuda), softcap=cap).double().cpu()
+    for h in range(4):
+        o, av, mag = scored.tree(q[0, :, h], k[0, h // 2], v[0, h // 2], 200, 6, mask, 0.125, cap)
+        lim = scored.bound(o, av, mag, dt, 206, 64, min(cap, float(mag.max())))  # the tanh is off by 3e-7 of the score
+        assert bool(((out[0, :, h] - o).abs() <= lim).all())
+
+
+@pytest.mark.gpu
 def test_tree_many_requests(cuda):
     """More requests than CTAs and than a scan's round, most of them short."""
     B = 700

@@ -70,6 +70,10 @@ __device__ __forceinline__ float tanh_acc(float x) {
   return ax < 0.35f ? small : big;
 }
 
+// A cap beyond these bounds gives the same weights in fp32 (equal ones below, the
+// uncapped scores' above), but its products would leave fp32's range.
+inline float cap_in_range(float cap) { return cap > 0.f ? (cap < 1e-30f ? 1e-30f : cap > 1e30f ? 1e30f : cap) : cap; }
+
 // Parameters of the CUDA-core kernel.  Rows of one (batch b, kv head hk) are
 // r = s * rep + hh (query position s, query head hk * rep + hh).
 struct SimtParams {

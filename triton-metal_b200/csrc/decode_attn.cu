@@ -416,9 +416,8 @@ decode_tc_kernel(const Params p) {
 
   const float sl2 = p.scale * 1.4426950408889634f;  // scores in log2 units
   const int g = lane >> 2, tq = lane & 3;
-  // SC: tanh y = 1 - 2 / (1 + e^2y), as in the prefill kernel
   const float cap_log2 = SC ? p.softcap * attn::kLog2e : 0.f;
-  const float cap_in = SC && p.softcap > 0.f ? 2.f * sl2 / p.softcap : 0.f;
+  const float cap_in = SC && p.softcap > 0.f ? fminf(p.scale / p.softcap, 1e37f) : 0.f;
   float slope0 = 0.f, slope1 = 0.f;
   if constexpr (SC) {
     if (p.slopes) {
@@ -498,7 +497,7 @@ decode_tc_kernel(const Params p) {
         const bool ok = key < s1;
         float x = s[j][e] * sl2;
         if constexpr (SC) {
-          if (p.softcap > 0.f) x = cap_log2 - 2.f * cap_log2 * __fdividef(1.f, 1.f + exp2f(s[j][e] * cap_in));
+          if (p.softcap > 0.f) x = cap_log2 * attn::tanh_acc(s[j][e] * cap_in);
           x -= (e < 2 ? slope0 : slope1) * fabsf((float)(qp - key));
         }
         s[j][e] = ok ? x : -INFINITY;
@@ -669,6 +668,7 @@ static int decode_impl(const void* q, const void* k, const void* v, void* o, con
   p.softcap = softcap;
   p.slopes = slopes;
   p.err = device_error_word();
+  B2_CHECK_ARG(p.err, B2_ERR_LAUNCH, "decode_attn: no device");
   const bool scored = softcap > 0.f || slopes;
   B2_CHECK_ARG(!rope_freqs || D % 2 == 0, B2_ERR_INVALID, "decode_attn: RoPE needs an even head dim");
   // with a window every sequence has at most `window` keys: split that
@@ -782,6 +782,7 @@ extern "C" int b2_decode_attn_scored(const void* q, const void* k, const void* v
   B2_CHECK_ARG(softcap >= 0.f && isfinite(softcap), B2_ERR_INVALID,
                "decode_attn_scored: softcap must be finite and >= 0");
   B2_CHECK_ARG(n_pages >= 0, B2_ERR_INVALID, "decode_attn_scored: bad shape");
+  softcap = attn::cap_in_range(softcap);
   if ((softcap > 0.f || alibi_slopes) && q_dtype == kv_dtype && !q_pos && window <= 0 && !rope_freqs && q && k && v && o &&
       seq_lens && k_strides && v_strides && B > 0 && Hq > 0 && Hkv > 0 && Hq % Hkv == 0 &&
       (page_size == 0 || (page_table && page_size > 0 && max_pages > 0 && max_seq_len <= page_size * max_pages))) {

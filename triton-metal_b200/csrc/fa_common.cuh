@@ -165,7 +165,7 @@ __device__ __forceinline__ uint64_t exp2_poly_f2(uint64_t x2) {
 struct Score {
   float scale_log2;        // scale * log2 e (> 0)
   float cap_in, cap_log2;  // 2 log2 e scale / cap; cap * log2 e
-  float small;             // scores up to this size take capped_small (0: none)
+  float small;             // scores up to this size take capped_small (negative: none)
   uint64_t t[5], scale2;   // its coefficients and scale_log2, each twice
   float slope, dist;       // slope * log2 e; row - first key of the tile
 };
@@ -187,8 +187,10 @@ __device__ __constant__ const float2 kKeys[32] = {
     {44, 45}, {46, 47}, {48, 49}, {50, 51}, {52, 53}, {54, 55}, {56, 57}, {58, 59}, {60, 61}, {62, 63}};
 // tanh z = z p(z^2) on [-3/4, 3/4]: this file's own minimax fit (largest error
 // 2.4e-7 in fp32).  The coefficients take scale, cap and log2 e with them, so
-// that a score s gives s q(s^2); where the powers of scale / cap would leave
-// fp32's range (scale / cap below 2e-4), the form is not used.
+// that a score s gives s q(s^2).  The powers of scale / cap have to stay in
+// fp32's range: above 1e3 the form is not used, and below 2e-4 (caps so high that
+// hardly a score feels them) only up to z = 0.05, where the first three terms
+// are enough: the other form's error, a part of the cap, would drown the scores.
 inline Cap make_cap(float scale, float softcap) {
   Cap c = {};
   auto twice = [](float x) {
@@ -198,15 +200,17 @@ inline Cap make_cap(float scale, float softcap) {
   };
   c.scale_log2 = scale * 1.4426950408889634f;
   c.scale2 = twice(c.scale_log2);
+  c.small = -1.f;
   if (softcap > 0.f) {
     const double log2e = 1.4426950408889634, z = (double)scale / softcap;
     const double p[5] = {0.9999971985816956, -0.33323076367378235, 0.13226091861724854, -0.04928044602274895,
                          0.012318830005824566};
-    c.in = (float)(2 * log2e * z);
+    c.in = (float)fmin(2 * log2e * z, 1e37);  // 0 times it is 0
     c.log2 = (float)(log2e * softcap);
-    c.small = z > 2e-4 ? (float)(0.75 / z) : 0.f;
+    if (z > 1e3) return c;
+    c.small = (float)(z > 2e-4 ? 0.75 / z : fmin(0.05 / z, 1e18));
     double f = log2e * softcap * z;
-    for (int i = 0; i < 5; ++i, f *= z * z) c.t[i] = twice((float)(p[i] * f));
+    for (int i = 0; i < (z > 2e-4 ? 5 : 3); ++i, f *= z * z) c.t[i] = twice((float)(p[i] * f));
   }
   return c;
 }
@@ -237,6 +241,10 @@ __device__ __forceinline__ uint64_t capped_small(uint64_t s, const Score& c, uin
   q = fma_f2(q, w, c.t[1]);
   q = fma_f2(q, w, c.t[0]);
   return fma_f2(s, q, add);
+}
+__device__ __forceinline__ float capped_any(float s, const Score& c, float add) {
+  if (fabsf(s) <= c.small) return f2_lo(capped_small(f2_pack(s, s), c, f2_pack(add, add)));
+  return capped(s, c, add);
 }
 // Whether all of the warp's N x 32 scores may take capped_small (w: 0 where the
 // row sees none of them).
@@ -441,7 +449,7 @@ __device__ __forceinline__ void softmax_chunk(uint32_t (&sv)[N], uint32_t tS, ui
   }
   float mx = max_chunk<BITS>(sv, w);
   if constexpr (!BIAS) {  // scale and cap keep the order
-    if constexpr (CAP) mx = mx == -INFINITY ? mx : capped(mx, sc, 0.f);
+    if constexpr (CAP) mx = mx == -INFINITY ? mx : capped_any(mx, sc, 0.f);
     else mx *= sc.scale_log2;
   }
   if (!BITS && !w) mx = -INFINITY;

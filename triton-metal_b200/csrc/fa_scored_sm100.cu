@@ -122,7 +122,7 @@ __device__ __noinline__ void again(float (&o)[32], const Row& r, int col, float 
     }
     float t = -m;
     if constexpr (BIAS) t = fmaf(-sc.slope, fabsf((float)(r.pos - key)), t);
-    const float w = ex2(CAP ? capped(s, sc, t) : fmaf(s, sc.scale_log2, t));
+    const float w = ex2(CAP ? capped_any(s, sc, t) : fmaf(s, sc.scale_log2, t));
     for (int e = 0; e < 32; ++e) o[e] = fmaf(w, widen16<FMT>(v[e]), o[e]);
   }
 }
@@ -549,6 +549,7 @@ extern "C" int b2_flash_attn_fwd_scored(const void* q, const void* k, const void
   B2_CHECK_ARG(B <= 65535 && Hq <= 65535 && Sq <= (1 << 24) && Skv <= (1 << 24), B2_ERR_UNSUPPORTED,
                "flash_attn_fwd_scored: sizes too large");
   if (Sq == 0) return B2_OK;
+  softcap = attn::cap_in_range(softcap);
   cudaStream_t st = (cudaStream_t)stream;
   attn::RangeMask range;
   range.causal = causal != 0;

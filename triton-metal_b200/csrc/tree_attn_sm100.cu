@@ -113,6 +113,7 @@ extern "C" int b2_tree_attn(const void* q, const void* k, const void* v, void* o
                "tree_attn: scale and softcap must be finite, softcap >= 0");
   B2_CHECK_ARG(mask_stride == 0 || mask_stride == T * T, B2_ERR_INVALID, "tree_attn: mask_stride must be 0 or T * T");
   if (B == 0 || T == 0) return B2_OK;
+  softcap = attn::cap_in_range(softcap);
   B2_CHECK_ARG(q && o && context_lens && tree_mask && q_strides && k_strides && v_strides && o_strides &&
                    (max_keys == 0 || (k && v)),
                B2_ERR_INVALID, "tree_attn: null pointer");
