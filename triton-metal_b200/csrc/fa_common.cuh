@@ -308,7 +308,7 @@ __device__ __forceinline__ float max_chunk(const uint32_t (&sv)[N], uint32_t w) 
 }
 
 // A tile that each of the warp's rows sees whole or not at all is gone through
-// in halves of 64 keys (two TMEM loads a wait), another one in four pieces of
+// in halves of 64 keys (WIDE; two TMEM loads a wait), another one in four pieces of
 // 32.  Of those, one that each row sees whole or not at all (and, with a bias,
 // whose keys lie on one side of the rows) takes the short way too, one that
 // nobody sees is passed over, and the rest are masked by bits.  So a document's
