@@ -168,6 +168,16 @@ def test_tree_page_sizes(cuda, dt, D, ps, T, Hq, Hkv, cap):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dt,D", [(BF16, 128), (F16, 64)])
+@pytest.mark.parametrize("ps", [0, 12, 16])
+@pytest.mark.parametrize("T,Hq,Hkv", [(1, 1, 1), (2, 6, 2), (4, 2, 1), (8, 3, 3), (1, 7, 1), (3, 3, 1)])
+@pytest.mark.parametrize("cap", [0.0, 10.0])
+def test_tree_few_rows(cuda, dt, D, ps, T, Hq, Hkv, cap):
+    """One to nine rows a group: around the eight that share a warp's lanes."""
+    _run(cuda, 4, T, Hq, Hkv, D, [0, 31, 400, 129], [T, T, T - 1, T], dt, dt, ps, cap, big=3.0)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dt", [BF16, F32])
 @pytest.mark.parametrize("T,Hq,Hkv", [(6, 3, 1), (4, 10, 2), (9, 7, 1), (3, 24, 1), (2, 40, 2), (2, 130, 1), (11, 48, 4)])
 def test_tree_head_groups(cuda, dt, T, Hq, Hkv):

@@ -4,8 +4,8 @@
 // the requests' lengths.  (The plain decode kernel gives a (request, kv head) to
 // one CTA; with lengths from 1 to 8192, 64 requests of 32 / 8 heads, its longest
 // CTAs and the cap's two MUFU operations a score took 484 us where the cache is
-// read in 164 us and this form takes 278: 250 with cap or bias alone, which the
-// 2 KB boxes of pages of 16 set, and 214 to 224 in pages of 32 keys and more.)
+// read in 164 us; this form takes 260 in pages of 16 keys, whose 2 KB boxes keep
+// the copy engine busy that long, and 212 to 230 in larger ones.)
 #include "tree_attn_kernel.cuh"
 
 namespace b2 {

@@ -527,6 +527,89 @@ __device__ __forceinline__ void softmax_tile(uint32_t tS, uint32_t tO, const uin
   }
 }
 
+// The same for a warp whose 32 rows are at most 8 (rows 0 to 7, its TMEM lanes)
+// and that takes 32 keys of the tile only, those of piece `piece` (its P is 0 for
+// the others): four lanes a row with 8 keys each, instead of 32 keys in each of a
+// few lanes.  Scores and weights change lanes through 1 KB of shared memory.  w:
+// keys that row `lane` sees; m and l: of row lane % 8, l of this lane's keys.
+template <int HD, int FMT, bool CAP, bool BIAS>
+__device__ __forceinline__ void softmax_few(uint8_t* room, uint32_t tS, uint32_t tO, int piece, uint32_t w,
+                                            const Score& sc, bool has_o, float& m, float& l) {
+  const int lane = threadIdx.x & 31, row = lane & 7, part = lane >> 3;
+  uint32_t sv[8];
+  {
+    uint32_t all[32];
+    tc::tmem_ld_32x32b_x32(tS + 32 * piece, all);
+    tc::tmem_ld_wait();
+    __syncwarp();  // the tile before is read
+    if (lane < 8) {
+#pragma unroll
+      for (int c = 0; c < 8; ++c)
+        *reinterpret_cast<uint4*>(room + row * 128 + ((c ^ row) << 4)) =
+            make_uint4(all[4 * c], all[4 * c + 1], all[4 * c + 2], all[4 * c + 3]);
+    }
+  }
+  __syncwarp();
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    const uint4 x = *reinterpret_cast<const uint4*>(room + row * 128 + (((2 * part + c) ^ row) << 4));
+    sv[4 * c] = x.x;
+    sv[4 * c + 1] = x.y;
+    sv[4 * c + 2] = x.z;
+    sv[4 * c + 3] = x.w;
+  }
+  const uint32_t bits = __shfl_sync(0xffffffffu, w, row) >> (8 * part) & 0xffu;
+  Score cc = sc;
+  cc.dist -= (float)(32 * piece + 8 * part);
+  bool small = false;
+  if constexpr (CAP) small = all_small(sv, bits, sc);
+  if constexpr (BIAS) {
+    cc.slope = __shfl_sync(0xffffffffu, sc.slope, row);
+    if (CAP && small) score_chunk<false, CAP, CAP>(sv, cc);
+    else score_chunk<false, CAP, false>(sv, cc);
+  }
+  float mx = max_chunk<true>(sv, bits);
+  if constexpr (!BIAS) {
+    if constexpr (CAP) mx = mx == -INFINITY ? mx : capped_any(mx, sc, 0.f);
+    else mx *= sc.scale_log2;
+  }
+  mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+  mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+  const bool need = mx > m + kRescale;
+  if (__any_sync(0xffffffffu, need)) {  // as in softmax_chunk
+    const float up = ceilf(mx - m);
+    const float alpha = need ? pow2_down(-up) : 1.f;
+    if (need) {
+      l *= alpha;
+      m = m == -INFINITY ? mx : m + up;
+    }
+    rescale<HD, FMT>(tO, 0, has_o, 0, 0, alpha);
+  }
+  const float mref = m == -INFINITY ? 0.f : m;
+  uint32_t pk[4];
+  if (CAP && !BIAS && small) l += exp_chunk<true, FMT, CAP, BIAS, CAP && !BIAS>(sv, pk, bits, cc, mref);
+  else l += exp_chunk<true, FMT, CAP, BIAS, false>(sv, pk, bits, cc, mref);
+  __syncwarp();  // the scores are read
+  *reinterpret_cast<uint4*>(room + row * 64 + ((part ^ (row >> 1 & 3)) << 4)) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+  __syncwarp();
+  uint32_t p[16];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    const uint4 x = *reinterpret_cast<const uint4*>(room + row * 64 + ((c ^ (row >> 1 & 3)) << 4));
+    p[4 * c] = lane < 8 ? x.x : 0;
+    p[4 * c + 1] = lane < 8 ? x.y : 0;
+    p[4 * c + 2] = lane < 8 ? x.z : 0;
+    p[4 * c + 3] = lane < 8 ? x.w : 0;
+  }
+  uint32_t zero[16];
+#pragma unroll
+  for (int e = 0; e < 16; ++e) zero[e] = 0;
+#pragma unroll 1
+  for (int c = 0; c < 4; ++c)
+    if (c != piece) tmem_st_32x32b_x16(tS + p_column(BIAS) + 16 * c, zero);
+  tmem_st_32x32b_x16(tS + p_column(BIAS) + 16 * piece, p);
+}
+
 template <int FMT>
 __device__ __forceinline__ bool not_finite16(uint32_t h) {  // of the low half
   constexpr uint32_t e = FMT == kF16 ? 0x7C00u : 0x7F80u;

@@ -582,7 +582,8 @@ extern "C" int b2_flash_attn_fwd_scored(const void* q, const void* k, const void
       p.Sq = (int)Sq;
       p.Skv = (int)Skv;
       p.q_tiles = (int)((Sq + fa::BQ - 1) / fa::BQ);
-      // Q-tile pairs, or single Q tiles when the pairs would not fill the SMs
+      // Q-tile pairs, or single Q tiles when the pairs would not fill the SMs (causal,
+      // cap, 8 heads of 128: 1024 tokens 35 us against 41 in pairs, 2048 55 against 65)
       p.per = (int64_t)((p.q_tiles + 1) / 2) * Hq * B < num_sms() ? 1 : 2;
       p.n_units = (p.q_tiles + p.per - 1) / p.per;
       p.o = o;

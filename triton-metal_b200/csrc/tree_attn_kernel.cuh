@@ -21,8 +21,8 @@
 //               K0 K1 V0 K2 V1 ...; a box is as many keys as divide a page and a
 //               tile.  Pages of 16 keys need eight boxes of 2 KB for 16 KB; with
 //               V copied by two warps instead, so that the copy engine had half
-//               the boxes, 48 requests of 16 heads over 4 to 8 thousand keys took
-//               365 us, not 282.
+//               the boxes, single tokens of 64 requests (32 / 8 heads of 128, up to
+//               8192 keys, cap and bias) took 365 us, not 282.
 //   warp 1      TMEM owner and MMA issuer
 //   warps 2-3   pass the tiles on; in V tiles with drafted tokens they zero the
 //               rows behind the last key and what is infinite or NaN
@@ -43,7 +43,7 @@
 // Measured: trees of 64, 32 requests of 8 to 32 thousand keys, 32 / 8 heads of
 // 128, bf16: 0.88 ms, 3.1 TB/s and 780 TF/s (either floor is 0.42 ms; the softmax
 // between a tile's two MMAs sets the time); trees of 26, 16 requests of up to
-// 4096 keys in pages of 16, fp16: 55 us, 2.6 TB/s (starts and ends of segments);
+// 4096 keys in pages of 16, fp16: 56 us, 2.6 TB/s (starts and ends of segments);
 // a tree of 8, one request of 500 keys: 19 us (two launches and one chain).
 #pragma once
 #include "attn_common.cuh"
@@ -58,7 +58,9 @@ using namespace fa;
 constexpr int kThreads = 384;
 constexpr int kCopyRows = 44;              // cp.async form: rows of a copying warp (the third: 40)
 constexpr int BR = 128, BK = 128;          // rows and keys of a tile
-constexpr int kItemCost = 2;               // what starting and ending an item costs, in tiles
+// What starting and ending an item costs, in tiles (0 instead of 2: trees of 26
+// over 16 requests 67 us, not 56; single tokens of 64 requests 307 us, not 260).
+constexpr int kItemCost = 2;
 
 template <int HD>
 struct Cfg {
@@ -743,6 +745,11 @@ tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
       float m_used = -INFINITY, l = 0.f;
       bool first = true;
       const int step = PAIR ? 1 : 2;
+      // at most 8 rows, each in a lane of its own in every warp (copies == 4): single
+      // tokens with cap and bias in pages of 32 take 222 us this way, 278 the other
+      const bool few = !PAIR && p.T * p.rep <= 8;
+      // rows 8 to 23 of a copy's place in Q's tile are none
+      uint8_t* room = sQ + (seg & 1) * C::kTile + (qw * 32 + 8 + 8 * u) * 128;
       for (int j = PAIR ? (u < units ? 0 : sg.n) : u; j < sg.n && ok; j += step) {
         ok = __all_sync(0xffffffffu, wait_abort(&s_full[u], sc & 1, p.err, 0xB2400009u, abort_flag));
         ++sc;
@@ -772,7 +779,8 @@ tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
           const bool whole = PAIR && whole_tile(vis);
           // single tokens only: every visible key is at or before the row's own
           if constexpr (BIAS) score.dist = (float)(sg.ctx - kv0);
-          softmax_tile<PAIR, HD, FMT, CAP, BIAS>(tS, tO + 256 * u, vis, whole, true, score, !first, m_used, l);
+          if (few) softmax_few<HD, FMT, CAP, BIAS>(room, tS, tO + 256 * u, qw, word_of(vis, qw), score, !first, m_used, l);
+          else softmax_tile<PAIR, HD, FMT, CAP, BIAS>(tS, tO + 256 * u, vis, whole, true, score, !first, m_used, l);
           tmem_st_wait();
         }
         first = false;
@@ -783,6 +791,14 @@ tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
       // ------------------------------ segment end ------------------------------
       // This thread writes row r: SINGLE, columns of half u from both units'
       // accumulators; PAIR, all columns of its own.
+      if (few) {  // each row's sums to the thread that has it
+        l += __shfl_xor_sync(0xffffffffu, l, 8);
+        l += __shfl_xor_sync(0xffffffffu, l, 16);
+        if (lane >= 8) {
+          m_used = -INFINITY;
+          l = 0.f;
+        }
+      }
       float M = m_used, L = l, f0 = 1.f, f1 = 0.f;
       if constexpr (!PAIR) {
         s_ml[u * 128 + r] = make_float2(m_used, l);
@@ -1095,7 +1111,8 @@ static void launch(const Maps& m, const Params& p, cudaStream_t st) {
 }
 
 // Copies of the rows in a tile: as many as fit.  (64 requests of up to 8192 keys,
-// four rows each, cap and bias: 296 us with one copy, 283 with four.)
+// four rows each, cap and bias, all by softmax_tile: 296 us with one copy, 283
+// with four.)
 inline int copies_of(int64_t rows) { return rows <= 32 ? 4 : rows <= 64 ? 2 : 1; }
 
 // Launches by what the call has (BIAS: p.slopes, CAP: p.softcap).
