@@ -1,6 +1,6 @@
 """Oracle for attention with masks, capped and biased scores (torch, float64).
 
-TEST INFRASTRUCTURE ONLY: imported by tests/ as the checker.  Never the
+TEST INFRASTRUCTURE ONLY: imported by tests/ for the right values.  Never the
 product.  The definition, one (request, head) at a time:
 
   s_ij = cap tanh(scale q_i.k_j / cap) + bias_ij      (cap 0: scale q_i.k_j)

@@ -69,7 +69,7 @@ struct Cfg {
   static constexpr int kRing = HD == 128 ? 5 : 10;    // 160 KB of K and V tiles
   // tiles a copying thread leaves in flight behind the one it hands over
   static constexpr int kLag = HD == 128 ? 2 : 4;
-  static constexpr int kHead = 3072;                  // barriers and the (m, l) exchange
+  static constexpr int kHead = 3 * 1024;                 // barriers and the (m, l) exchange
   static constexpr int kSmem = kHead + (2 + kRing) * kTile;
   static_assert(kSmem <= 232448, "shared memory");
   static_assert(kLag < kRing, "a ring slot is handed over before it is waited for again");
