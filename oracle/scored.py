@@ -71,3 +71,14 @@ def bound(o, av, mag, dtype, keys, D, cap=0.0, dist=0.0):
     serr = (D + 4) * 2.0 ** -24 * mag + cap * 3e-7 + dist * 2.0 ** -23
     weights = (keys + 16) * 2.0 ** -24 + (half + 1e-4 if dtype != torch.float32 else 0.0)
     return half * o.abs() + av * (2 * serr + weights) + 1e-30
+
+
+def growing(B, T, Hq, Hkv, S, D, dtype, gen, down=False):
+    """q [B, T, Hq, D], k and v [B, Hkv, S, D] whose scores (scale D^-1/2) rise by 6 to 9 (8.6 to 13 in log2) with every
+    32 keys, towards the last key, or with ``down`` towards the first; each row at its own rate."""
+    q = (1.0 + torch.arange(T)[:, None] % 3 / 4).expand(T, Hq)[None, ..., None].expand(B, T, Hq, D)
+    step = torch.arange(S) // 32
+    step = step.flip(0) if down else step
+    k = (6.0 / D ** 0.5 * step)[None, None, :, None].expand(B, Hkv, S, D) + torch.randn(B, Hkv, S, D, generator=gen) / 16
+    v = torch.randn(B, Hkv, S, D, generator=gen)
+    return q.to(dtype).contiguous(), k.to(dtype), v.to(dtype)

@@ -399,3 +399,31 @@ def test_scored_no_bounded_wait_ran_out(cuda):
     code = ctypes.c_uint(0)
     st = _lib.load().b2_device_error(torch.cuda.current_stream().cuda_stream, ctypes.byref(code))
     assert st == 0 and code.value == 0, hex(code.value)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt,D", [(BF16, 128), (F16, 64)])
+@pytest.mark.parametrize("S", [300, 513])
+@pytest.mark.parametrize("alibi", [False, True])
+def test_growing_maximum(cuda, dt, D, S, alibi):
+    """Scores that rise by more than the rescaling threshold (8 in log2) with every 32 keys, in the order in which the
+    keys are taken (a bias takes them from the last one back): O is rescaled several times within a tile, in pieces of
+    32 keys and in halves of 64.  Prompts, and single tokens with 2, 12 and 40 rows a kv head."""
+    g = torch.Generator().manual_seed(S)
+    q, k, v = scored.growing(1, S, 4, 2, S, D, dt, g, down=alibi)
+    q = q.transpose(1, 2).contiguous()
+    slopes = _slopes(4) / 64 if alibi else None
+    docs = torch.tensor([[0, 70, S - 3]], dtype=torch.int32)
+    for kw in (dict(docs=docs), dict(docs=docs, causal=True), dict(causal=True, window=200), dict(prefix=torch.tensor(
+            [260], dtype=torch.int32), causal=True)):
+        _check_flash(cuda, q, k, v, slopes=slopes, **kw)
+    for rep in (2, 12, 40):
+        q1, k, v = scored.growing(1, 3, 2 * rep, 2, S, D, dt, g, down=alibi)
+        sl = _slopes(2 * rep) / 64 if alibi else torch.zeros(2 * rep)
+        out = bk.decode_attention(q1[:, 2].to(cuda), k.to(cuda), v.to(cuda), torch.tensor([S], dtype=torch.int32, device=cuda),
+                                  alibi_slopes=sl.to(cuda)).double().cpu()
+        for h in range(2 * rep):
+            bias = -sl[h].double() * (S - 1 - torch.arange(S).double())[None]
+            o, av, mag = scored.rows(q1[0, 2, h:h + 1], k[0, h // rep], v[0, h // rep], torch.ones(1, S, dtype=torch.bool),
+                                     1 / math.sqrt(D), 0.0, bias)
+            assert bool(((out[0, h] - o[0]).abs() <= scored.bound(o, av, mag, dt, S, D, 0.0, float(sl[h]) * S)[0]).all()), (rep, h)

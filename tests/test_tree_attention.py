@@ -390,3 +390,23 @@ def test_tree_no_bounded_wait_ran_out(cuda):
     code = ctypes.c_uint(0)
     st = _lib.load().b2_device_error(torch.cuda.current_stream().cuda_stream, ctypes.byref(code))
     assert st == 0 and code.value == 0, hex(code.value)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt,D", [(BF16, 128), (F16, 64)])
+@pytest.mark.parametrize("T,Hq,Hkv", [(2, 4, 1), (12, 8, 2), (25, 4, 1), (80, 4, 2)])
+@pytest.mark.parametrize("ps", [0, 12, 16])
+def test_tree_growing_maximum(cuda, dt, D, T, Hq, Hkv, ps):
+    """Scores that rise by more than the rescaling threshold (8 in log2) with every 32 keys: O is rescaled several times
+    within a tile."""
+    gen = torch.Generator().manual_seed(T)
+    ctx, B = 500, 1
+    q, k, v = scored.growing(B, T, Hq, Hkv, ctx + T, D, dt, gen)
+    mask = torch.tril(torch.ones(T, T, dtype=torch.bool))
+    kc, vc, table = k, v, None
+    if ps:
+        kc, vc, table = _paged(k, v, ps, gen)
+        table = table.to(cuda)
+    out = bk.tree_attention(q.to(cuda), kc.to(cuda), vc.to(cuda), torch.tensor([ctx], dtype=torch.int32, device=cuda),
+                            mask.to(cuda), page_table=table)
+    _check(out, q, k, v, [ctx], [T], mask, 1 / math.sqrt(D), 0.0, dt)

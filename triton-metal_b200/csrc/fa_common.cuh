@@ -390,9 +390,11 @@ __device__ __forceinline__ uint32_t narrow2(float a, float b) {
 
 // The running maximum has grown: O (HD columns, if there is one yet) and the P
 // of the keys [from, to), which this tile has stored already, are brought to the
-// new one.
+// new one.  Both may still be on their way to TMEM, O from an earlier rescaling of
+// the same tile, and nothing orders a load behind a store but the wait.
 template <int HD, int FMT>
 __device__ __forceinline__ void rescale(uint32_t tO, uint32_t tP, bool has_o, int from, int to, float alpha) {
+  tmem_st_wait();
   if (has_o) {
 #pragma unroll 1
     for (int c = 0; c < HD / 32; ++c) {
@@ -405,7 +407,6 @@ __device__ __forceinline__ void rescale(uint32_t tO, uint32_t tP, bool has_o, in
     }
   }
   if (from < to) {
-    tmem_st_wait();
 #pragma unroll 1
     for (int c = from / 32; c < to / 32; ++c) {
       uint32_t x[16];
