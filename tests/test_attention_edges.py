@@ -1,0 +1,107 @@
+"""Values at the edges of the capped, biased and tree attention: slopes of either
+sign.  Against the float64 oracle, within the bound that oracle/scored.py
+derives."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+import b200kern as bk
+from b200kern import _lib
+from oracle import scored
+
+F16, BF16, F32 = torch.float16, torch.bfloat16, torch.float32
+
+
+def _rand(g, *shape, dt=F32, big=1.0):
+    return (torch.randn(*shape, generator=g) * big).to(dt)
+
+
+def _i32(a, dev):
+    return torch.tensor(a, dtype=torch.int32, device=dev)
+
+
+def _pages(k, v, ps, gen):
+    """A contiguous cache [B, Hkv, S, D] as shuffled pages and their table."""
+    B, Hkv, S, D = k.shape
+    width = -(-S // ps)
+    table = torch.randperm(B * width, generator=gen).reshape(B, width).to(torch.int32)
+    out = []
+    for x in (k, v):
+        pad = torch.zeros(B, Hkv, width * ps, D, dtype=x.dtype)
+        pad[:, :, :S] = x
+        p = torch.empty(B * width, ps, Hkv, D, dtype=x.dtype)
+        p[table.reshape(-1).long()] = pad.view(B, Hkv, width, ps, D).permute(0, 2, 3, 1, 4).reshape(-1, ps, Hkv, D)
+        out.append(p)
+    return out[0], out[1], table
+
+
+# ----------------------------------------------------------- slopes
+def _signed(h):
+    """Slopes of both signs, up to 1/2."""
+    return torch.tensor([(-1.0) ** i * 2.0 ** (-1.0 - 5.0 * i / h) for i in range(h)], dtype=F32)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt,D", [(BF16, 128), (F16, 64), (F32, 64), (BF16, 80)])
+@pytest.mark.parametrize("causal,docs,prefix,cap", [(True, None, None, 0.0), (False, None, None, 0.0),
+                                                    (True, [0, 130, 140, 290], None, 0.0),
+                                                    (False, [20, 150, 300], None, 20.0), (True, None, 170, 20.0)])
+def test_prompt_slopes_of_either_sign(cuda, dt, D, causal, docs, prefix, cap):
+    """s - slope |i - j| for any sign of the slope, on the diagonal, at documents' ends and between them."""
+    g = torch.Generator().manual_seed(D)
+    Hq, Hkv, S = 6, 3, 300
+    q, k, v = _rand(g, 1, Hq, S, D, dt=dt, big=3.0), _rand(g, 1, Hkv, S, D, dt=dt), _rand(g, 1, Hkv, S, D, dt=dt)
+    sl = _signed(Hq)
+    out = bk.flash_attention(q.to(cuda), k.to(cuda), v.to(cuda), causal=causal, softcap=cap, alibi_slopes=sl.to(cuda),
+                             doc_offsets=None if docs is None else _i32([docs], cuda),
+                             prefix_lens=None if prefix is None else _i32([prefix], cuda)).double().cpu()
+    vis = scored.ranges(S, S, causal, 0, docs, None if prefix is None else [prefix])
+    far = (torch.arange(S).double()[:, None] - torch.arange(S).double()).abs()
+    for h in range(Hq):
+        o, av, mag = scored.rows(q[0, h], k[0, h // 2], v[0, h // 2], vis, 1 / math.sqrt(D), cap, -sl[h].double() * far)
+        lim = scored.bound(o, av, mag, dt, S, D, cap, abs(float(sl[h])) * S)
+        err = (out[0, h] - o).abs()
+        assert bool((err <= lim).all()), f"h={h}: {(err / lim).max():.3g} of the bound"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt,D", [(BF16, 128), (F16, 64), (F32, 64), (F16, 256)])
+@pytest.mark.parametrize("rep", [1, 4, 12, 16])
+@pytest.mark.parametrize("ps", [0, 16, 24])
+def test_token_slopes_of_either_sign(cuda, dt, D, rep, ps):
+    _token_slopes(cuda, dt, D, rep, ps)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt,D", [(BF16, 128), (F16, 64)])
+@pytest.mark.parametrize("rep", [40, 100])
+def test_token_slopes_of_either_sign_many_heads(cuda, dt, D, rep):
+    _token_slopes(cuda, dt, D, rep, 16)
+
+
+def _token_slopes(cuda, dt, D, rep, ps):
+    g = torch.Generator().manual_seed(rep + D)
+    lens = [300, 1, 129]
+    B, Hkv, S = len(lens), 2, max(lens)
+    Hq = rep * Hkv
+    q, k, v = _rand(g, B, Hq, D, dt=dt, big=3.0), _rand(g, B, Hkv, S, D, dt=dt), _rand(g, B, Hkv, S, D, dt=dt)
+    kc, vc, table = (k, v, None) if not ps else _pages(k, v, ps, g)
+    sl = _signed(Hq)
+    out = bk.decode_attention(q.to(cuda), kc.to(cuda), vc.to(cuda), _i32(lens, cuda), alibi_slopes=sl.to(cuda),
+                              page_table=None if table is None else table.to(cuda)).double().cpu()
+    for b, n in enumerate(lens):
+        far = (n - 1 - torch.arange(n).double())[None]
+        for h in range(Hq):
+            o, av, mag = scored.rows(q[b, h:h + 1], k[b, h // rep, :n], v[b, h // rep, :n],
+                                     torch.ones(1, n, dtype=torch.bool), 1 / math.sqrt(D), 0.0, -sl[h].double() * far)
+            lim = scored.bound(o, av, mag, dt, n, D, 0.0, abs(float(sl[h])) * n)
+            assert bool(((out[b, h] - o[0]).abs() <= lim[0]).all()), (b, h)
+
+
+@pytest.mark.gpu
+def test_edges_no_bounded_wait_ran_out(cuda):
+    code = ctypes.c_uint(0)
+    st = _lib.load().b2_device_error(torch.cuda.current_stream().cuda_stream, ctypes.byref(code))
+    assert st == 0 and code.value == 0, hex(code.value)

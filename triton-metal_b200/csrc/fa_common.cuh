@@ -167,7 +167,8 @@ struct Score {
   float cap_in, cap_log2;  // 2 log2 e scale / cap; cap * log2 e
   float small;             // scores up to this size take capped_small (negative: none)
   uint64_t t[5], scale2;   // its coefficients and scale_log2, each twice
-  float slope, dist;       // slope * log2 e; row - first key of the tile
+  float slope, dist;       // slope * log2 e (score_pair: with a side's sign); row - first key of the tile
+  float slope0;            // slope * log2 e as given, of either sign
 };
 
 // What a kernel's parameters hold of it.  The operands of the paired instructions
@@ -178,7 +179,7 @@ struct Cap {
   uint64_t t[5], scale2;
 };
 __device__ __forceinline__ Score make_score(const Cap& c) {
-  return {c.scale_log2, c.in, c.log2, c.small, {c.t[0], c.t[1], c.t[2], c.t[3], c.t[4]}, c.scale2, 0.f, 0.f};
+  return {c.scale_log2, c.in, c.log2, c.small, {c.t[0], c.t[1], c.t[2], c.t[3], c.t[4]}, c.scale2, 0.f, 0.f, 0.f};
 }
 // key numbers of a piece, for the distance bias
 __device__ __constant__ const float2 kKeys[32] = {
@@ -258,14 +259,14 @@ __device__ __forceinline__ bool all_small(const uint32_t (&sv)[N], uint32_t w, c
 
 // Score of two neighbouring keys (e and e + 1 from where c.dist counts), plus
 // `add`.  ABS: keys on both sides of the row.  Otherwise all keys of the tile
-// lie on one side, the bias is linear in the key and slope carries its sign
-// (slope > 0: keys before the row).
+// lie on one side, the bias is linear in the key and c.slope is the slope where
+// they are before the row, minus the slope where they are behind it.
 template <bool ABS, bool CAP, bool BIAS, bool SMALL>
 __device__ __forceinline__ uint64_t score_pair(uint32_t s0, uint32_t s1, int e, const Score& c, float add) {
   uint64_t a = f2_pack(add, add);
   if constexpr (BIAS) {
     if constexpr (ABS) {
-      const float sl = -fabsf(c.slope);
+      const float sl = -c.slope0;
       a = f2_pack(fmaf(sl, fabsf(c.dist - (float)e), add), fmaf(sl, fabsf(c.dist - (float)(e + 1)), add));
     } else {
       const float b = fmaf(-c.slope, c.dist, add);

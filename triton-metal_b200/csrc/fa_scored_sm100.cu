@@ -128,7 +128,7 @@ __device__ __noinline__ void again(float (&o)[32], const Row& r, int col, float 
       }
     }
     float t = -m;
-    if constexpr (BIAS) t = fmaf(-sc.slope, fabsf((float)(r.pos - key)), t);
+    if constexpr (BIAS) t = fmaf(-sc.slope0, fabsf((float)(r.pos - key)), t);
     const float w = ex2(CAP ? capped_any(s, sc, t) : fmaf(s, sc.scale_log2, t));
     for (int e = 0; e < 32; ++e) o[e] = fmaf(w, widen16<FMT>(v[e]), o[e]);
   }
@@ -418,8 +418,7 @@ scored_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
       const int q0 = un.q0 + u * BQ, qpos = q0 + r;
       const bool exists = u < p.per && qpos < p.Sq;
       const int row_lo = next_lo, row_hi = next_hi;
-      float slope = 0.f;
-      if constexpr (BIAS) slope = p.slopes[un.h] * attn::kLog2e;
+      if constexpr (BIAS) score.slope0 = p.slopes[un.h] * attn::kLog2e;
       ok = __all_sync(0xffffffffu, wait_abort(&info_full[k & 1], (k >> 1) & 1, p.err, 0xB260000Eu, abort_flag));
       if (!ok) break;
       read_info(k, f);
@@ -438,7 +437,7 @@ scored_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
         const bool one_side = kv0 + BKV - 1 <= q0 || kv0 >= q0 + BQ - 1;  // where the tile's rows are not in it
         if constexpr (BIAS) {
           score.dist = (float)(qpos - kv0);
-          score.slope = kv0 <= q0 ? slope : -slope;
+          score.slope = kv0 <= q0 ? score.slope0 : -score.slope0;
         }
         uint32_t vis[4] = {~0u, ~0u, ~0u, ~0u};
         if (f.masked(u, tile_of(j))) range_bits(vis, row_lo, row_hi, kv0);
@@ -479,7 +478,6 @@ scored_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
             const Row rw = {p.q + un.b * p.qs[0] + un.h * p.qs[1] + (int64_t)qpos * p.qs[2],
                             p.k + un.b * p.ks[0] + hk * p.ks[1], p.v + un.b * p.vs[0] + hk * p.vs[1], p.ks[2], p.vs[2],
                             row_lo, row_hi, qpos};
-            score.slope = slope;
             float t[32];  // not o itself: that would have to live in local memory
             again<HD, FMT, CAP, BIAS>(t, rw, 32 * c, m_used, score);
 #pragma unroll

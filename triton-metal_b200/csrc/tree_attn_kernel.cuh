@@ -736,7 +736,7 @@ tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
       const int t0 = rt * p.tpt + w0 / p.rep, t1 = min(rt * p.tpt + min((w0 + 31) / p.rep, p.tpt - 1), sg.dl - 1);
       const bool warp_ok = t0 < sg.dl && w0 < br, warp_in = t0 < p.T && w0 < br;
       const uint8_t* mask = p.mask ? p.mask + sg.b * p.mask_stride : nullptr;
-      if constexpr (BIAS) score.slope = row_in ? p.slopes[head] * attn::kLog2e : 0.f;
+      if constexpr (BIAS) score.slope0 = score.slope = row_in ? p.slopes[head] * attn::kLog2e : 0.f;
       // mask bits of the first 128 drafted tokens, read while the first keys are
       // still on their way (wider trees read theirs tile by tile)
       uint32_t drafted[4] = {0, 0, 0, 0};
