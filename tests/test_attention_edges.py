@@ -8,7 +8,7 @@ import pytest
 import torch
 
 import b200kern as bk
-from b200kern import _lib
+from b200kern import _lib, errors
 from oracle import scored
 
 F16, BF16, F32 = torch.float16, torch.bfloat16, torch.float32
@@ -35,6 +35,41 @@ def _pages(k, v, ps, gen):
         p[table.reshape(-1).long()] = pad.view(B, Hkv, width, ps, D).permute(0, 2, 3, 1, 4).reshape(-1, ps, Hkv, D)
         out.append(p)
     return out[0], out[1], table
+
+
+# --------------------------------------------------------- refusals
+class _Cuda(torch.Tensor):
+    """A CPU tensor that says it is on a GPU, to reach the checks behind the device's."""
+    is_cuda = True
+
+
+def _on_gpu(*shape, dtype=F16):
+    return torch.zeros(*shape, dtype=dtype).as_subclass(_Cuda)
+
+
+@pytest.mark.parametrize("k,v,table", [
+    ((2, 2, 8, 64), (2, 2, 9, 64), None), ((2, 2, 8, 64), (2, 1, 8, 64), None),  # caches of two shapes
+    ((2, 2, 8, 32), (2, 2, 8, 32), None), ((2, 2, 8, 128), (2, 2, 8, 128), None),  # another head dim
+    ((1, 2, 8, 64), (1, 2, 8, 64), None),                                          # fewer requests than q
+    ((2, 8, 64), (2, 8, 64), None), ((2, 0, 8, 64), (2, 0, 8, 64), None),
+    ((5, 16, 2, 64), (4, 16, 2, 64), (2, 3)),                                      # V has fewer pages
+    ((5, 16, 2, 64), (5, 16, 2, 64), (1, 3)), ((5, 16, 2, 64), (5, 16, 2, 64), (6,)),
+    ((5, 16, 2, 48), (5, 16, 2, 48), (2, 3))])
+@pytest.mark.parametrize("cap", [0.0, 5.0])
+def test_decode_attention_refuses_shapes(k, v, table, cap):
+    table = None if table is None else torch.zeros(table, dtype=torch.int32)
+    with pytest.raises(errors.B2ShapeError):
+        bk.decode_attention(_on_gpu(2, 4, 64), _on_gpu(*k), _on_gpu(*v), [1, 2], page_table=table, softcap=cap)
+
+
+def test_decode_attention_refuses_other_devices():
+    other = lambda *s: torch.zeros(*s, dtype=F16, device="meta").as_subclass(_Cuda)
+    mine = _on_gpu(2, 2, 8, 64)
+    for k, v in ((other(2, 2, 8, 64), mine), (mine, other(2, 2, 8, 64))):
+        with pytest.raises(errors.B2ShapeError, match="meta"):
+            bk.decode_attention(_on_gpu(2, 4, 64), k, v, [1, 2])
+    with pytest.raises(errors.B2ShapeError, match="meta"):
+        bk.decode_attention(_on_gpu(2, 4, 64), mine, mine, [1, 2], out=other(2, 4, 64))
 
 
 # ----------------------------------------------------------- slopes

@@ -197,31 +197,35 @@ def decode_attention(q, k_cache, v_cache, seq_lens, scale=None, page_table=None,
     if q.dtype not in _DT or k_cache.dtype not in _DT or v_cache.dtype != k_cache.dtype:
         raise B2DtypeError("q and the cache must be fp32, fp16 or bf16")
     B, Hq, D = q.shape
+    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape or k_cache.shape[3] != D:
+        raise B2ShapeError(f"k_cache and v_cache must be 4-d of one shape with head dim {D}, got "
+                           f"{tuple(k_cache.shape)} and {tuple(v_cache.shape)}")
+    _lib.check_device(q, k_cache=k_cache, v_cache=v_cache, out=out)
     if k_cache.stride(-1) != 1:
         k_cache = k_cache.contiguous()
     if v_cache.stride(-1) != 1:
         v_cache = v_cache.contiguous()
     if page_table is None:
+        if k_cache.shape[0] < B:
+            raise B2ShapeError(f"a contiguous cache must hold {B} requests, got {k_cache.shape[0]}")
         Hkv, S = k_cache.shape[1], k_cache.shape[2]
         ks, vs = k_cache.stride()[:3], v_cache.stride()[:3]
         ps, max_pages, pt = 0, 0, None
     else:
+        if page_table.dim() != 2 or page_table.shape[0] < B:
+            raise B2ShapeError(f"page_table must be [{B}, max_pages], got {tuple(page_table.shape)}")
         ps, Hkv = k_cache.shape[1], k_cache.shape[2]
         pt = page_table.to(device=q.device, dtype=torch.int32).contiguous()
         max_pages = pt.shape[1]
         S = max_pages * ps
         ks, vs = k_cache.stride()[:3], v_cache.stride()[:3]
-    if Hq % Hkv:
+    if Hkv == 0 or Hq % Hkv:
         raise B2ShapeError(f"Hq={Hq} must be a multiple of Hkv={Hkv}")
     lens = _seq_lens(seq_lens, B, q.device)
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
     q = q.contiguous()
     o = (_lib.check_out(out, (B, Hq, D), q.dtype, "decode_attention") if out is not None
          else torch.empty(B, Hq, D, dtype=q.dtype, device=q.device))
-    scored = softcap or alibi_slopes is not None
-    need = int(_lib.fn("b2_decode_attn_scored_workspace_size" if scored else "b2_decode_attn_workspace_size")(
-        B, Hq, Hkv, D, S))
-    ws = torch.empty(max(need, 1), dtype=torch.uint8, device=q.device)
     qp = None if q_pos is None else _seq_lens(q_pos, B, q.device)
     fr = None
     if rope_freqs is not None:
@@ -230,12 +234,15 @@ def decode_attention(q, k_cache, v_cache, seq_lens, scale=None, page_table=None,
             raise B2ShapeError(f"rope_freqs must have D/2 = {D // 2} entries")
     slopes = _score_args(Hq, q.device, softcap, alibi_slopes)
     n_pages = k_cache.shape[0] if pt is not None else 0
-    _lib.call("b2_decode_attn_scored", q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), o.data_ptr(),
-              None if pt is None else pt.data_ptr(), lens.data_ptr(), ws.data_ptr(), B, Hq, Hkv, D, S, ps,
-              max_pages, n_pages, _lib.strides_arg(ks), _lib.strides_arg(vs), None if qp is None else qp.data_ptr(),
-              int(window), None if fr is None else fr.data_ptr(), scale, float(softcap),
-              None if slopes is None else slopes.data_ptr(), _DT[q.dtype], _DT[k_cache.dtype],
-              _stream())
+    with _lib.on_device(q):
+        size = "b2_decode_attn_scored_workspace_size" if softcap or slopes is not None else "b2_decode_attn_workspace_size"
+        ws = torch.empty(max(int(_lib.fn(size)(B, Hq, Hkv, D, S)), 1), dtype=torch.uint8, device=q.device)
+        _lib.call("b2_decode_attn_scored", q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), o.data_ptr(),
+                  None if pt is None else pt.data_ptr(), lens.data_ptr(), ws.data_ptr(), B, Hq, Hkv, D, S, ps,
+                  max_pages, n_pages, _lib.strides_arg(ks), _lib.strides_arg(vs),
+                  None if qp is None else qp.data_ptr(), int(window), None if fr is None else fr.data_ptr(), scale,
+                  float(softcap), None if slopes is None else slopes.data_ptr(), _DT[q.dtype], _DT[k_cache.dtype],
+                  _stream())
     return o
 
 
