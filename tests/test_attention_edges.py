@@ -8,7 +8,7 @@ import pytest
 import torch
 
 import b200kern as bk
-from b200kern import _lib, errors
+from b200kern import _lib, attention, errors
 from oracle import scored
 
 F16, BF16, F32 = torch.float16, torch.bfloat16, torch.float32
@@ -70,6 +70,37 @@ def test_decode_attention_refuses_other_devices():
             bk.decode_attention(_on_gpu(2, 4, 64), k, v, [1, 2])
     with pytest.raises(errors.B2ShapeError, match="meta"):
         bk.decode_attention(_on_gpu(2, 4, 64), mine, mine, [1, 2], out=other(2, 4, 64))
+
+
+# ------------------------------------------------------------- caps
+def test_caps_reach_the_kernels_in_range():
+    """A cap is a Python float; fp32 knows neither 1e-60 (would be 0: no cap) nor 1e60 (infinite: refused)."""
+    assert attention._cap(0) == 0.0 and attention._cap(30) == 30.0
+    assert attention._cap(1e-60) == 1e-30 and attention._cap(1e60) == 1e30
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt,D", [(BF16, 64), (F32, 64), (F16, 256)])
+@pytest.mark.parametrize("cap", [1e-60, 1e-300, 1e60, 1e300])
+@pytest.mark.parametrize("binding", [True, False])
+def test_caps_beyond_fp32(cuda, dt, D, cap, binding, monkeypatch):
+    """Such caps leave all scores equal, or change none; with and without the C++ argument handling."""
+    if not binding:
+        monkeypatch.setattr(_lib, "fast", lambda: None)
+    g = torch.Generator().manual_seed(D)
+    q, k, v = (_rand(g, 1, 2, 130, D, dt=dt) for _ in range(3))
+    dq, dk, dv = q.to(cuda), k.to(cuda), v.to(cuda)
+    n = _i32([129], cuda)
+    tri = torch.ones(1, 1, dtype=torch.bool, device=cuda)
+    got = [bk.flash_attention(dq, dk, dv, softcap=cap)[0], bk.decode_attention(dq[:, :, 7], dk, dv, n + 1, softcap=cap)[0],
+           bk.tree_attention(dq[:, :, 7][:, None].contiguous(), dk, dv, n, tri, softcap=cap)[0, 0]]
+    sc = 0.0 if cap < 1 else 1 / math.sqrt(D)
+    for h in range(2):
+        o, av, mag = scored.rows(q[0, h], k[0, h], v[0, h], torch.ones(130, 130, dtype=torch.bool), sc)
+        lim = scored.bound(o, av, mag, dt, 130, D, min(cap, float(mag.max())))
+        assert bool(((got[0][h].double().cpu() - o).abs() <= lim).all())
+        for x in got[1:]:
+            assert bool(((x[h].double().cpu() - o[7]).abs() <= lim[7]).all())
 
 
 # ----------------------------------------------------------- slopes

@@ -47,6 +47,12 @@ def _score_args(Hq, device, softcap, alibi_slopes):
     return alibi_slopes.contiguous()
 
 
+def _cap(softcap):
+    """A checked cap as the kernels' fp32 argument: beyond these bounds the weights are the same in fp32, but a float
+    could round to 0 (no cap) or to infinity."""
+    return min(max(float(softcap), 1e-30), 1e30) if softcap else 0.0
+
+
 def flash_attention(q, k, v, causal=False, scale=None, out=None, window=0, softcap=0.0, alibi_slopes=None,
                     doc_offsets=None, prefix_lens=None):
     """O = softmax(scale Q K^T [causal]) V for [B, H, S, D] tensors (GQA when Hq > Hkv).
@@ -134,7 +140,7 @@ def _flash_scored(q, k, v, o, qs, ks, vs, os_, causal, scale, window, softcap, a
     with _lib.on_device(q):
         if o.numel():
             _lib.call("b2_flash_attn_fwd_scored", p(q), p(k), p(v), p(o), B, Hq, Hkv, Sq, Skv, D, qs, ks, vs, os_,
-                      float(scale), int(bool(causal)), int(window), float(softcap), p(slopes), p(doc_offsets), n_docs,
+                      float(scale), int(bool(causal)), int(window), _cap(softcap), p(slopes), p(doc_offsets), n_docs,
                       p(prefix_lens), _DT[q.dtype], _stream())
     return o
 
@@ -241,7 +247,7 @@ def decode_attention(q, k_cache, v_cache, seq_lens, scale=None, page_table=None,
                   None if pt is None else pt.data_ptr(), lens.data_ptr(), ws.data_ptr(), B, Hq, Hkv, D, S, ps,
                   max_pages, n_pages, _lib.strides_arg(ks), _lib.strides_arg(vs),
                   None if qp is None else qp.data_ptr(), int(window), None if fr is None else fr.data_ptr(), scale,
-                  float(softcap), None if slopes is None else slopes.data_ptr(), _DT[q.dtype], _DT[k_cache.dtype],
+                  _cap(softcap), None if slopes is None else slopes.data_ptr(), _DT[q.dtype], _DT[k_cache.dtype],
                   _stream())
     return o
 
@@ -319,7 +325,7 @@ def tree_attention(q, k_cache, v_cache, context_lens, tree_mask, draft_lens=None
                   None if draft_lens is None else draft_lens.data_ptr(), tree_mask.data_ptr(), mask_stride,
                   None if ws is None else ws.data_ptr(), B, T, Hq, Hkv, D, keys, ps, max_pages, k_cache.shape[0],
                   _lib.strides_arg(q.stride()[:3]), _lib.strides_arg(k_cache.stride()[:3]),
-                  _lib.strides_arg(v_cache.stride()[:3]), _lib.strides_arg(o.stride()[:3]), scale, float(softcap),
+                  _lib.strides_arg(v_cache.stride()[:3]), _lib.strides_arg(o.stride()[:3]), scale, _cap(softcap),
                   qd, kd, _stream())
     return o
 

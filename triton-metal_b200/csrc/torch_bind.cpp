@@ -23,6 +23,9 @@
 #include <c10/cuda/CUDAFunctions.h>
 #include <torch/extension.h>
 
+#include <algorithm>
+#include <cmath>
+
 #include "b2.h"
 
 namespace {
@@ -90,6 +93,9 @@ bool here(const OptT& t, c10::DeviceIndex dev) { return !t.has_value() || here(*
 bool is_i32(const at::Tensor& t, std::initializer_list<int64_t> shape) {
   return t.scalar_type() == at::kInt && t.is_contiguous() && t.sizes() == at::IntArrayRef(shape);
 }
+// a cap as the kernels' fp32 argument: beyond these bounds the weights are the same
+// in fp32, but a float could round to 0 (no cap) or to infinity
+float cap_arg(double cap) { return cap > 0 ? (float)std::min(std::max(cap, 1e-30), 1e30) : 0.f; }
 const void* ptr(const OptT& t) { return t.has_value() ? t->data_ptr() : nullptr; }
 void* current_stream() { return (void*)at::cuda::getCurrentCUDAStream().stream(); }
 // the output to write: the caller's, when it is what the operator would make
@@ -179,7 +185,7 @@ py::object tree_attention(const at::Tensor& q, const at::Tensor& k, const at::Te
   Cache c;
   if (!c.take(k, v, table, B, D, dev) || Hq % c.Hkv || !here(ctx, dev) || !here(mask, dev) || !here(draft, dev) ||
       !is_i32(ctx, {B}) || (draft.has_value() && !is_i32(*draft, {B})) || !mask.is_contiguous() ||
-      (mask.scalar_type() != at::kBool && mask.scalar_type() != at::kByte) || !(softcap >= 0))
+      (mask.scalar_type() != at::kBool && mask.scalar_type() != at::kByte) || !(softcap >= 0 && std::isfinite(softcap)))
     return py::none();
   const bool each = mask.dim() == 3;
   if (mask.sizes() != (each ? at::IntArrayRef({B, T, T}) : at::IntArrayRef({T, T}))) return py::none();
@@ -193,7 +199,7 @@ py::object tree_attention(const at::Tensor& q, const at::Tensor& k, const at::Te
                               ctx.data_ptr<int>(), (const int32_t*)ptr(draft), (const uint8_t*)mask.data_ptr(),
                               each ? T * T : 0, need ? ws.data_ptr() : nullptr, B, T, Hq, c.Hkv, D, c.keys, c.page_size,
                               c.max_pages, c.n_pages, q.strides().data(), k.strides().data(), v.strides().data(),
-                              o.strides().data(), (float)scale, (float)softcap, qd, kd, current_stream());
+                              o.strides().data(), (float)scale, cap_arg(softcap), qd, kd, current_stream());
   if (rc != 0) return py::int_(rc);
   return py::cast(o);
 }
@@ -210,7 +216,7 @@ py::object decode_attention(const at::Tensor& q, const at::Tensor& k, const at::
   if (!device_of(q, dev) || q.dim() != 3 || !q.is_contiguous() || q.numel() == 0 || qd < 0) return py::none();
   const int64_t B = q.size(0), Hq = q.size(1), D = q.size(2);
   Cache c;
-  if (!c.take(k, v, table, B, D, dev) || Hq % c.Hkv || !here(lens, dev) || !is_i32(lens, {B}) || !(softcap >= 0) ||
+  if (!c.take(k, v, table, B, D, dev) || Hq % c.Hkv || !here(lens, dev) || !is_i32(lens, {B}) || !(softcap >= 0 && std::isfinite(softcap)) ||
       !slopes_ok(slopes, Hq, dev))
     return py::none();
   at::Tensor o;
@@ -222,7 +228,7 @@ py::object decode_attention(const at::Tensor& q, const at::Tensor& k, const at::
   const int rc = b2_decode_attn_scored(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
                                        (const int32_t*)ptr(table), lens.data_ptr<int>(), ws.data_ptr(), B, Hq, c.Hkv, D,
                                        c.keys, c.page_size, c.max_pages, c.n_pages, k.strides().data(),
-                                       v.strides().data(), nullptr, 0, nullptr, (float)scale, (float)softcap,
+                                       v.strides().data(), nullptr, 0, nullptr, (float)scale, cap_arg(softcap),
                                        (const float*)ptr(slopes), qd, dtype_code(k), current_stream());
   if (rc != 0) return py::int_(rc);
   return py::cast(o);
@@ -239,7 +245,7 @@ py::object flash_scored(const at::Tensor& q, const at::Tensor& k, const at::Tens
     return py::none();
   const int64_t B = q.size(0), Hq = q.size(1), S = q.size(2), D = q.size(3), Hkv = k.size(1), Skv = k.size(2);
   if (k.size(0) != B || k.size(3) != D || Hq % Hkv || ((causal || docs.has_value()) && S != Skv) || window < 0 ||
-      (window && !causal) || !(softcap >= 0) || !slopes_ok(slopes, Hq, dev) || !here(docs, dev) || !here(prefix, dev))
+      (window && !causal) || !(softcap >= 0 && std::isfinite(softcap)) || !slopes_ok(slopes, Hq, dev) || !here(docs, dev) || !here(prefix, dev))
     return py::none();
   int64_t n_docs = 0;
   if (docs.has_value()) {
@@ -253,7 +259,7 @@ py::object flash_scored(const at::Tensor& q, const at::Tensor& k, const at::Tens
   if (!output(out, q, q.sizes(), o)) return py::none();
   const int rc = b2_flash_attn_fwd_scored(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), B, Hq, Hkv, S, Skv, D,
                                           q.strides().data(), k.strides().data(), v.strides().data(),
-                                          o.strides().data(), (float)scale, causal, window, (float)softcap,
+                                          o.strides().data(), (float)scale, causal, window, cap_arg(softcap),
                                           (const float*)ptr(slopes), (const int32_t*)ptr(docs), n_docs,
                                           (const int32_t*)ptr(prefix), dt, current_stream());
   if (rc != 0) return py::int_(rc);
