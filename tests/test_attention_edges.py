@@ -72,6 +72,15 @@ def test_decode_attention_refuses_other_devices():
         bk.decode_attention(_on_gpu(2, 4, 64), mine, mine, [1, 2], out=other(2, 4, 64))
 
 
+def test_rows_beyond_31_bits_refused_without_gpu():
+    """Head dims off the tensor cores count a kv head's rows (queries times query heads) in 32 bits."""
+    s = _lib.strides_arg((8, 8, 8))
+    call = lambda S, Hq: _lib.load().b2_flash_attn_fwd_scored(8, 8, 8, 8, 1, Hq, 1, S, 4, 8, s, s, s, s, 1.0, 0, 0, 1.0,
+                                                              None, None, 0, None, 0, None)
+    assert call(1 << 24, 128) == errors.ERR_UNSUPPORTED and b"rows a kv head" in _lib.load().b2_last_error()
+    assert call(1 << 24, 65535) == errors.ERR_UNSUPPORTED
+
+
 # ------------------------------------------------------------- caps
 def test_caps_reach_the_kernels_in_range():
     """A cap is a Python float; fp32 knows neither 1e-60 (would be 0: no cap) nor 1e60 (infinite: refused)."""

@@ -615,6 +615,8 @@ extern "C" int b2_flash_attn_fwd_scored(const void* q, const void* k, const void
       return launch_status("flash_attn_fwd_scored");
     }
   }
+  B2_CHECK_ARG(Sq * (Hq / Hkv) <= 2147483647 - 64, B2_ERR_UNSUPPORTED,
+               "flash_attn_fwd_scored: %lld rows a kv head", (long long)(Sq * (Hq / Hkv)));
   attn::SimtParams s = {};
   s.q = q;
   s.k = k;
