@@ -175,6 +175,75 @@ def _token_slopes(cuda, dt, D, rep, ps):
             assert bool(((out[b, h] - o[0]).abs() <= lim[0]).all()), (b, h)
 
 
+# ------------------------------------- infinities and NaN that a row sees
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt,D", [(BF16, 128), (F16, 64), (F32, 64)])
+@pytest.mark.parametrize("causal,cap,alibi", [(False, 0.0, False), (True, 0.0, True), (True, 30.0, False),
+                                              (False, 30.0, True)])
+def test_prompt_nan_scores(cuda, dt, D, causal, cap, alibi):
+    """A NaN in K of one key, each key in turn: all rows that see it are NaN, the others as without it.  An infinite
+    score without a cap is NaN as well (inf - inf in the softmax)."""
+    g = torch.Generator().manual_seed(D)
+    S = 140
+    q, k, v = (_rand(g, 1, 1, S, D, dt=dt).expand(S, 1, S, D) for _ in range(3))
+    sl = torch.tensor([0.01], device=cuda) if alibi else None
+    docs = _i32([[0, S]], cuda).expand(S, 2).contiguous()
+    run = lambda x: bk.flash_attention(q.to(cuda), x.to(cuda), v.to(cuda), causal=causal, softcap=cap, alibi_slopes=sl,
+                                       doc_offsets=docs).float().cpu()
+    clean = run(k)
+    sees = torch.arange(S)[None] >= torch.arange(S)[:, None] if causal else torch.ones(S, S, dtype=torch.bool)
+    for x in (math.nan, math.inf):
+        k2 = k.clone()
+        k2[torch.arange(S), 0, torch.arange(S), 0] = x
+        out = run(k2)[:, 0]
+        sick = sees if math.isnan(x) else sees & (q[0, 0, :, 0] > 0)[None]  # -inf: the key has weight 0
+        if cap and x == math.inf:
+            assert torch.isfinite(out).all()
+            continue
+        assert torch.isnan(out[sick]).all()
+        hidden = ~sees
+        assert torch.equal(out[hidden], clean[:, 0][hidden])
+        assert torch.isfinite(out[~sick]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt,D,window", [(BF16, 128, 0), (F16, 64, 0), (F32, 64, 0), (F16, 256, 0), (BF16, 64, 200)])
+@pytest.mark.parametrize("rep", [1, 4, 16])
+@pytest.mark.parametrize("cap,alibi", [(30.0, False), (0.0, True)])
+def test_token_nan_scores(cuda, dt, D, window, rep, cap, alibi):
+    g = torch.Generator().manual_seed(D + rep)
+    S = 140
+    q = _rand(g, 1, 2 * rep, D, dt=dt).expand(S, 2 * rep, D)
+    k, v = (_rand(g, 1, 2, S, D, dt=dt).expand(S, 2, S, D) for _ in range(2))
+    k2 = k.clone()
+    k2[torch.arange(S), 0, torch.arange(S), 0] = math.nan  # kv head 0 only
+    sl = _signed(2 * rep).abs().to(cuda) / 16 if alibi else None
+    run = lambda x: bk.decode_attention(q.contiguous().to(cuda), x.to(cuda), v.to(cuda), _i32([S] * S, cuda), softcap=cap,
+                                        alibi_slopes=sl, window=window).float().cpu()
+    out = run(k2)
+    assert torch.isnan(out[:, :rep]).all()
+    assert torch.equal(out[:, rep:], run(k)[:, rep:])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt,D", [(BF16, 128), (F16, 64), (F32, 64)])
+@pytest.mark.parametrize("T,rep", [(1, 4), (4, 4), (4, 12), (2, 40), (9, 16)])
+def test_tree_nan_scores(cuda, dt, D, T, rep):
+    g = torch.Generator().manual_seed(D + T)
+    S = 140
+    q = _rand(g, 1, T, 2 * rep, D, dt=dt).expand(S, T, 2 * rep, D)
+    k, v = (_rand(g, 1, 2, S + T, D, dt=dt).expand(S, 2, S + T, D) for _ in range(2))
+    k2 = k.clone()
+    k2[torch.arange(S), 0, torch.arange(S), 0] = math.nan
+    k2[:, 1, S + T - 1] = math.nan  # kv head 1: a drafted token that only the last row sees
+    mask = torch.tril(torch.ones(T, T, dtype=torch.bool)).to(cuda)
+    run = lambda x: bk.tree_attention(q.to(cuda), x.to(cuda), v.to(cuda), _i32([S] * S, cuda), mask).float().cpu()
+    out, clean = run(k2), run(k)
+    assert torch.isnan(out[:, :, :rep]).all()
+    assert torch.isnan(out[:, -1, rep:]).all()
+    assert torch.equal(out[:, :-1, rep:], clean[:, :-1, rep:])
+
+
 # ------------------------------------------------------------ pages
 @pytest.mark.gpu
 @pytest.mark.parametrize("dt,D", [(BF16, 128), (F16, 64), (BF16, 256), (F32, 64)])

@@ -71,6 +71,11 @@ struct Params {
 // among them would make each wait for the one before.
 __device__ __forceinline__ bool page_ok(const Params& p, int pg) { return (uint32_t)pg < p.n_pages; }
 
+// Whether a row with the sum of weights l has an output, or saw nothing and gives
+// 0.  With score forms a NaN score makes a NaN row; without them such a row gives 0.
+__device__ __forceinline__ bool scored(const Params& p) { return p.softcap > 0.f || p.slopes; }
+__device__ __forceinline__ bool has_sum(const Params& p, float l) { return scored(p) ? l != 0.f : l > 0.f; }
+
 // Key range [lo, hi) of sequence b and its query position.
 __device__ __forceinline__ void key_range(const Params& p, int b, int& lo, int& hi, int& qp) {
   // seq_lens[b] beyond the caller's max_seq_len is clamped to it: the splits
@@ -236,7 +241,7 @@ decode_split_kernel(const Params p) {
     if (hh >= rep) break;
     const int hq = hk * rep + hh;
     if (p.nsplit == 1) {
-      const float inv = l[i] > 0.f ? 1.f / l[i] : 0.f;
+      const float inv = has_sum(p, l[i]) ? 1.f / l[i] : 0.f;
 #pragma unroll
       for (int jd = 0; jd < kDPL; ++jd) {
         const int d = lane + 32 * jd;
@@ -268,12 +273,12 @@ __global__ void decode_combine_kernel(const Params p) {
     float num = 0.f, den = 0.f;
     for (int s = 0; s < p.nsplit; ++s) {
       const float* ws = w + s * (D + 2);
-      if (ws[0] == -INFINITY) continue;  // empty split
+      if (scored(p) ? ws[1] == 0.f : ws[0] == -INFINITY) continue;  // empty split
       const float f = __expf(ws[0] - M);
       num += f * ws[2 + d];
       den += f * ws[1];
     }
-    stf((TQ*)p.o + (int64_t)bh * D + d, den > 0.f ? num / den : 0.f);
+    stf((TQ*)p.o + (int64_t)bh * D + d, has_sum(p, den) ? num / den : 0.f);
   }
 }
 
@@ -602,7 +607,7 @@ decode_tc_kernel(const Params p) {
     }
     const int hq = hk * rep + r;
     if (p.nsplit == 1) {
-      ((T*)p.o)[((int64_t)b * p.Hq + hq) * D + d] = from_f32<T>(L > 0.f ? O / L : 0.f);
+      ((T*)p.o)[((int64_t)b * p.Hq + hq) * D + d] = from_f32<T>(has_sum(p, L) ? O / L : 0.f);
     } else {
       float* w = p.ws + (((int64_t)b * p.Hq + hq) * p.nsplit + split) * (D + 2);
       if (d == 0) {

@@ -134,6 +134,11 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {  // NaN if one of them is
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 // exp2 of two lanes on the FMA pipe, to take part of the softmax's
 // exponentials off the MUFU unit (the method of FlashAttention-4: Cody-Waite
 // split x = j + f, j = rint(x), |f| <= 1/2, then a polynomial for 2^f and j
@@ -292,7 +297,7 @@ __device__ __forceinline__ void score_chunk(uint32_t (&sv)[N], const Score& c) {
   }
 }
 
-// Largest of N columns; BITS: of those with a bit in w (N = 32).
+// Largest of N columns, NaN if one of them is; BITS: of those with a bit in w (N = 32).
 template <bool BITS, int N>
 __device__ __forceinline__ float max_chunk(const uint32_t (&sv)[N], uint32_t w) {
   float mx = -INFINITY;
@@ -303,7 +308,7 @@ __device__ __forceinline__ float max_chunk(const uint32_t (&sv)[N], uint32_t w) 
       if (!(w >> e & 1)) v0 = -INFINITY;
       if (!(w >> (e + 1) & 1)) v1 = -INFINITY;
     }
-    mx = max3(mx, v0, v1);
+    mx = max3_nan(mx, v0, v1);
   }
   return mx;
 }
@@ -455,6 +460,9 @@ __device__ __forceinline__ void softmax_chunk(uint32_t (&sv)[N], uint32_t tS, ui
     else mx *= sc.scale_log2;
   }
   if (!BITS && !w) mx = -INFINITY;
+  // a score that is NaN, or infinite (inf - inf), makes NaN of the row; where its
+  // exponential is the polynomial's, that would lose it
+  if (!(mx < INFINITY)) l = NAN;
   const bool need = mx > m + kRescale;
   if (__any_sync(0xffffffffu, need)) {
     // the first maximum as it is (a row's only key has weight 1), then whole steps
@@ -575,6 +583,7 @@ __device__ __forceinline__ void softmax_few(uint8_t* room, uint32_t tS, uint32_t
     if constexpr (CAP) mx = mx == -INFINITY ? mx : capped_any(mx, sc, 0.f);
     else mx *= sc.scale_log2;
   }
+  if (!(mx < INFINITY)) l = NAN;  // as in softmax_chunk; this lane's part of the row's sum
   mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
   mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
   const bool need = mx > m + kRescale;
