@@ -176,6 +176,69 @@ def _token_slopes(cuda, dt, D, rep, ps):
 
 
 # ------------------------------------- infinities and NaN that a row sees
+def _same_kind(out, ref):
+    """Infinite and NaN where ref is, in kind and sign."""
+    return torch.equal(torch.isnan(out), torch.isnan(ref)) and torch.equal(out == math.inf, ref == math.inf) and \
+        torch.equal(out == -math.inf, ref == -math.inf)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt,D", [(BF16, 128), (F16, 64), (F32, 64)])
+@pytest.mark.parametrize("T,Hq,Hkv", [(1, 2, 2), (2, 8, 2), (3, 24, 2), (5, 8, 1), (30, 8, 2)])
+@pytest.mark.parametrize("ps", [0, 12, 16])
+def test_tree_visible_infinities(cuda, dt, D, T, Hq, Hkv, ps):
+    """V of context keys holds infinities and NaN: +inf, -inf, both, NaN, an infinity that meets a drafted token's of
+    the other sign; elsewhere nothing changes.  Rows stand in their tile four times, twice, once and in pairs."""
+    g = torch.Generator().manual_seed(T + D)
+    for ctx in (150, 3000):
+        q = _rand(g, 2, T, Hq, D, dt=dt)
+        k, v = _rand(g, 2, Hkv, ctx + T, D, dt=dt), _rand(g, 2, Hkv, ctx + T, D, dt=dt)
+        clean, bad = v, v.clone()
+        mask = torch.tril(torch.ones(T, T, dtype=torch.bool))
+        for key, col, x in ((0, 1, math.inf), (ctx // 2, 2, -math.inf), (37, 3, math.inf), (ctx - 1, 3, -math.inf),
+                            (ctx // 3, 4, math.nan), (ctx - 20, D - 1, math.inf), (ctx - 90, D - 1, math.inf),
+                            (ctx, 6, -math.inf), (60, 6, math.inf), (ctx + T - 1, 7, -math.inf), (101, D // 2, math.inf)):
+            bad[0, :, key, col] = x
+        res = []
+        for x in (clean, bad):
+            kc, vc, table = (k, x, None) if not ps else _pages(k, x, ps, torch.Generator().manual_seed(1))
+            res.append(bk.tree_attention(q.to(cuda), kc.to(cuda), vc.to(cuda), _i32([ctx, ctx - 7], cuda), mask.to(cuda),
+                                         page_table=None if table is None else table.to(cuda)).float().cpu())
+        want = res[0].clone()
+        want[0, :, :, [1, D - 1, D // 2]] = math.inf
+        want[0, :, :, 2] = -math.inf
+        want[0, :, :, [3, 4, 6]] = math.nan
+        want[0, -1, :, 7] = -math.inf
+        assert _same_kind(res[1], want), ctx
+        fine = torch.isfinite(want)
+        assert torch.equal(res[1][fine], want[fine])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt,D,window", [(BF16, 128, 0), (F16, 64, 0), (F32, 64, 0), (F16, 256, 0), (BF16, 64, 90)])
+@pytest.mark.parametrize("rep", [1, 4, 12])
+@pytest.mark.parametrize("cap,alibi", [(20.0, False), (0.0, True)])
+def test_token_visible_infinities(cuda, dt, D, window, rep, cap, alibi):
+    g = torch.Generator().manual_seed(rep + D)
+    n, Hkv = 400, 2
+    q, k, v = _rand(g, 2, rep * Hkv, D, dt=dt), _rand(g, 2, Hkv, n, D, dt=dt), _rand(g, 2, Hkv, n, D, dt=dt)
+    sl = _signed(rep * Hkv).abs().to(cuda) / 16 if alibi else None
+    run = lambda x: bk.decode_attention(q.to(cuda), k.to(cuda), x.to(cuda), _i32([n, n - 3], cuda), softcap=cap,
+                                        alibi_slopes=sl, window=window).float().cpu()
+    bad = v.clone()
+    for key, col, x in ((n - 1, 1, math.inf), (n - 40, 2, -math.inf), (n - 70, 3, math.inf), (n - 5, 3, -math.inf),
+                        (n - 33, 4, math.nan), (n - 90, D - 1, math.inf)):
+        bad[0, :, key, col] = x
+    want = run(v)
+    want[0, :, [1, D - 1]] = math.inf
+    want[0, :, 2] = -math.inf
+    want[0, :, [3, 4]] = math.nan
+    out = run(bad)
+    assert _same_kind(out, want)
+    fine = torch.isfinite(want)
+    assert torch.equal(out[fine], want[fine])
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dt,D", [(BF16, 128), (F16, 64), (F32, 64)])
 @pytest.mark.parametrize("causal,cap,alibi", [(False, 0.0, False), (True, 0.0, True), (True, 30.0, False),

@@ -44,7 +44,7 @@
 // 128, bf16: 0.88 ms, 3.1 TB/s and 780 TF/s (either floor is 0.42 ms; the softmax
 // between a tile's two MMAs sets the time); trees of 26, 16 requests of up to
 // 4096 keys in pages of 16, fp16: 56 us, 2.6 TB/s (starts and ends of segments);
-// a tree of 8, one request of 500 keys: 19 us (two launches and one chain).
+// a tree of 8, one request of 500 keys: 20 us (two launches and one chain).
 #pragma once
 #include "attn_common.cuh"
 #include "fa_common.cuh"
@@ -238,6 +238,16 @@ __device__ __forceinline__ bool any_of_softmax(bool x) {
       : "memory");
   return r != 0;
 }
+// the same of one softmax warpgroup
+__device__ __forceinline__ bool any_of_warpgroup(int u, bool x) {
+  uint32_t r;
+  asm volatile(
+      "{\n .reg .pred p, q;\n setp.ne.b32 p, %2, 0;\n barrier.cta.red.or.pred q, %1, 128, p;\n selp.u32 %0, 1, 0, q;\n}"
+      : "=r"(r)
+      : "r"(3 + u), "r"((uint32_t)x)
+      : "memory");
+  return r != 0;
+}
 __device__ __forceinline__ void warpgroup_sync(int u) { asm volatile("barrier.cta.sync %0, 128;" ::"r"(3 + u) : "memory"); }
 __device__ __forceinline__ void softmax_sync() { asm volatile("barrier.cta.sync 2, 256;" ::: "memory"); }
 
@@ -258,6 +268,22 @@ __device__ __forceinline__ bool key_offset(const Params& p, int b, int hk, int p
   ko = b * p.ks[0] + hk * p.ks[1] + (int64_t)pos * p.ks[2];
   vo = b * p.vs[0] + hk * p.vs[1] + (int64_t)pos * p.vs[2];
   return true;
+}
+
+// Bits of the columns, of the 8 in x, that are +inf, -inf or NaN.
+struct Kinds {
+  uint32_t pos, neg, nan;
+};
+template <int FMT>
+__device__ __forceinline__ void find_kinds(const uint4& x, Kinds& k) {
+  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const uint32_t h = w[e >> 1] >> (16 * (e & 1)) & 0xffffu;
+    if (!not_finite16<FMT>(h)) continue;
+    constexpr uint32_t frac = FMT == kF16 ? 0x03ffu : 0x007fu;
+    (h & frac ? k.nan : h & 0x8000u ? k.neg : k.pos) |= 1u << e;
+  }
 }
 
 // ring index of K_i and V_i within a segment of n tiles: K0 K1 V0 K2 V1 ... V(n-1)
@@ -838,9 +864,26 @@ tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
           }
         }
       };
+      auto drafted_bad = [&](int c) {  // what add_bad adds to one column
+        const int j0 = max(sg.tile * BK - sg.ctx, 0), j1 = min((sg.tile + sg.n) * BK - sg.ctx, sg.dl);
+        float x = 0.f;
+        for (int j = j0; j < j1; ++j) {
+          int64_t ko, vo;
+          if (mask && !mask[(int64_t)t * p.T + j]) continue;
+          if (!key_offset(p, sg.b, sg.hk, sg.ctx + j, key_page(p, sg.b, sg.ctx + j), ko, vo)) continue;
+          if (not_finite16<FMT>(p.v[vo + c])) x += widen16<FMT>(p.v[vo + c]);
+        }
+        return x;
+      };
       if (!PAIR && copies > 1) {
         // Copies: each warp stages its rows' sums over the units, CW columns at a
-        // time, and the warpgroup adds the copies up on the way out.
+        // time, and the warpgroup adds the copies up on the way out.  A copy's weight
+        // is 0 for the other copies' keys, which makes NaN of an infinity in their V:
+        // where a sum is not finite, the columns of V that hold any in this segment's
+        // context are looked up (all rows see the context), and such a column's sum is
+        // the sum of those values, whatever their weights.  That reads V once more,
+        // HD / 2 columns by each warpgroup, 32 or 64 keys at a time: 64 requests of up
+        // to 8192 keys with an infinity in each, 32 / 8 heads of 128: 1.2 ms, not 0.25.
         if (!any_of_softmax(!ok)) {
           tc::fence_after_sync();
           constexpr int CW = HD == 128 ? 32 : 16, CPR = CW / 4;
@@ -868,13 +911,53 @@ tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
               if (units == 2 && f1 != 0.f) x = fmaf(o1[e], f1, x);
               o[e] = x;
             }
+            uint64_t zero2 = 0;  // NaN if one is not finite
+#pragma unroll
+            for (int e = 0; e < CW; e += 2) zero2 = fma_f2(f2_pack(o[e], o[e + 1]), 0, zero2);
+            const float finite = f2_lo(zero2) + f2_hi(zero2);
             if (bad && row_ok && copy == 0) add_bad(o, c, CW);
             const float scale = whole ? inv : 1.f;
 #pragma unroll
             for (int e = 0; e < CW; ++e) o[e] = row_ok && L != 0.f ? o[e] * scale : 0.f;
 #pragma unroll
             for (int e = 0; e < CPR; ++e) *staged(r, e) = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
-            warpgroup_sync(u);
+            // (a row whose weights add up to NaN is NaN anyway)
+            if (__builtin_expect(any_of_warpgroup(u, row_ok && finite != 0.f && L == L), 0)) {
+              constexpr int NL = CW / 8;  // threads a key
+              const int part8 = (tid & 127) % NL, key1 = min((sg.tile + sg.n) * BK, sg.ctx);
+              Kinds k = {0, 0, 0};
+#pragma unroll 4
+              for (int key = sg.tile * BK + (tid & 127) / NL; key < key1; key += 128 / NL) {
+                int64_t ko, vo;
+                if (!key_offset(p, sg.b, sg.hk, key, key_page(p, sg.b, key), ko, vo)) continue;
+                find_kinds<FMT>(*reinterpret_cast<const uint4*>(p.v + vo + c + 8 * part8), k);
+              }
+              uint32_t* found = reinterpret_cast<uint32_t*>(s_ml + u * 128);  // its sums are read: room for [4 warps][3]
+              __syncwarp();
+              k.pos = __reduce_or_sync(0xffffffffu, k.pos << (8 * part8));
+              k.neg = __reduce_or_sync(0xffffffffu, k.neg << (8 * part8));
+              k.nan = __reduce_or_sync(0xffffffffu, k.nan << (8 * part8));
+              if (lane == 0) {
+                found[3 * qw] = k.pos;
+                found[3 * qw + 1] = k.neg;
+                found[3 * qw + 2] = k.nan;
+              }
+              warpgroup_sync(u);
+              k.pos = found[0] | found[3] | found[6] | found[9];
+              k.neg = found[1] | found[4] | found[7] | found[10];
+              k.nan = found[2] | found[5] | found[8] | found[11];
+              for (uint32_t left = k.pos | k.neg | k.nan; left; left &= left - 1) {
+                const int e = __ffs(left) - 1;
+                float x = 0.f;
+                if (row_ok && copy == 0 && L != 0.f) {
+                  x = k.nan >> e & 1 ? NAN : k.pos >> e & 1 ? (k.neg >> e & 1 ? NAN : INFINITY) : -INFINITY;
+                  if (bad) x += drafted_bad(c + e);
+                  x *= scale;
+                }
+                reinterpret_cast<float*>(staged(r, e >> 2))[e & 3] = x;
+              }
+              warpgroup_sync(u);
+            }
             for (int i = tid & 127; i < rw * CPR; i += 128) {
               const int rr = i / CPR, ch = i % CPR, t2 = rt * p.tpt + rr / p.rep;
               if (rr >= br || t2 >= p.T) continue;
