@@ -215,6 +215,34 @@ def test_tree_visible_infinities(cuda, dt, D, T, Hq, Hkv, ps):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dt,D", [(BF16, 128), (F16, 128), (F16, 64)])
+@pytest.mark.parametrize("T,Hq,Hkv", [(1, 8, 2), (12, 8, 2), (30, 8, 2), (60, 8, 2), (33, 4, 1)])
+@pytest.mark.parametrize("ps", [0, 16])
+def test_tree_infinities_of_small_weight(cuda, dt, D, T, Hq, Hkv, ps):
+    """Visible infinities whose weights are far below fp16's smallest (scores up to 50 below the row's largest), but not
+    below fp32's."""
+    g = torch.Generator().manual_seed(T + D)
+    ctx = 700
+    q, k, v = _rand(g, 1, T, Hq, D, dt=dt, big=5.0), _rand(g, 1, Hkv, ctx + T, D, dt=dt), _rand(g, 1, Hkv, ctx + T, D, dt=dt)
+    mask = torch.tril(torch.ones(T, T, dtype=torch.bool))
+
+    def run(x):
+        kc, vc, table = (k, x, None) if not ps else _pages(k, x, ps, torch.Generator().manual_seed(1))
+        return bk.tree_attention(q.to(cuda), kc.to(cuda), vc.to(cuda), _i32([ctx], cuda), mask.to(cuda),
+                                 page_table=None if table is None else table.to(cuda)).float().cpu()
+    bad = v.clone()
+    for key in range(0, 640, 64):
+        bad[0, :, key, key // 64] = math.inf if key % 128 else -math.inf
+    bad[0, :, 650, D - 1], bad[0, :, 30, D - 1] = math.inf, -math.inf
+    want = run(v)
+    want[..., 0:10:2], want[..., 1:10:2], want[..., D - 1] = -math.inf, math.inf, math.nan
+    out = run(bad)
+    assert _same_kind(out, want)
+    fine = torch.isfinite(want)
+    assert torch.equal(out[fine], want[fine])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dt,D,window", [(BF16, 128, 0), (F16, 64, 0), (F32, 64, 0), (F16, 256, 0), (BF16, 64, 90)])
 @pytest.mark.parametrize("rep", [1, 4, 12])
 @pytest.mark.parametrize("cap,alibi", [(20.0, False), (0.0, True)])

@@ -638,6 +638,39 @@ __device__ __forceinline__ bool zero_not_finite(uint4& x) {
   }
   return hit;
 }
+// sum of a flag over the 256 softmax threads: a barrier and a vote in one, so
+// that all of them leave together
+__device__ __forceinline__ bool any_of_softmax(bool x) {
+  uint32_t r;
+  asm volatile(
+      "{\n .reg .pred p, q;\n setp.ne.b32 p, %1, 0;\n barrier.cta.red.or.pred q, 1, 256, p;\n selp.u32 %0, 1, 0, q;\n}"
+      : "=r"(r)
+      : "r"((uint32_t)x)
+      : "memory");
+  return r != 0;
+}
+
+// Bits of columns that hold +inf, -inf or NaN, and the sum of those values in one.
+struct Kinds {
+  uint32_t pos, neg, nan;
+  __device__ __forceinline__ uint32_t any() const { return pos | neg | nan; }
+  __device__ __forceinline__ uint32_t undefined() const { return nan | (pos & neg); }  // the sum is NaN
+  __device__ __forceinline__ float sum(int e) const {
+    return undefined() >> e & 1 ? NAN : pos >> e & 1 ? INFINITY : neg >> e & 1 ? -INFINITY : 0.f;
+  }
+};
+// adds those of the 8 in x to k
+template <int FMT>
+__device__ __forceinline__ void find_kinds(const uint4& x, Kinds& k) {
+  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const uint32_t h = w[e >> 1] >> (16 * (e & 1)) & 0xffffu;
+    if (!not_finite16<FMT>(h)) continue;
+    constexpr uint32_t frac = FMT == kF16 ? 0x03ffu : 0x007fu;
+    (h & frac ? k.nan : h & 0x8000u ? k.neg : k.pos) |= 1u << e;
+  }
+}
 // 4-D tensor map coordinates: (d, s, h, b)
 __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, int d, int s, int h, int b,
                                             uint64_t* bar) {

@@ -227,18 +227,7 @@ __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commi
 template <int N>
 __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-// sum of a flag over the 256 softmax threads: a barrier and a vote in one, so
-// that all of them leave together
-__device__ __forceinline__ bool any_of_softmax(bool x) {
-  uint32_t r;
-  asm volatile(
-      "{\n .reg .pred p, q;\n setp.ne.b32 p, %1, 0;\n barrier.cta.red.or.pred q, 1, 256, p;\n selp.u32 %0, 1, 0, q;\n}"
-      : "=r"(r)
-      : "r"((uint32_t)x)
-      : "memory");
-  return r != 0;
-}
-// the same of one softmax warpgroup
+// any_of_softmax of one softmax warpgroup
 __device__ __forceinline__ bool any_of_warpgroup(int u, bool x) {
   uint32_t r;
   asm volatile(
@@ -268,22 +257,6 @@ __device__ __forceinline__ bool key_offset(const Params& p, int b, int hk, int p
   ko = b * p.ks[0] + hk * p.ks[1] + (int64_t)pos * p.ks[2];
   vo = b * p.vs[0] + hk * p.vs[1] + (int64_t)pos * p.vs[2];
   return true;
-}
-
-// Bits of the columns, of the 8 in x, that are +inf, -inf or NaN.
-struct Kinds {
-  uint32_t pos, neg, nan;
-};
-template <int FMT>
-__device__ __forceinline__ void find_kinds(const uint4& x, Kinds& k) {
-  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const uint32_t h = w[e >> 1] >> (16 * (e & 1)) & 0xffffu;
-    if (!not_finite16<FMT>(h)) continue;
-    constexpr uint32_t frac = FMT == kF16 ? 0x03ffu : 0x007fu;
-    (h & frac ? k.nan : h & 0x8000u ? k.neg : k.pos) |= 1u << e;
-  }
 }
 
 // ring index of K_i and V_i within a segment of n tiles: K0 K1 V0 K2 V1 ... V(n-1)
@@ -864,6 +837,20 @@ tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
           }
         }
       };
+      // Kinds of the 8 columns from c on in the context of this segment, of every n-th
+      // key from the i-th on.
+      auto context_kinds = [&](int c, int i, int n) {
+        Kinds k = {0, 0, 0};
+        const int end = min((sg.tile + sg.n) * BK, sg.ctx);
+#pragma unroll 4
+        for (int key = sg.tile * BK + i; key < end; key += n) {
+          int64_t ko, vo;
+          if (!key_offset(p, sg.b, sg.hk, key, key_page(p, sg.b, key), ko, vo)) continue;
+          find_kinds<FMT>(*reinterpret_cast<const uint4*>(p.v + vo + c), k);
+        }
+        __syncwarp();
+        return k;
+      };
       auto drafted_bad = [&](int c) {  // what add_bad adds to one column
         const int j0 = max(sg.tile * BK - sg.ctx, 0), j1 = min((sg.tile + sg.n) * BK - sg.ctx, sg.dl);
         float x = 0.f;
@@ -924,16 +911,9 @@ tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
             // (a row whose weights add up to NaN is NaN anyway)
             if (__builtin_expect(any_of_warpgroup(u, row_ok && finite != 0.f && L == L), 0)) {
               constexpr int NL = CW / 8;  // threads a key
-              const int part8 = (tid & 127) % NL, key1 = min((sg.tile + sg.n) * BK, sg.ctx);
-              Kinds k = {0, 0, 0};
-#pragma unroll 4
-              for (int key = sg.tile * BK + (tid & 127) / NL; key < key1; key += 128 / NL) {
-                int64_t ko, vo;
-                if (!key_offset(p, sg.b, sg.hk, key, key_page(p, sg.b, key), ko, vo)) continue;
-                find_kinds<FMT>(*reinterpret_cast<const uint4*>(p.v + vo + c + 8 * part8), k);
-              }
+              const int part8 = (tid & 127) % NL;
+              Kinds k = context_kinds(c + 8 * part8, (tid & 127) / NL, 128 / NL);
               uint32_t* found = reinterpret_cast<uint32_t*>(s_ml + u * 128);  // its sums are read: room for [4 warps][3]
-              __syncwarp();
               k.pos = __reduce_or_sync(0xffffffffu, k.pos << (8 * part8));
               k.neg = __reduce_or_sync(0xffffffffu, k.neg << (8 * part8));
               k.nan = __reduce_or_sync(0xffffffffu, k.nan << (8 * part8));
@@ -946,11 +926,11 @@ tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
               k.pos = found[0] | found[3] | found[6] | found[9];
               k.neg = found[1] | found[4] | found[7] | found[10];
               k.nan = found[2] | found[5] | found[8] | found[11];
-              for (uint32_t left = k.pos | k.neg | k.nan; left; left &= left - 1) {
+              for (uint32_t left = k.any(); left; left &= left - 1) {
                 const int e = __ffs(left) - 1;
                 float x = 0.f;
                 if (row_ok && copy == 0 && L != 0.f) {
-                  x = k.nan >> e & 1 ? NAN : k.pos >> e & 1 ? (k.neg >> e & 1 ? NAN : INFINITY) : -INFINITY;
+                  x = k.sum(e);
                   if (bad) x += drafted_bad(c + e);
                   x *= scale;
                 }
@@ -1029,6 +1009,22 @@ tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
               float x = f0 == 0.f ? 0.f : o[e] * f0;
               if (units == 2 && f1 != 0.f) x = fmaf(o1[e], f1, x);
               o[e] = x;
+            }
+          }
+          if constexpr (FMT == kF16) {
+            // A weight that rounds to 0 in fp16 (below 2^-25) makes NaN of an infinity,
+            // as another copy's keys do above; one warp for its rows.
+            float finite = 0.f;
+#pragma unroll
+            for (int e = 0; e < 32; ++e) finite = fmaf(o[e], 0.f, finite);
+            if (__builtin_expect(__any_sync(0xffffffffu, row_ok && finite != 0.f && L == L), 0)) {
+              Kinds k = context_kinds(c + 8 * (lane % 4), lane / 4, 8);
+              k.pos = __reduce_or_sync(0xffffffffu, k.pos << (8 * (lane % 4)));
+              k.neg = __reduce_or_sync(0xffffffffu, k.neg << (8 * (lane % 4)));
+              k.nan = __reduce_or_sync(0xffffffffu, k.nan << (8 * (lane % 4)));
+#pragma unroll
+              for (int e = 0; e < 32; ++e)
+                if (k.any() >> e & 1) o[e] = k.sum(e);
             }
           }
           if (bad && row_ok) add_bad(o, c, 32);
