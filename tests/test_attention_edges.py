@@ -335,6 +335,108 @@ def test_tree_nan_scores(cuda, dt, D, T, rep):
     assert torch.equal(out[:, :-1, rep:], clean[:, :-1, rep:])
 
 
+# --------------------------------- infinities and NaN that a row must not see
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt,D", [(BF16, 128), (F16, 64), (F32, 64)])
+@pytest.mark.parametrize("kw", [dict(causal=True, docs=[0, 600]), dict(causal=True, docs=[0, 3, 130, 131, 400, 555]),
+                                dict(docs=[20, 150, 384, 590]), dict(causal=True, window=100, cap=20.0),
+                                dict(causal=True, window=1, docs=[0, 600]), dict(causal=True, prefix=300, cap=30.0),
+                                dict(causal=True, alibi=True), dict(docs=[0, 200, 600], alibi=True, cap=9.0)])
+@pytest.mark.parametrize("far", [False, True])
+def test_prompt_hidden_values(cuda, dt, D, kw, far):
+    """Infinities and NaN in V of keys all over the prompt, in different columns (far: only at both ends): each row
+    shows those of the keys it sees, and nothing of the others."""
+    g = torch.Generator().manual_seed(D)
+    S, Hq, Hkv = 600, 4, 2
+    q, k, v = (_rand(g, 1, h, S, D, dt=dt) for h in (Hq, Hkv, Hkv))
+    where = [(0, 1, math.nan), (599, 2, math.inf)] + ([] if far else [(128, 3, math.inf), (127, 4, -math.inf),
+             (300, 5, math.nan), (301, 3, -math.inf), (450, D - 1, math.inf)])
+    vis = scored.ranges(S, S, kw.get("causal", False), kw.get("window", 0), kw.get("docs"),
+                        [kw["prefix"]] if "prefix" in kw else None)
+    sl = _slopes(Hq) if kw.get("alibi") else None
+    bad, finite = v.clone(), v.clone()
+    want = torch.zeros(Hkv, S, D)
+    for key, col, x in where:
+        bad[:, :, key, col] = x
+        finite[:, :, key, col] = 0
+        want[:, vis[:, key], col] += x
+    bad[0, 1, 400] = math.inf  # a whole row, in one kv head only
+    finite[0, 1, 400] = 0
+    want[1][vis[:, 400]] += math.inf
+    out = bk.flash_attention(q.to(cuda), k.to(cuda), bad.to(cuda), causal=kw.get("causal", False),
+                             window=kw.get("window", 0), softcap=kw.get("cap", 0.0),
+                             alibi_slopes=None if sl is None else sl.to(cuda),
+                             doc_offsets=_i32([kw["docs"]], cuda) if "docs" in kw else _i32([[0, S]], cuda),
+                             prefix_lens=_i32([[kw["prefix"]]], cuda) if "prefix" in kw else None).double().cpu()[0]
+    pos = torch.arange(S).double()
+    for h in range(Hq):
+        w = want[h // 2]
+        bias = None if sl is None else -sl[h].double() * (pos[:, None] - pos).abs()
+        o, av, mag = scored.rows(q[0, h], k[0, h // 2], finite[0, h // 2], vis, 1 / math.sqrt(D), kw.get("cap", 0.0), bias)
+        lim = scored.bound(o, av, mag, dt, S, D, kw.get("cap", 0.0), 0.0 if sl is None else float(sl[h]) * S)
+        fine = w == 0
+        assert bool(((out[h] - o).abs() <= lim)[fine].all()), h
+        assert _same_kind(out[h][~fine], w[~fine].double()), h
+
+
+def _slopes(h):
+    """Gentle ones: no visible key's weight falls to 0 in fp32, which would make NaN of its infinity."""
+    return torch.tensor([2.0 ** -(4 + i) for i in range(h)], dtype=F32)
+
+
+@pytest.mark.gpu
+def test_prompt_hidden_values_many_turns(cuda):
+    """More units than 31 turns of all CTAs: rows of every turn are looked at again."""
+    g = torch.Generator(device=cuda).manual_seed(1)
+    B, H, S, D = 16, 64, 1200, 64
+    q, k, v = (torch.randn(B, H, S, D, generator=g, device=cuda).bfloat16() for _ in range(3))
+    docs = _i32([[0, 500, 1190]] * B, cuda)
+    run = lambda: bk.flash_attention(q, k, v, causal=True, doc_offsets=docs)
+    clean = run()
+    v[:, :, 1190:] = math.nan
+    v[:, :, 500, 7] = math.inf
+    out = run()
+    far = 2.0 ** -6  # two outputs, each within the bound of weights rounded to 16 bits, |o| up to 4 in their rows
+    sees = torch.zeros(S, D, dtype=torch.bool, device=cuda)
+    sees[500:1190, 7] = True
+    assert (out[:, :, sees] == math.inf).all()
+    assert not out[:, :, 1190:].any()
+    diff = (out.float() - clean.float()).abs()[:, :, ~sees]
+    assert bool((diff <= far * (1 + clean.float().abs()[:, :, ~sees])).all())
+
+
+def _us(f, n=9):
+    for _ in range(2):
+        f()
+    ev = [[torch.cuda.Event(enable_timing=True) for _ in range(2)] for _ in range(n)]
+    for a, z in ev:
+        a.record()
+        f()
+        z.record()
+    torch.cuda.synchronize()
+    return sorted(a.elapsed_time(z) for a, z in ev)[n // 2] * 1e3
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt,D", [(BF16, 128), (F16, 64)])
+def test_prompt_cost_of_what_is_not_finite(cuda, dt, D):
+    """A NaN that the rows do see costs a look at their tiles' hidden keys, not their attention anew, and one that they
+    must not see only the rows whose tiles hold it."""
+    H, S = 16, 4096
+    q, k, v = (torch.randn(1, H, S, D, device=cuda, dtype=dt) for _ in range(3))
+    docs = _i32([[0, 4000]], cuda)
+    run = lambda: _us(lambda: bk.flash_attention(q, k, v, causal=True, doc_offsets=docs))
+    clean = run()
+    v[:, :, 0, 5] = math.nan
+    seen = run()
+    v[:, :, 2000:4000] = math.nan
+    most = run()
+    v[:, :, :4000] = 0
+    v[:, :, 4000:] = math.nan
+    padding = run()
+    assert seen <= 3 * clean and most <= 6 * clean + 2000 and padding <= 40 * clean, (clean, seen, most, padding)
+
+
 # ------------------------------------------------------------ pages
 @pytest.mark.gpu
 @pytest.mark.parametrize("dt,D", [(BF16, 128), (F16, 64), (BF16, 256), (F32, 64)])

@@ -103,35 +103,272 @@ __device__ __forceinline__ void range_bits(uint32_t (&vis)[4], int lo, int hi, i
   }
 }
 
-// 32 columns (from `col` on) of a row, key by key, for an output that is not finite: the
-// tiles' PV takes every key of a tile, and a hidden one's infinity or NaN times
-// its weight of 0 is NaN.  Slow (no tile, no tensor core) and rarely needed.
-struct Row {
-  const uint16_t *q, *k, *v;
-  int64_t ks, vs;
-  int lo, hi, pos;
-};
+// Rows looked at again.  A tile's PV takes every key of the tile, and a hidden one's
+// infinity or NaN in V times its weight of 0 is NaN.  In fp16 a visible one's weight
+// may round to 0 as well (below 2^-25, where bf16's last is fp32's), which makes NaN
+// of an infinity.  So rows whose output is not finite are looked at once more when
+// all turns are over (no wait with a limit is left then, and the tiles' shared
+// memory is free):
+//   * a key in V that is not finite and hidden from a row (fp16: from any of the
+//     warp's 32 rows) in a tile that was taken for it: the row is computed anew over
+//     the keys that it sees, 32 at a time, one key a lane for the scores and HD / 32
+//     columns a lane for PV;
+//   * fp16, such keys only where all rows see them: their columns are the sum of
+//     those values, whatever the weights;
+//   * else the row is what the formula gives.
+// Each softmax warp finds out about its own rows; rows to compute anew go through a
+// list in shared memory to all eight, four at a time.  8192 tokens, causal, 32 heads
+// of 128: 0.57 ms clean, 0.64 (fp16 0.75) with a NaN in V of token 0, which all rows
+// see, 3.1 with NaN in 96 tokens of padding, whose tile 32 rows of each head share.
+template <int FMT>
+__device__ __forceinline__ bool any_not_finite(const uint4& x) {
+  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+  bool hit = false;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) hit |= not_finite16<FMT>(w[e]) | not_finite16<FMT>(w[e] >> 16);
+  return hit;
+}
+
+// First (LAST: last) of the keys [a, z) with a value in V (rows vs apart) that is
+// not finite; LAST ? -1 : INT_MAX where there is none.  For a whole warp.
+template <int HD, int FMT, bool LAST>
+__device__ __forceinline__ int bad_key(const uint16_t* v, int64_t vs, int a, int z) {
+  constexpr int NL = HD / 8, KEYS = 32 / NL, U = 4;  // lanes a key, keys side by side, steps in flight
+  const int lane = threadIdx.x & 31, none = LAST ? -1 : INT_MAX;
+  for (int i0 = 0; i0 < z - a; i0 += KEYS * U) {
+    uint4 x[U];
+    int best = none;
+#pragma unroll
+    for (int e = 0; e < U; ++e) {
+      const int i = i0 + e * KEYS + lane / NL, key = LAST ? z - 1 - i : a + i;
+      x[e] = i < z - a ? *reinterpret_cast<const uint4*>(v + key * vs + lane % NL * 8) : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int e = 0; e < U; ++e) {
+      const int i = i0 + e * KEYS + lane / NL, key = LAST ? z - 1 - i : a + i;
+      if (any_not_finite<FMT>(x[e])) best = LAST ? max(best, key) : min(best, key);
+    }
+    best = LAST ? __reduce_max_sync(0xffffffffu, best) : __reduce_min_sync(0xffffffffu, best);
+    if (best != none) return best;
+  }
+  return none;
+}
+
+// HD / 32 columns of V, this lane's
+template <int HD, int FMT>
+__device__ __forceinline__ void load_columns(float (&o)[HD / 32], const uint16_t* v) {
+  const int lane = threadIdx.x & 31;
+  uint32_t w[HD / 64];
+  if constexpr (HD == 128) *reinterpret_cast<uint2*>(w) = *reinterpret_cast<const uint2*>(v + 4 * lane);
+  else w[0] = *reinterpret_cast<const uint32_t*>(v + 2 * lane);
+#pragma unroll
+  for (int e = 0; e < HD / 64; ++e) {
+    o[2 * e] = widen16<FMT>((uint16_t)w[e]);
+    o[2 * e + 1] = widen16<FMT>((uint16_t)(w[e] >> 16));
+  }
+}
+
+// Whether V of the keys lo and hi - 1, the first and the last that a row sees, makes
+// NaN of all its columns (as in a prompt that is NaN from some token on).
+template <int HD, int FMT>
+__device__ __forceinline__ bool all_nan(const uint16_t* vb, int64_t vs, int lo, int hi) {
+  float x[HD / 32], y[HD / 32];
+  load_columns<HD, FMT>(x, vb + lo * vs);
+  load_columns<HD, FMT>(y, vb + (hi - 1) * vs);
+  bool nan = true;
+#pragma unroll
+  for (int e = 0; e < HD / 32; ++e) nan = nan && (x[e] != x[e] || y[e] != y[e]);
+  return __all_sync(0xffffffffu, nan);
+}
+
+// The rows first + r, r in `rows` (a bit each, kAgain at most), of a unit over the
+// keys that they see, by one warp; they share what they load.
+constexpr int kAgain = 4;
 template <int HD, int FMT, bool CAP, bool BIAS>
-__device__ __noinline__ void again(float (&o)[32], const Row& r, int col, float m, const Score& sc) {
+__device__ __forceinline__ void compute_rows(const Params& p, const Unit& un, int first, uint32_t rows, const Score& sc) {
+  constexpr int V = HD / 32;
+  const int lane = threadIdx.x & 31, hk = un.h / (p.Hq / p.Hkv);
+  const uint16_t* qb = p.q + un.b * p.qs[0] + un.h * p.qs[1];
+  const uint16_t* kb = p.k + un.b * p.ks[0] + hk * p.ks[1];
+  const uint16_t* vb = p.v + un.b * p.vs[0] + hk * p.vs[1];
+  int row[kAgain], from[kAgain], to[kAgain], a = INT_MAX, z = 0;  // row < 0: none
 #pragma unroll
-  for (int e = 0; e < 32; ++e) o[e] = 0.f;
-  for (int key = r.lo; key < r.hi; ++key) {
-    const uint16_t *k = r.k + key * r.ks, *v = r.v + key * r.vs + col;
-    float s = 0.f;
-    for (int d = 0; d < HD; d += 8) {
-      const uint4 a = *reinterpret_cast<const uint4*>(r.q + d), b = *reinterpret_cast<const uint4*>(k + d);
-      const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
+  for (int i = 0; i < kAgain; ++i) {
+    row[i] = rows ? first + __ffs(rows) - 1 : -1;
+    from[i] = to[i] = 0;
+    if (rows) {
+      attn::row_range(p.range, un.b, row[i], p.Skv, from[i], to[i]);
+      a = min(a, from[i]);
+      z = max(z, to[i]);
+    }
+    rows &= rows - 1;
+  }
+  float m[kAgain], l[kAgain], acc[kAgain][V];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        s = fmaf(widen16<FMT>((uint16_t)x[e]), widen16<FMT>((uint16_t)y[e]), s);
-        s = fmaf(widen16<FMT>((uint16_t)(x[e] >> 16)), widen16<FMT>((uint16_t)(y[e] >> 16)), s);
+  for (int i = 0; i < kAgain; ++i) {
+    m[i] = -INFINITY;
+    l[i] = 0.f;
+#pragma unroll
+    for (int e = 0; e < V; ++e) acc[i][e] = 0.f;
+  }
+  for (int key0 = a; key0 < z; key0 += 32) {
+    const int key = key0 + lane;
+    float w[kAgain] = {};  // scores, then weights; < 0: the row does not see the key
+    if (key < z) {
+      const uint16_t* k = kb + key * p.ks[2];
+#pragma unroll 4
+      for (int d = 0; d < HD; d += 8) {
+        const uint4 y = *reinterpret_cast<const uint4*>(k + d);
+        const uint32_t b[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int i = 0; i < kAgain; ++i) {
+          const uint4 q = *reinterpret_cast<const uint4*>(qb + max(row[i], 0) * p.qs[2] + d);
+          const uint32_t c[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            w[i] = fmaf(widen16<FMT>((uint16_t)c[e]), widen16<FMT>((uint16_t)b[e]), w[i]);
+            w[i] = fmaf(widen16<FMT>((uint16_t)(c[e] >> 16)), widen16<FMT>((uint16_t)(b[e] >> 16)), w[i]);
+          }
+        }
       }
     }
-    float t = -m;
-    if constexpr (BIAS) t = fmaf(-sc.slope0, fabsf((float)(r.pos - key)), t);
-    const float w = ex2(CAP ? capped_any(s, sc, t) : fmaf(s, sc.scale_log2, t));
-    for (int e = 0; e < 32; ++e) o[e] = fmaf(w, widen16<FMT>(v[e]), o[e]);
+#pragma unroll
+    for (int i = 0; i < kAgain; ++i) {
+      const bool sees = key >= from[i] && key < to[i];
+      float add = 0.f;
+      if constexpr (BIAS) add = -sc.slope0 * fabsf((float)(row[i] - key));
+      const float x = CAP ? capped_any(w[i], sc, add) : fmaf(w[i], sc.scale_log2, add);
+      float mx = sees ? x : -INFINITY;
+#pragma unroll
+      for (int off = 16; off; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+      const float mn = fmaxf(m[i], mx), ref = mn == -INFINITY ? 0.f : mn;
+      const float alpha = m[i] == -INFINITY ? 0.f : ex2(m[i] - ref);
+      w[i] = sees ? ex2(x - ref) : -1.f;
+      m[i] = mn;
+      l[i] = l[i] * alpha + (sees ? w[i] : 0.f);
+#pragma unroll
+      for (int e = 0; e < V; ++e) acc[i][e] *= alpha;
+    }
+    const int n = min(z - key0, 32);
+#pragma unroll 8
+    for (int j = 0; j < n; ++j) {
+      float y[V];
+      load_columns<HD, FMT>(y, vb + (key0 + j) * p.vs[2]);
+#pragma unroll
+      for (int i = 0; i < kAgain; ++i) {
+        const float wj = __shfl_sync(0xffffffffu, w[i], j);
+        if (!(wj < 0.f))
+#pragma unroll
+          for (int e = 0; e < V; ++e) acc[i][e] = fmaf(wj, y[e], acc[i][e]);
+      }
+    }
   }
+#pragma unroll
+  for (int i = 0; i < kAgain; ++i) {
+#pragma unroll
+    for (int off = 16; off; off >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], off);
+    if (row[i] < 0) continue;
+    const float inv = l[i] == 0.f ? 0.f : 1.f / l[i];
+    uint16_t* o = reinterpret_cast<uint16_t*>(p.o) + un.b * p.os_b + un.h * p.os_h + row[i] * p.os_s + V * lane;
+#pragma unroll
+    for (int e = 0; e < V / 2; ++e)
+      reinterpret_cast<uint32_t*>(o)[e] = narrow2<FMT>(acc[i][2 * e] * inv, acc[i][2 * e + 1] * inv);
+  }
+}
+
+// fp16, 32 rows (sees: this lane's row) whose keys that are not finite in V are all
+// among [a, z), which each of them sees.  Returns those of them to compute anew, a
+// bit each.
+template <int HD>
+__device__ __forceinline__ uint32_t columns_again(const Params& p, const Unit& un, int first, bool sees, int a, int z,
+                                                  const uint16_t* vb) {
+  constexpr int NL = HD / 8, KEYS = 32 / NL, U = 8;
+  const int lane = threadIdx.x & 31;
+  const uint32_t rows = __ballot_sync(0xffffffffu, sees);
+  auto at = [&](int r) {  // 8 columns of row first + r
+    return reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.o) + un.b * p.os_b + un.h * p.os_h + (first + r) * p.os_s +
+                                    lane % NL * 8);
+  };
+  uint32_t want = 0;  // this lane's columns, 8 (lane % NL) .., that are NaN in some row
+  for (uint32_t left = rows; left; left &= left - 1) {
+    Kinds have = {0, 0, 0};
+    find_kinds<kF16>(*at(__ffs(left) - 1), have);
+    want |= have.nan;
+  }
+  // V from key a on, until those columns are known to be NaN by the formula
+  Kinds k = {0, 0, 0};
+  for (int i0 = a; i0 < z; i0 += KEYS * U) {
+    if (__all_sync(0xffffffffu, !(want & ~k.undefined()))) return 0;
+    uint4 x[U];
+#pragma unroll
+    for (int e = 0; e < U; ++e) {
+      const int key = i0 + e * KEYS + lane / NL;
+      x[e] = key < z ? *reinterpret_cast<const uint4*>(vb + key * p.vs[2] + lane % NL * 8) : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int e = 0; e < U; ++e)
+      if (any_not_finite<kF16>(x[e])) find_kinds<kF16>(x[e], k);
+#pragma unroll
+    for (int off = NL; off < 32; off <<= 1) {
+      k.pos |= __shfl_xor_sync(0xffffffffu, k.pos, off);
+      k.neg |= __shfl_xor_sync(0xffffffffu, k.neg, off);
+      k.nan |= __shfl_xor_sync(0xffffffffu, k.nan, off);
+    }
+  }
+  const uint32_t wrong = k.any() & ~k.undefined();
+  uint32_t anew = 0;
+  for (uint32_t left = rows; left; left &= left - 1) {
+    const int r = __ffs(left) - 1;
+    uint4 x = *at(r);
+    Kinds have = {0, 0, 0};
+    find_kinds<kF16>(x, have);
+    if (__all_sync(0xffffffffu, have.nan == 0xffu)) {  // its scores, or all columns
+      anew |= 1u << r;
+      continue;
+    }
+    uint32_t* w = reinterpret_cast<uint32_t*>(&x);
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (have.nan & wrong & 1u << e) {
+        const uint32_t h = __half_as_ushort(__float2half_rn(k.sum(e)));
+        w[e >> 1] = e & 1 ? (w[e >> 1] & 0xffffu) | h << 16 : (w[e >> 1] & 0xffff0000u) | h;
+      }
+    if (lane < NL && (have.nan & wrong)) *at(r) = x;
+  }
+  return anew;
+}
+
+// Which of the rows first .. first + 31 of the Q tile from row q0 on to compute
+// anew, a bit each.
+template <int HD, int FMT>
+__device__ __forceinline__ uint32_t rows_again(const Params& p, const Unit& un, int q0, int first) {
+  const int lane = threadIdx.x & 31, hk = un.h / (p.Hq / p.Hkv);
+  const uint16_t* vb = p.v + un.b * p.vs[0] + hk * p.vs[1];
+  int t0 = INT_MAX, t1 = 0, lo = 0, hi = 0;  // the tile's first key and end; this lane's row
+  for (int i = 0; i < BQ / 32; ++i) {
+    const int row = q0 + 32 * i + lane;
+    int a = 0, z = 0;
+    if (row < p.Sq) attn::row_range(p.range, un.b, row, p.Skv, a, z);
+    if (z > a) t0 = min(t0, a), t1 = max(t1, z);
+    if (q0 + 32 * i == first) lo = a, hi = z;
+  }
+  t0 = __reduce_min_sync(0xffffffffu, t0) / BKV * BKV;
+  t1 = min((__reduce_max_sync(0xffffffffu, t1) + BKV - 1) / BKV * BKV, p.Skv);  // zeros behind the last key
+  const bool sees = hi > lo;
+  const int before = __reduce_max_sync(0xffffffffu, sees ? lo : 0);
+  const int behind = __reduce_min_sync(0xffffffffu, sees ? hi : INT_MAX);
+  const int bad0 = bad_key<HD, FMT, false>(vb, p.vs[2], t0, before);
+  const int bad1 = bad_key<HD, FMT, true>(vb, p.vs[2], behind, t1);
+  if (bad0 == INT_MAX && bad1 == -1) {
+    if constexpr (FMT == kF16) return columns_again<HD>(p, un, first, sees, before, behind, vb);
+    return 0;
+  }
+  uint32_t again = __ballot_sync(0xffffffffu, sees && (FMT == kF16 || bad0 < lo || bad1 >= hi));
+  for (uint32_t left = again; left; left &= left - 1) {
+    const int r = __ffs(left) - 1;
+    if (all_nan<HD, FMT>(vb, p.vs[2], __shfl_sync(0xffffffffu, lo, r), __shfl_sync(0xffffffffu, hi, r))) again &= ~(1u << r);
+  }
+  return again;
 }
 
 template <int HD, int FMT, bool CAP, bool BIAS>
@@ -405,6 +642,7 @@ scored_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
     const uint32_t tS = tmem + 256 * u + lane_off, tO = tS + 128;
     Score score = make_score(p.cap);
     uint32_t sc = 0, oc = 0;  // S tiles / outputs waited for
+    uint32_t sick = 0;        // turns with a row to look at again (bit 31: all from the 31st on)
     bool ok = true;
     int next_lo = 0, next_hi = 0;
     auto find_row = [&](int k) {  // keys of this thread's row in turn k
@@ -463,26 +701,17 @@ scored_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
       ++oc;
       tc::fence_after_sync();
       const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-      const int hk = un.h / (p.Hq / p.Hkv);
 #pragma unroll 1
       for (int c = 0; c < HD / 32; ++c) {
         float o[32];
         tc::tmem_ld_32x32b_x32(tO + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(o));
         tc::tmem_ld_wait();
-        if (any_masked) {
-          // 0 x infinity: V of a hidden key may have made NaN of the row
+        if ((any_masked || FMT == kF16) && exists) {
           float sum = 0.f;
 #pragma unroll
           for (int e = 0; e < 32; ++e) sum = fmaf(o[e], 0.f, sum);
-          if (sum != 0.f && l != 0.f && exists) {
-            const Row rw = {p.q + un.b * p.qs[0] + un.h * p.qs[1] + (int64_t)qpos * p.qs[2],
-                            p.k + un.b * p.ks[0] + hk * p.ks[1], p.v + un.b * p.vs[0] + hk * p.vs[1], p.ks[2], p.vs[2],
-                            row_lo, row_hi, qpos};
-            float t[32];  // not o itself: that would have to live in local memory
-            again<HD, FMT, CAP, BIAS>(t, rw, 32 * c, m_used, score);
-#pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = t[e];
-          }
+          // (a row whose weights add up to 0 or NaN is 0 or NaN anyway)
+          if (sum != 0.f && l != 0.f && l == l) sick |= 1u << min(k, 31);
         }
         if (l == 0.f) {
 #pragma unroll
@@ -500,6 +729,36 @@ scored_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
       }
       // the next unit's first PV overwrites O_u once this warpgroup hands over a P
       tc::fence_before_sync();
+    }
+    // rows looked at again
+    if (any_of_softmax(sick != 0) && !any_of_softmax(!ok)) {
+      struct Entry {
+        int turn, warp;  // u * 4 + qw
+        uint32_t rows;
+      };
+      constexpr int kTurns = (kQ * kTile - 16) / (8 * (int)sizeof(Entry));  // a round's, eight warps each
+      int* count = reinterpret_cast<int*>(sQ);
+      Entry* list = reinterpret_cast<Entry*>(sQ + 16);
+      sick = __reduce_or_sync(0xffffffffu, sick);
+      for (int k0 = 0; unit_of(p, k0, un); k0 += kTurns) {
+        any_of_softmax(false);  // the round before is over
+        if (threadIdx.x == 128) *count = 0;
+        any_of_softmax(false);
+        for (int k = k0; k < k0 + kTurns && u < p.per && sick >> min(k, 31) && unit_of(p, k, un); ++k) {
+          if (!(sick >> min(k, 31) & 1)) continue;
+          const uint32_t rows = rows_again<HD, FMT>(p, un, un.q0 + u * BQ, un.q0 + u * BQ + qw * 32);
+          if (rows && lane == 0) list[atomicAdd(count, 1)] = {k, u * 4 + qw, rows};
+        }
+        any_of_softmax(false);
+        for (int t = warp - 4, n = 8 * *count; t < n; t += 8) {
+          const Entry e = list[t / 8];
+          const uint32_t rows = e.rows & 0xfu << t % 8 * 4;
+          if (!rows) continue;
+          unit_of(p, e.turn, un);
+          if constexpr (BIAS) score.slope0 = p.slopes[un.h] * attn::kLog2e;
+          compute_rows<HD, FMT, CAP, BIAS>(p, un, un.q0 + e.warp * 32, rows, score);
+        }
+      }
     }
   }
 
@@ -565,8 +824,8 @@ extern "C" int b2_flash_attn_fwd_scored(const void* q, const void* k, const void
   bool wide = aligned(q, 16) && aligned(k, 16) && aligned(v, 16) && aligned(o, 16);
   for (int i = 0; i < 3; ++i) wide = wide && qs[i] % 8 == 0 && ks[i] % 8 == 0 && vs[i] % 8 == 0 && os[i] % 8 == 0;
   // scale > 0: the row maximum is taken before the scale.  fp32 stays fp32 here
-  // (the plain kernel reads it as tf32 at head dim 64).  Up to 2^20 keys a row
-  // that is done again takes about a second, well inside the others' waits.
+  // (the plain kernel reads it as tf32 at head dim 64).  2^20 keys bound the time
+  // that rows computed anew may take: 0.3 s for 32 of them over so many.
   unsigned* err = device_error_word();
   if (wide && (D == 64 || D == 128) && dtype != B2_F32 && scale > 0.f && Skv > 0 && err &&
       B * Hq * ((Sq + fa::BQ - 1) / fa::BQ) <= (1 << 30) && Skv <= (1 << 20)) {
