@@ -335,6 +335,35 @@ def test_tree_nan_scores(cuda, dt, D, T, rep):
     assert torch.equal(out[:, :-1, rep:], clean[:, :-1, rep:])
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [F32, BF16, F16])
+@pytest.mark.parametrize("D", [64, 80])
+def test_infinities_of_no_weight(cuda, dt, D):
+    """An infinity in V of a key that a row sees with a weight far below fp32's smallest is in its output, as an
+    infinity or as NaN (0 times infinity)."""
+    g = torch.Generator().manual_seed(D)
+    S = 400
+    q, k, v = (_rand(g, 1, 2, S, D, dt=dt) for _ in range(3))
+    bad = v.clone()
+    bad[:, :, 0, 3], bad[:, :, S - 1, 4] = math.inf, -math.inf
+    slope = torch.tensor([2.0, 4.0], device=cuda)  # 800 to 1600 over the prompt
+    run = lambda x: bk.flash_attention(q.to(cuda), k.to(cuda), x.to(cuda), causal=True, alibi_slopes=slope).cpu()[0]
+    clean, out = run(v), run(bad)
+    assert not torch.isfinite(out[:, :, 3]).any()
+    assert torch.isfinite(out[:, :-1, 4]).all() and (out[:, -1, 4] == -math.inf).all()
+    # a tree whose first context key scores 128 or more below the rest
+    q2 = torch.full((1, 3, 2, D), 4.0, dtype=dt)
+    k2 = k.abs()
+    k2[:, :, 0] = -4
+    tree = lambda x: bk.tree_attention(q2.to(cuda), k2.to(cuda), x.to(cuda), _i32([S - 3], cuda),
+                                       torch.tril(torch.ones(3, 3, dtype=torch.bool, device=cuda))).cpu()[0]
+    clean, out = tree(v), tree(bad)
+    assert not torch.isfinite(out[..., 3]).any()
+    assert torch.isfinite(out[:-1, :, 4]).all() and not torch.isfinite(out[-1, :, 4]).any()
+    rest = [d for d in range(D) if d not in (3, 4)]
+    assert torch.equal(out[..., rest], clean[..., rest])
+
+
 # --------------------------------- infinities and NaN that a row must not see
 @pytest.mark.gpu
 @pytest.mark.parametrize("dt,D", [(BF16, 128), (F16, 64), (F32, 64)])

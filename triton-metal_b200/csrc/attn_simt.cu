@@ -214,7 +214,8 @@ __global__ void __launch_bounds__(kThreads) simt_kernel(const SimtParams p) {
       float ts = 0.f;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float e = s[i][j] == -INFINITY ? 0.f : exp2f(fmaf(s[i][j], kLog2e, -rl));
+        // -0: a key that the row does not see
+        const float e = s[i][j] == -INFINITY ? -0.f : exp2f(fmaf(s[i][j], kLog2e, -rl));
         ts += e;
         sP[rr * (BN + 4) + tx + 16 * j] = e;
       }
@@ -247,16 +248,20 @@ __global__ void __launch_bounds__(kThreads) simt_kernel(const SimtParams p) {
           }
       }
     } else {
-      // some V of the tile is infinite or NaN: a weight of 0 must drop it, not
-      // multiply it
+      // some V of the tile is infinite or NaN: one that the row does not see must be
+      // dropped, not multiplied by 0, and one that it sees counts whatever its weight
+      // (0 where the score is too far below the largest)
       for (int j = 0; j < BN; ++j)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const float pj = sP[(ty * 4 + i) * (BN + 4) + j];
-          if (pj != 0.f)
+          if (__float_as_uint(pj) != 0x80000000u)
 #pragma unroll
-            for (int d = 0; d < DP / 16; ++d)
-              acc[i][d] = fmaf(pj, sV[j * C::LD + 64 * (d >> 2) + 4 * tx + (d & 3)], acc[i][d]);
+            for (int d = 0; d < DP / 16; ++d) {
+              const float vv = sV[j * C::LD + 64 * (d >> 2) + 4 * tx + (d & 3)];
+              if (pj != 0.f) acc[i][d] = fmaf(pj, vv, acc[i][d]);
+              else if (!(fabsf(vv) < INFINITY)) acc[i][d] += vv;
+            }
         }
     }
   }
