@@ -499,6 +499,37 @@ def test_token_pages_of_every_tile(cuda, dt, D, ps, cap):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dt,D", [(BF16, 128), (F16, 64), (F32, 64)])
+@pytest.mark.parametrize("T", [2, 9, 40])
+@pytest.mark.parametrize("ps", [8, 16, 24, 128])
+def test_tree_pages_outside_in_every_tile(cuda, dt, D, T, ps):
+    """Every third page number lies outside the cache: zeros there, call after call, whatever the ring held before."""
+    lib = _lib.load()
+    code, stream = ctypes.c_uint(0), torch.cuda.current_stream().cuda_stream
+    g = torch.Generator().manual_seed(D + ps)
+    ctx, S = [900, 130], 900 + T
+    q, k, v = _rand(g, 2, T, 8, D, dt=dt), _rand(g, 2, 2, S, D, dt=dt), _rand(g, 2, 2, S, D, dt=dt)
+    kp, vp, table = _pages(k, v, ps, g)
+    mask = torch.tril(torch.ones(T, T, dtype=torch.bool))
+    table[:, ::3] = torch.tensor([-1, 2 ** 31 - 1], dtype=torch.int32)[:, None]
+    gone = (torch.arange(S) // ps) % 3 == 0
+    k[:, :, gone] = 0
+    v[:, :, gone] = 0
+    run = lambda: bk.tree_attention(q.to(cuda), kp.to(cuda), vp.to(cuda), _i32(ctx, cuda), mask.to(cuda),
+                                    page_table=table.to(cuda))
+    out = run()
+    for _ in range(5):
+        assert torch.equal(run(), out)
+    lib.b2_device_error(stream, ctypes.byref(code))
+    assert code.value == 0xB2500001
+    out = out.double().cpu()
+    for b, n in enumerate(ctx):
+        for h in range(8):
+            o, av, mag = scored.tree(q[b, :, h], k[b, h // 4], v[b, h // 4], n, T, mask, 1 / math.sqrt(D))
+            assert bool(((out[b, :, h] - o).abs() <= scored.bound(o, av, mag, dt, n + T, D)).all()), (b, h)
+
+
+@pytest.mark.gpu
 def test_token_pages_cost(cuda):
     """Single tokens over pages of 64 keys: the page table's latency does not stand before every tile (1.33 times the
     contiguous cache's time with the pages looked up a tile ahead, 1.94 with a check and a branch among the loads)."""

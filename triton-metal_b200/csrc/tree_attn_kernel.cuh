@@ -410,6 +410,7 @@ tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
         tc::fence_proxy_async_smem();
       }
       const int n = __popc(__ballot_sync(0xffffffffu, valid));
+      __syncwarp();  // zeros written before the arrival that hands them over
       if (lane == 0) mbar_arrive_expect_tx(&full[slot], n * p.box * 128 + q_tiles * copies * NA * br * 128);
       __syncwarp();
       if (valid) {
