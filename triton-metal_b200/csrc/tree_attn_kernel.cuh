@@ -272,7 +272,7 @@ tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
   constexpr int kRows = PAIR ? 2 * BR : BR;  // rows of an item
   const int tokens = p.tpt * (PAIR ? 2 : 1), br = p.tpt * p.rep;  // of an item; rows of a tile
   const int copies = PAIR ? 1 : p.copies, rw = BR / copies;       // rows a copy takes up
-  extern __shared__ uint8_t smem_raw[];
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem_raw);
   uint64_t* ready = full + NS;        // TMA: a tile passed on by warps 2-3 (else unused)
