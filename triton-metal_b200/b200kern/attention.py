@@ -61,7 +61,8 @@ def flash_attention(q, k, v, causal=False, scale=None, out=None, window=0, softc
     (Mistral-style sliding window).
 
     softcap > 0 caps the scores: softcap * tanh(scale q.k / softcap).
-    alibi_slopes fp32 [Hq] subtracts slope * |query - key| from them (after the cap).
+    alibi_slopes fp32 [Hq], of either sign, subtracts slope * |query - key| from
+    them (after the cap).
     doc_offsets int32 [B, n_docs + 1], ascending: several documents packed in a
     row, tokens offsets[d] .. offsets[d + 1] - 1 each; a query sees only its own
     document (a padded batch is one document a row).  Tokens in no document see
@@ -183,7 +184,8 @@ def decode_attention(q, k_cache, v_cache, seq_lens, scale=None, page_table=None,
     Contiguous cache: k/v [B, Hkv, S, D] (any strides, last dim contiguous).
     Paged cache (page_table int32 [B, max_pages] given): k/v
     [n_pages, page_size, Hkv, D].  GQA: kv head = q head // (Hq // Hkv).
-    The cache dtype may differ from q's (e.g. fp16 KV with fp32 queries).
+    k and v share one shape and dtype; the cache or table may have more rows than
+    B.  The cache dtype may differ from q's (e.g. fp16 KV with fp32 queries).
     q_pos [B] (default seq_len - 1); window > 0 keeps the keys
     [max(0, q_pos + 1 - window), min(q_pos + 1, seq_len)) (sliding window);
     rope_freqs [D/2] rotates q at q_pos and each key at its position (RoPE).

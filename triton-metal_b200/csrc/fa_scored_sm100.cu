@@ -34,8 +34,9 @@ using namespace fa;
 //               which of them are masked
 //   warps 4-11  two softmax warpgroups, one per Q tile, one row per thread
 // Measured: 2 x 8192 tokens in 11 documents a row, causal, 32 / 8 heads of 128,
-// bf16: 272 us, 430 TF/s of visible pairs;
-// 6001 tokens, causal, cap 50, 16 / 8 heads, fp16: 273 us, 540 TF/s of visible
+// bf16: 274 to 282 us, 430 TF/s of visible pairs (one document of 8192 in each of 4
+// rows: 950, where the plain kernel has 1040);
+// 6001 tokens, causal, cap 50, 16 / 8 heads, fp16: 275 us, 540 TF/s of visible
 // pairs; 3 x 1111 tokens, prefix 300 and bias, 12 heads of 64: 40 us.  In the
 // capped case the tensor pipe is active for 28 % of the cycles and the softmax
 // warps, two a scheduler, issue in 42 %: their chains of dependent instructions
@@ -52,7 +53,7 @@ struct Params {
   const float* slopes;     // [Hq]
   void* o;
   int64_t os_b, os_h, os_s;
-  const uint16_t *q, *k, *v;  // for rows that are done again
+  const uint16_t *q, *k, *v;  // for rows that are looked at again
   int64_t qs[3], ks[3], vs[3];
   unsigned* err;
 };

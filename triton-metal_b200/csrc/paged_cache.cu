@@ -23,10 +23,11 @@ namespace paged {
 // either read or written, never both, and nothing has to wait for anything.
 // Latency sets the time (a step moves kilobytes), so it is one launch: every
 // CTA redoes the scan over the requests up to its own tokens (kReqs of them
-// per round) instead of waiting for a first kernel to publish it.  A call takes
-// 8.8 us for 256 requests of one token and for 93 prompts of up to 4099 (1.6 MB),
-// about 5 of which any launch from Python takes; the rest are dependent loads:
-// lengths, table or free list, slots.
+// per round) instead of waiting for a first kernel to publish it.  256 requests of
+// one token: the kernel takes 4.2 us (calls in a graph; dependent loads: lengths,
+// table or free list, slots), a call from Python 8.5, which is what the host needs
+// for three outputs, their tuple and the launch; 93 prompts of up to 4099 tokens
+// (1.6 MB) the same.
 // ---------------------------------------------------------------------------
 constexpr int kThreads = 256;
 constexpr int kPer = 4;                    // requests / tokens per thread
@@ -171,7 +172,7 @@ __global__ void __launch_bounds__(kThreads) build_table_kernel(const TableParams
 // a chunk by the head size is done once per thread and column, and the 64-bit
 // division of a slot by the page size once per row (in shared memory).  60001
 // fp32 rows of 8 x 128 into an fp16 cache, 738 MB: 131 us, 5.6 TB/s (0.86 of a
-// copy's rate); 201 rows: 5.4 us, a launch.
+// copy's rate); 201 rows: 2.0 us in a graph, 5.2 a call.
 // ---------------------------------------------------------------------------
 constexpr int kMaxRows = 64;  // rows per CTA
 constexpr int kRows = 4;      // rows in flight per thread

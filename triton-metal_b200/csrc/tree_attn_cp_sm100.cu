@@ -1,5 +1,6 @@
 // Attention of a tree of drafted tokens and of single tokens: the cp.async form,
-// for page sizes that are no multiple of 8.
+// for page sizes that are no multiple of 8 and for tensors that no tensor map
+// describes.
 #include "tree_attn_kernel.cuh"
 
 namespace b2 {

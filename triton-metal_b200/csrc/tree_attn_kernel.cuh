@@ -41,10 +41,10 @@
 // others), so that all warps share the exponentials.  The copies are joined like
 // the units, through shared memory.
 // Measured: trees of 64, 32 requests of 8 to 32 thousand keys, 32 / 8 heads of
-// 128, bf16: 0.88 ms, 3.1 TB/s and 780 TF/s (either floor is 0.42 ms; the softmax
-// between a tile's two MMAs sets the time); trees of 26, 16 requests of up to
-// 4096 keys in pages of 16, fp16: 56 us, 2.6 TB/s (starts and ends of segments);
-// a tree of 8, one request of 500 keys: 20 us (two launches and one chain).
+// 128, bf16: 0.86 to 0.91 ms, 3.1 TB/s and 770 TF/s (either floor is 0.42 ms);
+// trees of 26, 16 requests of up to 4096 keys in pages of 16, fp16: 57 us, 2.5 TB/s
+// (starts and ends of segments); a tree of 8, one request of 500 keys: 19 to 20 us
+// (two launches and one chain).
 #pragma once
 #include "attn_common.cuh"
 #include "fa_common.cuh"
