@@ -434,6 +434,19 @@ def test_prompt_hidden_values_many_turns(cuda):
     assert bool((diff <= far * (1 + clean.float().abs()[:, :, ~sees])).all())
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("D,B", [(64, 300), (128, 600)])
+def test_prompt_hidden_values_many_rounds(cuda, D, B):
+    """More units than the list of rows to compute anew has room for at once."""
+    g = torch.Generator(device=cuda).manual_seed(2)
+    q, k, v = (torch.randn(B, 256, 2, D, generator=g, device=cuda).bfloat16() for _ in range(3))
+    first = v[:, :, 0].clone()
+    v[:, :, 1, ::2] = math.inf
+    out = bk.flash_attention(q, k, v, causal=True, doc_offsets=_i32([[0, 2]] * B, cuda))
+    assert torch.equal(out[:, :, 0], first)  # its only key
+    assert (out[:, :, 1, ::2] == math.inf).all() and torch.isfinite(out[:, :, 1, 1::2]).all()
+
+
 def _us(f, n=9):
     for _ in range(2):
         f()
