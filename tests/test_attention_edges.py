@@ -364,6 +364,23 @@ def test_infinities_of_no_weight(cuda, dt, D):
     assert torch.equal(out[..., rest], clean[..., rest])
 
 
+# ------------------------------------------------------------- prefixes
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt,D", [(BF16, 128), (F16, 64), (F32, 64), (BF16, 80)])
+def test_prefix_of_a_document_that_begins_before_the_row(cuda, dt, D):
+    """Offsets may lie before the row's first token; a document's prefix counts from where it begins."""
+    g = torch.Generator().manual_seed(D)
+    S, docs, prefix = 300, [[-400, 130, 300], [-5, 2, 290]], [[460, 60], [3, 2 ** 31 - 1]]
+    q, k, v = (_rand(g, 2, 2, S, D, dt=dt, big=2.0) for _ in range(3))
+    out = bk.flash_attention(q.to(cuda), k.to(cuda), v.to(cuda), causal=True, doc_offsets=_i32(docs, cuda),
+                             prefix_lens=_i32(prefix, cuda)).double().cpu()
+    for b in range(2):
+        vis = scored.ranges(S, S, True, 0, docs[b], prefix[b])
+        for h in range(2):
+            o, av, mag = scored.rows(q[b, h], k[b, h], v[b, h], vis, 1 / math.sqrt(D))
+            assert bool(((out[b, h] - o).abs() <= scored.bound(o, av, mag, dt, S, D)).all()), (b, h)
+
+
 # --------------------------------- infinities and NaN that a row must not see
 @pytest.mark.gpu
 @pytest.mark.parametrize("dt,D", [(BF16, 128), (F16, 64), (F32, 64)])

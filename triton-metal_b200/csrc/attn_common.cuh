@@ -25,7 +25,7 @@ struct RangeMask {
 __device__ __forceinline__ void row_range(const RangeMask& m, int b, int row, int Skv, int& lo, int& hi) {
   lo = 0;
   hi = Skv;
-  int d = 0;
+  int d = 0, start = 0;  // document and its first token, which may lie before the row's
   if (m.docs) {
     const int32_t* off = m.docs + (int64_t)b * (m.n_docs + 1);
     int a = 0, z = m.n_docs;  // d = how many of off[1..n_docs] are <= row
@@ -37,16 +37,17 @@ __device__ __forceinline__ void row_range(const RangeMask& m, int b, int row, in
     d = a;
     lo = hi = 0;
     if (d < m.n_docs && off[d] <= row && row < off[d + 1]) {
-      lo = max(off[d], 0);
+      start = off[d];
+      lo = max(start, 0);
       hi = min(off[d + 1], Skv);
     }
   }
   if (m.causal) {
     int last = row + 1;
     if (m.prefix) {
-      // prefix lengths are clamped to [0, Skv] so that the sum stays in 32 bits
+      // prefix lengths are clamped so that the sum stays in 32 bits
       const int p = m.prefix[(int64_t)b * max(m.n_docs, 1) + min(d, max(m.n_docs, 1) - 1)];
-      last = max(last, lo + min(max(p, 0), Skv));
+      last = max(last, start + (start < 0 ? max(p, 0) : min(max(p, 0), Skv)));
     }
     hi = min(hi, last);
     if (m.window > 0) lo = max(lo, row - m.window + 1);
